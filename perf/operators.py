@@ -317,11 +317,11 @@ def run_pages(s):
     if own:
         from rai_b200 import paged
         if c["what"] == "fork":
-            table, lens = paged.fork(s["table"], s["lens"], refs, s["parents"])
+            table, lens = paged.fork(s["table"], s["lens"], refs, s["parents"], c["page"])
             short = paged.resize(table, lens, refs, s["k"], s["v"], delta=1)
             return [table, lens, refs, short, s["k"], s["v"]]
         table = s["table"].clone()
-        used = paged.compact(table, refs, s["k"], s["v"])
+        used = paged.compact(table, s["lens"], refs, s["k"], s["v"])
         return [table, refs, used, s["k"], s["v"]]
     if c["what"] == "compact":
         page = torch.arange(refs.numel(), device="cuda")
