@@ -253,7 +253,9 @@ RAI_API int rai_gpu_w4a8_matmul(float* out, const void* packed, const float* inp
 /* Status of the kernel-level calls on the current device (the w4a8 GEMM
  * entries), which return as soon as their kernels are queued: synchronizes
  * `stream`, then returns RAI_ERR_TIMEOUT if one of their bounded device waits
- * gave up since the last query (that call's output is incomplete), else
+ * gave up since the last query (that call's output is incomplete),
+ * RAI_ERR_INVALID if a paged-cache or beam call met a value on the device
+ * (a page number, length, row range or parent) outside its tensors, else
  * RAI_OK. The status word is per device and cleared by the query. */
 RAI_API int rai_gpu_kernel_status(void* stream);
 
@@ -324,6 +326,208 @@ RAI_API int rai_gpu_expf_range(uint32_t first_bits, size_t n, float* out, void* 
  * kernel nodes for the decoder's current configuration; 0 before the first
  * step). */
 RAI_API int rai_gpu_step_kernel_count(const rai_dec* dec, size_t* kernels);
+
+/* ---- paged caches and beam search (device pointers, caller's stream) ----
+ *
+ * rai-infer's KVCache (rai-infer/src/kv_cache.rs:143-304) is one contiguous
+ * window per stream; these entries keep many streams' tokens in pages that
+ * they can share (a prompt common to several streams, the beams of a search)
+ * and run over them what rai_gpu_attention, the RoPE of
+ * rai-infer/src/layers.rs:561-727 and the sampler (rai-infer/src/sampler.rs)
+ * do for one window: no reference counterpart beyond those.
+ *
+ * Token t of sequence s is slot t % page_size of page
+ * table[s * table_stride + t / page_size]. refs[page] counts the table cells
+ * that name a page; 0 means free. Lengths and page numbers live on the
+ * device, so a step needs no host round trip and can be captured in a CUDA
+ * graph; sizes here are upper bounds (max_pages columns of the table,
+ * max_rows rows of a sequence). A value on the device that passes those
+ * bounds is cut to them (a page number outside the pool reads as masked and
+ * is not written) and reported by rai_gpu_kernel_status.
+ *
+ * All calls return as soon as their kernels are queued, allocate nothing and
+ * keep nothing between calls; call them with the stream's device current.
+ * (The first call on a device looks up the status word: make one before
+ * capturing a stream.) Workspaces need no initialisation; calls that may
+ * overlap on the GPU need one each. Addresses and strides: the innermost dimension is contiguous,
+ * every row of a tensor starts on a 16-byte boundary. */
+enum { RAI_F32 = 0, RAI_F16 = 1, RAI_BF16 = 2 };
+
+/* One layer's pages and a ragged chunk of new rows. Sequence s has the rows
+ * q_start[s] .. q_start[s + 1] - 1 of the row tensors, at most max_rows of
+ * them; they are the last of its kv_len[s] tokens, so its row i is the token
+ * at position kv_len[s] - n_s + i. Rows that no sequence has are neither
+ * read nor written. Strides are in elements. */
+typedef struct {
+  void* k;                 /* page p, KV head h, slot t at k + p * k_page + h * k_head + t * k_slot */
+  void* v;
+  int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;
+  const int32_t* table;    /* [n_seqs][max_pages], rows table_stride apart */
+  const int32_t* kv_len;   /* [n_seqs] */
+  const int32_t* q_start;  /* [n_seqs + 1] */
+  int64_t table_stride;
+  uint32_t n_seqs, max_pages, n_pages, page_size, n_kv_heads, head_dim;
+  uint32_t rows;           /* rows of the row tensors */
+  uint32_t max_rows;
+  uint32_t dtype;          /* of the pages */
+} rai_paged_chunk;
+
+/* Causal attention of the chunk's rows over the cache (attention_head_avx2,
+ * rai-infer/src/layers.rs:1266-1380, in another order of summation): row i
+ * of a sequence sees the tokens up to its own position, with window > 0 only
+ * the last `window` of them. scores = scale * q.k, with softcap > 0
+ * softcap * tanh(scale * q.k / softcap). q and out [rows][n_heads][head_dim]
+ * in the pages' dtype; lse (f32 [rows][n_heads], may be NULL) the natural
+ * logarithm of the row's sum of exponentials. A row at a negative position
+ * (kv_len below the row count) sees nothing: its output is 0, its lse
+ * -infinity. What a row may not see does not reach its output, whatever it
+ * holds. head_dim up to 256, a multiple of 16 bytes; n_heads a multiple of
+ * n_kv_heads; scale positive. Scores, softmax sums and outputs are summed in
+ * f32; probabilities are rounded to the pages' type before their product
+ * with V (f32 pages: 22 significant bits). */
+typedef struct {
+  rai_paged_chunk chunk;
+  const void* q;
+  void* out;
+  float* lse;
+  int64_t q_row, q_head, out_row, out_head;
+  uint32_t n_heads, window;
+  float scale, softcap;
+  void* workspace;
+  size_t workspace_bytes;  /* rai_gpu_paged_attention_workspace_bytes */
+} rai_paged_attention;
+RAI_API size_t rai_gpu_paged_attention_workspace_bytes(const rai_paged_attention* args);
+RAI_API int rai_gpu_paged_attention(const rai_paged_attention* args, void* stream);
+
+/* Rotary positions of the chunk's q and k rows and the store of k and v in
+ * the cache's pages. Pair i of a head turns by position * inv_freq[i] (the
+ * angle in 64 bits), its sine and cosine times mscale: (x[i], x[i + rot/2])
+ * (RoPETable::apply, rai-infer/src/layers.rs:689-727), or (x[2i], x[2i + 1])
+ * with interleaved != 0; elements from rot_dim on are copied. q, k, v in
+ * in_dtype; q_out and the pages in the chunk's dtype, rounded once. q_out may
+ * be q itself (same strides and dtype). A row at a negative position stores
+ * nothing and turns by its negative angle. */
+typedef struct {
+  rai_paged_chunk chunk;
+  const void* q;           /* [rows][n_heads][head_dim] */
+  const void* k;           /* [rows][n_kv_heads][head_dim] */
+  const void* v;
+  void* q_out;
+  const float* inv_freq;   /* [rot_dim / 2], device */
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+  uint32_t n_heads, rot_dim, interleaved, in_dtype;
+  float mscale;
+} rai_rope_append;
+RAI_API int rai_gpu_rope_append(const rai_rope_append* args, void* stream);
+
+/* Frequencies for rai_gpu_rope_append (host): inv_freq[i] = theta^(-2i/rot),
+ * rescaled for contexts longer than the trained `original` positions.
+ * RAI_ROPE_LINEAR: / factor. RAI_ROPE_NTK: theta * factor^(rot / (rot - 2)).
+ * RAI_ROPE_LLAMA3: the banded rule of apply_llama3_scaling
+ * (rai-infer/src/layers.rs:760-808) with low / high frequency factors.
+ * RAI_ROPE_YARN: a ramp between pairs that turn more than `high` times
+ * within `original` (kept) and less than `low` times (/ factor), and *mscale
+ * = 0.1 ln(factor) + 1; *mscale is 1 for the others. */
+enum { RAI_ROPE_PLAIN = 0, RAI_ROPE_LINEAR = 1, RAI_ROPE_NTK = 2, RAI_ROPE_LLAMA3 = 3, RAI_ROPE_YARN = 4 };
+RAI_API int rai_rope_frequencies(int kind, uint32_t rot_dim, double theta, double factor, double low, double high,
+                                 double original, float* inv_freq, float* mscale);
+
+/* The sequences of a paged cache: their table, lengths and pages in use. */
+typedef struct {
+  int32_t* table;          /* [n_seqs][max_pages]; cells behind a sequence's length are not read */
+  int32_t* lens;           /* [n_seqs] */
+  int32_t* refs;           /* [n_pages] */
+  int64_t table_stride;
+  uint32_t n_seqs, max_pages, n_pages, page_size;
+} rai_page_table;
+
+/* Every layer's pages of a cache: page p of layer l is page_bytes bytes at
+ * k + l * k_layer + p * k_page (strides in bytes, all multiples of 16). */
+typedef struct {
+  void* k;
+  void* v;
+  int64_t k_layer, k_page, v_layer, v_page;
+  int64_t page_bytes;
+  uint32_t n_layers, n_pages;
+} rai_page_pool;
+
+/* Fork: out sequence i takes the pages of `in` sequence parents[i] (device;
+ * -1: empty). No data moves: refs (shared, in place) of a page become the
+ * number of out cells that name it, so a sequence without children is freed
+ * and one with several is shared, its last page too (rai_gpu_kv_resize then
+ * copies it on write). `out` has its own table and lengths and in's refs;
+ * cells behind a sequence's pages become -1. One parent may be named any
+ * number of times. */
+RAI_API int rai_gpu_kv_fork(const rai_page_table* in, const rai_page_table* out, const int32_t* parents,
+                            void* stream);
+
+/* Resize every sequence in place to new_lens[s] (device), or to its length +
+ * delta when new_lens is NULL (not below 0). First the pages behind the new
+ * end of sequences that shrink are released (their cells become -1; to
+ * length 0 frees the sequence). Then the sequences that grow take the free
+ * pages with the lowest numbers, in sequence order: one for the copy of a
+ * partly filled last page that other cells name too (the last sequence to
+ * grow into a page that only growing ones hold keeps it), then the new ones.
+ * *status (device) = 0, or the number of pages missing: then none of the
+ * growing sequences changes. n_seqs at most 4096. */
+RAI_API size_t rai_gpu_kv_resize_workspace_bytes(uint32_t n_seqs);
+RAI_API int rai_gpu_kv_resize(const rai_page_table* table, const rai_page_pool* pool, const int32_t* new_lens,
+                              int32_t delta, int32_t* status, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* Compact the pool in place: with n pages in use, the i-th of those numbered
+ * n or above moves to the i-th free page below n; tables and refs follow.
+ * *used (device) = n. Every table that names the pool's pages has to be in
+ * the call. */
+RAI_API size_t rai_gpu_kv_compact_workspace_bytes(uint32_t n_pages);
+RAI_API int rai_gpu_kv_compact(const rai_page_table* table, const rai_page_pool* pool, int32_t* used,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* Copy page src[i] to page dst[i] (device) of every layer for i < n. No
+ * destination may be named twice or be a source. */
+RAI_API int rai_gpu_kv_copy_pages(const rai_page_pool* pool, const int32_t* src, const int32_t* dst, size_t n,
+                                  void* stream);
+
+/* Beam search's choice. logits [batch][beams][vocab] (rows row_stride
+ * elements apart, any alignment), scores [batch][beams] f32 the beams' log
+ * probabilities. Candidates (beam, token) are ordered by
+ * scores[beam] + log softmax(logits[beam])[token] in 64 bits, equal ones by
+ * logit, then by beam and token, lowest first. cand_* [batch][keep] the first
+ * `keep`; score / parent / token [batch][beams] the first `beams` of those
+ * whose token is not eos (-1: none is), parent as the sequence number
+ * request * beams + beam, for rai_gpu_kv_fork. Places that nothing fills hold
+ * -infinity and -1. NaN logits and scores count as -infinity; in a row with
+ * +infinity those share the mass, a row of -infinity is uniform (the
+ * degenerate rows of softmax_probabilities, rai-infer/src/speculative.rs).
+ * history (may be NULL): int32 [batch * beams][.] with hist_len tokens a
+ * row; out_history row i becomes its parent's tokens and the new one,
+ * out_len their number (0 without a parent); rows hold hist_cap tokens, a
+ * full one is reported and not extended. Outputs may not overlap inputs.
+ * beams up to 32, keep from beams to 64, beams * vocab below 2^31. */
+typedef struct {
+  const void* logits;
+  const float* scores;
+  int64_t row_stride;
+  float* cand_score;
+  int32_t* cand_beam;
+  int32_t* cand_token;
+  float* score;
+  int32_t* parent;
+  int32_t* token;
+  const int32_t* history;
+  const int32_t* hist_len;
+  int32_t* out_history;
+  int32_t* out_len;
+  int64_t hist_stride, out_hist_stride;
+  uint32_t hist_cap;
+  uint32_t batch, beams, vocab, keep;
+  int32_t eos;
+  uint32_t dtype;          /* of the logits */
+  void* workspace;
+  size_t workspace_bytes;  /* rai_gpu_beam_workspace_bytes */
+} rai_beam_select;
+RAI_API size_t rai_gpu_beam_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t keep);
+RAI_API int rai_gpu_beam_select(const rai_beam_select* args, void* stream);
 
 /* ---- host-side .raimodel writer utilities (no device needed) ----
  *

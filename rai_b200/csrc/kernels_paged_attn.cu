@@ -1,0 +1,822 @@
+// Attention of a ragged chunk of new rows over a paged cache, for few query
+// rows per KV head (decoding, draft verification) and for every type and head
+// size the tcgen05 kernel does not take.
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(s_ij - max_j s_ij),
+//   s_ij = scale q_i . k_j   (or cap tanh(scale q_i . k_j / cap)),
+// over the tokens j that row i sees: j <= pos_i, and j > pos_i - window.
+//
+// The query rows of one KV head (group heads x chunk rows, flattened) form
+// row tiles of MT rows; K and V stream through shared memory in tiles of NT
+// tokens, once per row tile, with the running maximum and sum of the softmax
+// in registers (one pass over the cache). What bounds it is HBM: at 8 chunk
+// rows x 4 heads a byte of K and V gets 32 multiply-adds, a few percent of
+// the tensor rate, so mma.sync from registers carries it.
+//
+// Work split: all (sequence, row tile, KV head) items' token tiles form one
+// line of W tiles, cut into equal ranges, one per resident CTA, so ragged
+// lengths and few long sequences fill the machine alike. An item cut between
+// CTAs leaves partial sums (m, l, unnormalized o in f32) in the workspace;
+// paged_combine_kernel joins them in CTA order (the same bits every run).
+//
+// 16-bit types: products of 16-bit operands in f32 (m16n8k16); P is rounded
+// to the operand type (relative 2^-9 bf16, 2^-12 f16, about the rounding of
+// the 16-bit output itself), its sum is taken before the rounding. f16
+// probabilities carry a factor 2^10 so that small ones stay normal.
+// f32: each operand is split in two tf32 halves and the three products that
+// matter are summed in f32 (2^-21 relative per product).
+//
+// Masked places never reach a result: scores are replaced, not biased; token
+// slots outside a row tile's visible range are not loaded (zero filled); and
+// a V value that is not finite in a tile where some row may not see it is
+// replaced by zero and added back to the rows that do see it at the end.
+#include <cuda_runtime.h>
+
+#include <mutex>
+
+#include "paged.h"
+
+namespace rai {
+
+cudaError_t paged_attention_tc(const AttnArgs& a, cudaStream_t s, bool* taken);
+
+namespace {
+
+constexpr int kThreads = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <int DT_, int HD_, int MT_>
+struct Cfg {
+  static constexpr int DT = DT_, HD = HD_, MT = MT_;
+  static constexpr int kElt = DT == kF32 ? 4 : 2;
+  static constexpr int kRowB = HD * kElt;
+  static constexpr int NT = DT == kF32 && HD >= 128 ? 32 : 64;
+  static constexpr int kTileB = NT * kRowB;
+  static constexpr int kStages = HD == 256 ? 2 : HD == 128 ? 3 : 4;
+  static constexpr int WM = MT / 16, WN = 4 / WM, NTW = NT / WN;
+  static constexpr bool kQReg = DT != kF32 && HD <= 128;  // query fragments stay in registers
+  static constexpr int kQB = kQReg ? 0 : MT * kRowB;
+  static constexpr int kMergeB = WN > 1 ? 2 * 16 * (HD + 4) * 4 + 4 * 16 * 8 : 0;
+  static constexpr int kSmem = kStages * 2 * kTileB + kQB + kMergeB + 128;
+  static constexpr int kPartFloats = MT * (HD + 2);
+  static constexpr float kPShift = DT == kF16 ? 10.f : 0.f;
+};
+
+struct Params {
+  AttnArgs a;
+  int row_tiles, min_tiles, grid;
+  bool whole;  // items are short: none is cut
+  float c;  // log2(e) * scale, or log2(e) when the scores are capped
+  FastDiv row_tiles_div, group_div;
+};
+
+struct Item {
+  int seq, start, n, len;  // rows and length of the sequence
+  int f0, nf;              // flattened rows of the row tile
+  int lo, hi;              // tokens that some row of the tile sees
+  int first, tiles;        // token tiles
+};
+
+template <int MT, int NT>
+__device__ __forceinline__ Item item_of(const Params& p, int unit) {
+  Item it;
+  it.seq = p.row_tiles_div.quot(unit);
+  const int rt = unit - it.seq * p.row_tiles;
+  const SeqRows r = seq_rows(p.a.c, it.seq);
+  it.start = r.start, it.n = r.n, it.len = r.len;
+  it.f0 = rt * MT;
+  it.nf = min(MT, r.n * p.a.group - it.f0);
+  it.lo = it.hi = it.first = it.tiles = 0;
+  if (it.nf <= 0) return it;
+  const int p0 = r.len - r.n;
+  it.hi = p0 + (int)p.group_div.quot(it.f0 + it.nf - 1) + 1;
+  const int plo = p0 + (int)p.group_div.quot(it.f0);
+  if (p.a.window > 0) it.lo = max(0, plo - p.a.window + 1);
+  it.tiles = 1;
+  if (it.hi <= 0) {
+    it.lo = it.hi = 0;
+  } else {
+    it.first = it.lo / NT;
+    it.tiles = (it.hi + NT - 1) / NT - it.first;
+  }
+  return it;
+}
+
+// The CTA's range [begin, end) of the line of tiles and the unit it starts
+// in. Every thread sums a run of units; a block scan places the runs. With
+// p.whole the cuts move down to the starts of the items they fall in.
+struct Range {
+  long long total, per, begin, end;
+  int unit;          // unit of `begin`
+  long long before;  // tiles of one KV head before it
+};
+template <int MT, int NT>
+__device__ __forceinline__ Range plan(const Params& p, long long cta, long long* sh) {
+  const int units = p.a.c.n_seqs * p.row_tiles;
+  const int per = (units + kThreads - 1) / kThreads;
+  const int u0 = min(units, (int)threadIdx.x * per), u1 = min(units, u0 + per);
+  long long own = 0;
+  for (int u = u0; u < u1; ++u) own += item_of<MT, NT>(p, u).tiles;
+  long long incl = own;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(~0u, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sh[warp] = incl;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) incl += sh[w];
+    total += sh[w];
+  }
+  Range r;
+  const int nkv = p.a.c.nkv;
+  r.total = total * nkv;
+  r.per = max((r.total + p.grid - 1) / p.grid, (long long)p.min_tiles);
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const long long at = min((cta + side) * r.per, r.total);
+    long long excl = incl - own;
+    if (at == r.total) {
+      if (threadIdx.x == 0) sh[4 + 3 * side] = at;
+    } else if (own && at >= excl * nkv && at < incl * nkv) {
+      int u = u0, t;
+      for (;; ++u) {
+        t = item_of<MT, NT>(p, u).tiles;
+        if (at < (excl + t) * nkv) break;
+        excl += t;
+      }
+      sh[4 + 3 * side] = p.whole ? at - (at - excl * nkv) % t : at;
+      sh[5 + 3 * side] = u;
+      sh[6 + 3 * side] = excl;
+    }
+  }
+  __syncthreads();
+  r.begin = sh[4];
+  r.unit = (int)sh[5];
+  r.before = sh[6];
+  r.end = sh[7];
+  return r;
+}
+
+// Walks the line of tiles.
+template <int MT, int NT>
+struct Cursor {
+  Item it;
+  int unit, head, tile;
+  __device__ __forceinline__ void seek(const Params& p, const Range& r, long long at) {
+    unit = r.unit;
+    it = item_of<MT, NT>(p, unit);
+    const long long in = at - r.before * p.a.c.nkv;
+    head = (int)(in / it.tiles);
+    tile = (int)(in - (long long)head * it.tiles);
+  }
+  __device__ __forceinline__ void next(const Params& p) {
+    if (++tile < it.tiles) return;
+    tile = 0;
+    if (++head < p.a.c.nkv) return;
+    head = 0;
+    const int units = p.a.c.n_seqs * p.row_tiles;
+    do {
+      if (++unit >= units) return;
+      it = item_of<MT, NT>(p, unit);
+    } while (it.tiles == 0);
+  }
+};
+
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+
+template <typename C>
+__device__ __forceinline__ uint32_t swz(int row, int chunk) {  // 16-byte chunk of a row, conflict free by rows of 8
+  return (uint32_t)row * C::kRowB + (uint32_t)((chunk ^ (row & 7)) << 4);
+}
+
+template <typename C>
+__device__ __forceinline__ void load_tile(const Params& p, const Cursor<C::MT, C::NT>& cur, uint32_t sk, uint32_t sv) {
+  constexpr int kChunks = C::kRowB / 16;  // per row
+  constexpr int kRowsPer = kThreads / kChunks;
+  const PagedChunk& c = p.a.c;
+  const int chunk = threadIdx.x % kChunks, r0 = threadIdx.x / kChunks;
+  const int t0 = (cur.it.first + cur.tile) * C::NT;
+  const bool in_head = chunk * 16 < c.hd * C::kElt;
+  const char* k = static_cast<const char*>(c.k) + (long long)cur.head * c.k_head * C::kElt + chunk * 16;
+  const char* v = static_cast<const char*>(c.v) + (long long)cur.head * c.v_head * C::kElt + chunk * 16;
+#pragma unroll
+  for (int i = 0; i < C::NT / kRowsPer; ++i) {
+    const int row = r0 + i * kRowsPer, t = t0 + row;
+    bool real = t >= cur.it.lo && t < cur.it.hi;
+    long long ko = 0, vo = 0;
+    if (real) {
+      const int pi = (int)c.page.quot(t);
+      const int page = page_of(c, cur.it.seq, pi), slot = t - pi * (int)c.page.d;
+      real = page >= 0 && in_head;
+      if (real) {
+        ko = (page * c.k_page + slot * c.k_slot) * C::kElt;
+        vo = (page * c.v_page + slot * c.v_slot) * C::kElt;
+      }
+    }
+    const uint32_t o = swz<C>(row, chunk);
+    cp_async16_or_zero(sk + o, real ? k + ko : k, real);
+    cp_async16_or_zero(sv + o, real ? v + vo : v, real);
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (DT == kBF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo with both in tf32, hi rounded to nearest (lo is exact before
+// its own rounding). A value that is not finite stays whole in hi.
+__device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  const float rest = x - __uint_as_float(hi);
+  const float r = fabsf(rest) <= 3.4e38f ? rest : 0.f;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(r));
+}
+// d += a b of f32 operands: the small products first.
+__device__ __forceinline__ void mma8x3(float (&d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], float b0, float b1) {
+  uint32_t h0, l0, h1, l1;
+  split(b0, h0, l0);
+  split(b1, h1, l1);
+  mma8(d, al, h0, h1);
+  mma8(d, ah, l0, l1);
+  mma8(d, ah, h0, h1);
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ float lds_f32(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+  if constexpr (DT == kBF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+template <int DT>
+__device__ __forceinline__ float value(const void* base, long long i) {
+  if constexpr (DT == kF32) return static_cast<const float*>(base)[i];
+  else if constexpr (DT == kF16) return __half2float(static_cast<const __half*>(base)[i]);
+  else return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i]);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ float capped(float s, float scale, float cap) {
+  const float x = __fdividef(s * scale, cap);
+  if constexpr (DT == kF32) {
+    return cap * tanhf(x);
+  } else {
+    // tanh x = 1 - 2 / (1 + e^2x): a few 2^-23 of the cap, far below the
+    // 2^-9 that a probability is rounded to.
+    return cap * (1.f - __fdividef(2.f, 1.f + exp2_fast(2.f * kLog2e * x)));
+  }
+}
+// The elements of a 32-bit word that are not finite, replaced by zero.
+template <int DT>
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
+  if constexpr (DT == kF32) {
+    return (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
+  } else {
+    constexpr uint32_t e = DT == kBF16 ? 0x7f80u : 0x7c00u;
+    if ((w & e) == e) w &= 0xffff0000u;
+    if ((w >> 16 & e) == e) w &= 0x0000ffffu;
+    return w;
+  }
+}
+
+template <typename C>
+__global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_constant__ Params p) {
+  constexpr int DT = C::DT, HD = C::HD, MT = C::MT, NT = C::NT, WN = C::WN, NTW = C::NTW, S = C::kStages;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  __shared__ long long sh[10];
+  const uint32_t base = (smem_u32(smem_raw) + 127) & ~127u;
+  const uint32_t sq = base + S * 2 * C::kTileB;
+  float* merge = reinterpret_cast<float*>(smem_raw + (sq + C::kQB - smem_u32(smem_raw)));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int wm = warp % C::WM, wn = warp / C::WM;
+  const int g = lane >> 2, t4 = lane & 3;
+  const PagedChunk& ch = p.a.c;
+
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const Range rg = plan<MT, NT>(p, blockIdx.x, sh);
+  const long long begin = rg.begin, end = rg.end;
+  if (begin >= end) return;
+
+  Cursor<MT, NT> ld, cur;
+  ld.seek(p, rg, begin);
+  cur = ld;
+  long long loaded = begin;
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) {
+    if (loaded < end) {
+      load_tile<C>(p, ld, base + s * 2 * C::kTileB, base + s * 2 * C::kTileB + C::kTileB);
+      ++loaded;
+      ld.next(p);
+    }
+    cp_async_commit();
+  }
+
+  uint32_t qf[C::kQReg ? HD / 16 : 1][4];
+  float acc[HD / 8][4];
+  float m[2], l[2];
+  int pos[2];  // position of the thread's two rows, below 0: none
+  bool poison = false, fresh = true;
+  int first_slot = 0;  // of the workspace: 0 for the CTA's first item, 1 for its last
+  for (long long at = begin; at < end; ++at) {
+    const Item& it = cur.it;
+    if (fresh) {
+      // The item's rows: query fragments, positions, empty sums.
+      const int p0 = it.len - it.n;
+      const void* q = p.a.q;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = wm * 16 + g + 8 * h;
+        const int f = it.f0 + r, i = (int)p.group_div.quot(f), j = f - i * p.a.group;
+        const bool real = r < it.nf;
+        pos[h] = real ? p0 + i : -1;
+        if constexpr (C::kQReg) {
+          const long long o = (long long)(it.start + i) * p.a.q_row + (long long)(cur.head * p.a.group + j) * p.a.q_head;
+          const uint16_t* row = static_cast<const uint16_t*>(q) + o;
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int col = kk * 16 + e * 8 + 2 * t4;
+              qf[kk][2 * e + h] = real && col < ch.hd ? *reinterpret_cast<const uint32_t*>(row + col) : 0u;
+            }
+        }
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+      }
+      if constexpr (!C::kQReg) {
+        __syncthreads();  // the last item's reads of the query tile are over
+        constexpr int kChunks = C::kRowB / 16;
+        for (int x = threadIdx.x; x < MT * kChunks; x += kThreads) {
+          const int r = x / kChunks, chunk = x % kChunks;
+          const int f = it.f0 + r, i = (int)p.group_div.quot(f), j = f - i * p.a.group;
+          const bool real = r < it.nf && chunk * 16 < ch.hd * C::kElt;
+          const long long o = (long long)(it.start + i) * p.a.q_row + (long long)(cur.head * p.a.group + j) * p.a.q_head;
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (real) w = *reinterpret_cast<const uint4*>(static_cast<const char*>(q) + o * C::kElt + chunk * 16);
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(sq + swz<C>(r, chunk)), "r"(w.x), "r"(w.y),
+                       "r"(w.z), "r"(w.w)
+                       : "memory");
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < HD / 8; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) acc[x][y] = 0.f;
+      poison = false;
+      fresh = false;
+    }
+    cp_async_wait<S - 2>();
+    __syncthreads();
+    // The stage that the last step read is free: fetch ahead.
+    if (loaded < end) {
+      const uint32_t st = base + (uint32_t)((loaded - begin) % S) * 2 * C::kTileB;
+      load_tile<C>(p, ld, st, st + C::kTileB);
+      ++loaded;
+      ld.next(p);
+    }
+    cp_async_commit();
+    const uint32_t sk = base + (uint32_t)((at - begin) % S) * 2 * C::kTileB, sv = sk + C::kTileB;
+    const int t0 = (it.first + cur.tile) * NT;
+    const int p0 = it.len - it.n;
+    const int plo = p0 + (int)p.group_div.quot(it.f0), phi = it.hi - 1;
+    const bool masked = t0 + NT - 1 > plo || t0 < it.lo || (p.a.window > 0 && t0 <= phi - p.a.window);
+
+    if (masked) {
+      // V values that are not finite, where a row may not see them.
+      bool bad = false;
+#pragma unroll 4
+      for (int x = threadIdx.x; x < C::kTileB / 16; x += kThreads) {
+        const uint32_t ad = sv + x * 16;
+        uint4 w;
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(ad));
+        const uint4 f = make_uint4(finite_or_zero<DT>(w.x), finite_or_zero<DT>(w.y), finite_or_zero<DT>(w.z),
+                                   finite_or_zero<DT>(w.w));
+        if (f.x != w.x || f.y != w.y || f.z != w.z || f.w != w.w) {
+          bad = true;
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(ad), "r"(f.x), "r"(f.y), "r"(f.z), "r"(f.w)
+                       : "memory");
+        }
+      }
+      if (__syncthreads_or(bad)) poison = true;
+    }
+
+    // ---- S = Q K^T over this warp's tokens ----
+    float s[NTW / 8][4];
+#pragma unroll
+    for (int x = 0; x < NTW / 8; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) s[x][y] = 0.f;
+    const int w0 = wn * NTW;  // first token of the warp in the tile
+    if constexpr (DT != kF32) {
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        uint32_t a[4];
+        if constexpr (C::kQReg) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[e] = qf[kk][e];
+        } else {
+          ldsm4(a, sq + swz<C>(wm * 16 + (lane & 15), kk * 2 + (lane >> 4)));
+        }
+#pragma unroll
+        for (int x = 0; x < NTW / 16; ++x) {
+          uint32_t b[4];
+          ldsm4(b, sk + swz<C>(w0 + x * 16 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
+          mma16<DT>(s[2 * x], a, b[0], b[1]);
+          mma16<DT>(s[2 * x + 1], a, b[2], b[3]);
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (int kk = 0; kk < HD / 8; ++kk) {
+        uint32_t ah[4], al[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          split(lds_f32(sq + swz<C>(wm * 16 + g + 8 * (e & 1), kk * 2 + (e >> 1)) + 4 * t4), ah[e], al[e]);
+#pragma unroll
+        for (int x = 0; x < NTW / 8; ++x) {
+          const int tk = w0 + x * 8 + g;
+          mma8x3(s[x], ah, al, lds_f32(sk + swz<C>(tk, kk * 2) + 4 * t4), lds_f32(sk + swz<C>(tk, kk * 2 + 1) + 4 * t4));
+        }
+      }
+    }
+    if (p.a.softcap > 0.f) {
+#pragma unroll
+      for (int x = 0; x < NTW / 8; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) s[x][y] = capped<DT>(s[x][y], p.a.scale, p.a.softcap);
+    }
+    if (masked) {
+#pragma unroll
+      for (int x = 0; x < NTW / 8; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int t = t0 + w0 + x * 8 + 2 * t4 + (y & 1), pr = pos[y >> 1];
+          const bool seen = t <= pr && t >= it.lo && (p.a.window <= 0 || t > pr - p.a.window);
+          if (!seen) s[x][y] = -INFINITY;
+        }
+    }
+    // ---- running softmax ----
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float top = m[h];
+#pragma unroll
+      for (int x = 0; x < NTW / 8; ++x) top = fmaxf(top, fmaxf(s[x][2 * h], s[x][2 * h + 1]));
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+      const float mc = top == -INFINITY ? 0.f : top * p.c;
+      const float fix = exp2_fast(m[h] * p.c - mc);  // m = -inf: 0
+      m[h] = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < NTW / 8; ++x)
+#pragma unroll
+        for (int y = 2 * h; y < 2 * h + 2; ++y) {
+          s[x][y] = exp2_fast(fmaf(s[x][y], p.c, C::kPShift - mc));
+          sum += s[x][y];
+        }
+      l[h] = l[h] * fix + sum;
+#pragma unroll
+      for (int x = 0; x < HD / 8; ++x) {
+        acc[x][2 * h] *= fix;
+        acc[x][2 * h + 1] *= fix;
+      }
+    }
+    // ---- O += P V ----
+    if constexpr (DT != kF32) {
+#pragma unroll
+      for (int kk = 0; kk < NTW / 16; ++kk) {
+        const uint32_t a[4] = {pack<DT>(s[2 * kk][0], s[2 * kk][1]), pack<DT>(s[2 * kk][2], s[2 * kk][3]),
+                               pack<DT>(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack<DT>(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+        for (int x = 0; x < HD / 16; ++x) {
+          uint32_t b[4];
+          ldsm4t(b, sv + swz<C>(w0 + kk * 16 + (lane & 15), x * 2 + (lane >> 4)));
+          mma16<DT>(acc[2 * x], a, b[0], b[1]);
+          mma16<DT>(acc[2 * x + 1], a, b[2], b[3]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int kk = 0; kk < NTW / 8; ++kk) {
+        // Column k of A is token 2k (k < 4) or 2 (k - 4) + 1, as the scores lie.
+        uint32_t ah[4], al[4];
+        split(s[kk][0], ah[0], al[0]);
+        split(s[kk][2], ah[1], al[1]);
+        split(s[kk][1], ah[2], al[2]);
+        split(s[kk][3], ah[3], al[3]);
+        const int tk = w0 + kk * 8 + 2 * t4;
+#pragma unroll
+        for (int x = 0; x < HD / 8; ++x) {
+          const int chunk = x * 2 + (g >> 2), off = 4 * (g & 3);
+          mma8x3(acc[x], ah, al, lds_f32(sv + swz<C>(tk, chunk) + off), lds_f32(sv + swz<C>(tk + 1, chunk) + off));
+        }
+      }
+    }
+
+    // ---- end of the item, or of this CTA's part of it ----
+    if (cur.tile + 1 == it.tiles || at + 1 == end) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(~0u, l[h], 1);
+        l[h] += __shfl_xor_sync(~0u, l[h], 2);
+      }
+      if constexpr (WN > 1) {
+        // Join the warps that took different tokens of the same rows.
+        float* ml = merge + 2 * 16 * (HD + 4);  // [warp][16] (m, l)
+        __syncthreads();
+        if (t4 == 0)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) *reinterpret_cast<float2*>(ml + (warp * 16 + g + 8 * h) * 2) = make_float2(m[h], l[h]);
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float2 w[WN];
+          float top = -INFINITY;
+#pragma unroll
+          for (int x = 0; x < WN; ++x) {
+            w[x] = *reinterpret_cast<const float2*>(ml + ((wm + x * C::WM) * 16 + g + 8 * h) * 2);
+            top = fmaxf(top, w[x].x);
+          }
+          const float mc = top == -INFINITY ? 0.f : top * p.c;
+          float sum = 0.f;
+#pragma unroll
+          for (int x = 0; x < WN; ++x) sum += w[x].y * exp2_fast(w[x].x * p.c - mc);
+          const float fix = exp2_fast(m[h] * p.c - mc);
+          m[h] = top;
+          l[h] = sum;
+#pragma unroll
+          for (int x = 0; x < HD / 8; ++x) {
+            acc[x][2 * h] *= fix;
+            acc[x][2 * h + 1] *= fix;
+          }
+        }
+#pragma unroll
+        for (int half = WN / 2; half >= 1; half >>= 1) {
+          float* buf = merge + ((wn % half) * C::WM + wm) * 16 * (HD + 4);
+          if (wn >= half && wn < 2 * half)
+#pragma unroll
+            for (int x = 0; x < HD / 8; ++x)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<float2*>(buf + (g + 8 * h) * (HD + 4) + x * 8 + 2 * t4) =
+                    make_float2(acc[x][2 * h], acc[x][2 * h + 1]);
+          __syncthreads();
+          if (wn < half)
+#pragma unroll
+            for (int x = 0; x < HD / 8; ++x)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float2 o = *reinterpret_cast<const float2*>(buf + (g + 8 * h) * (HD + 4) + x * 8 + 2 * t4);
+                acc[x][2 * h] += o.x;
+                acc[x][2 * h + 1] += o.y;
+              }
+          __syncthreads();
+        }
+      }
+      if (wn == 0) {
+        const long long item_at = at - cur.tile;  // where the item begins on the line
+        if (poison) {
+          // Rows that see a V value which is not finite get it after all.
+          const int ta = it.first * NT + (int)max(0ll, begin - item_at) * NT, tb = (it.first + cur.tile + 1) * NT;
+          for (int t = max(ta, it.lo); t < min(tb, it.hi); ++t) {
+            const int tt = t / NT * NT;
+            if (!(tt + NT - 1 > plo || tt < it.lo || (p.a.window > 0 && tt <= phi - p.a.window))) continue;
+            const int pi = (int)ch.page.quot(t), page = page_of(ch, it.seq, pi);
+            if (page < 0) continue;
+            const long long vo = page * ch.v_page + (long long)cur.head * ch.v_head + (t - pi * (int)ch.page.d) * ch.v_slot;
+            for (int h = 0; h < 2; ++h) {
+              if (t > pos[h] || (p.a.window > 0 && t <= pos[h] - p.a.window)) continue;
+#pragma unroll
+              for (int x = 0; x < HD / 8; ++x)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int col = x * 8 + 2 * t4 + e;
+                  const float v = col < ch.hd ? value<DT>(ch.v, vo + col) : 0.f;
+                  if (!(fabsf(v) <= 3.4028235e38f)) acc[x][2 * h + e] += v;
+                }
+            }
+          }
+        }
+        const bool whole = item_at >= begin && cur.tile + 1 == it.tiles;
+        if (whole) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = wm * 16 + g + 8 * h;
+            if (r >= it.nf) continue;
+            const int f = it.f0 + r, i = (int)p.group_div.quot(f), j = f - i * p.a.group, head = cur.head * p.a.group + j;
+            const float inv = l[h] > 0.f || l[h] != l[h] ? 1.f / l[h] : 0.f;
+            const long long o = (long long)(it.start + i) * p.a.o_row + (long long)head * p.a.o_head;
+#pragma unroll
+            for (int x = 0; x < HD / 8; ++x) {
+              const int col = x * 8 + 2 * t4;
+              if (col >= ch.hd) continue;
+              const float a0 = acc[x][2 * h] * inv, a1 = acc[x][2 * h + 1] * inv;
+              if constexpr (DT == kF32)
+                *reinterpret_cast<float2*>(static_cast<float*>(p.a.out) + o + col) = make_float2(a0, a1);
+              else
+                *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.a.out) + o + col) = pack<DT>(a0, a1);
+            }
+            if (p.a.lse && t4 == 0)
+              p.a.lse[(long long)(it.start + i) * (ch.nkv * p.a.group) + head] =
+                  l[h] > 0.f || l[h] != l[h] ? (m[h] * p.c - C::kPShift) * kLn2 + logf(l[h]) : -INFINITY;
+          }
+        } else {
+          float* part = p.a.part + (2ll * blockIdx.x + first_slot) * C::kPartFloats;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = wm * 16 + g + 8 * h;
+#pragma unroll
+            for (int x = 0; x < HD / 8; ++x)
+              *reinterpret_cast<float2*>(part + r * HD + x * 8 + 2 * t4) = make_float2(acc[x][2 * h], acc[x][2 * h + 1]);
+            if (t4 == 0) {
+              part[MT * HD + r] = m[h] == -INFINITY ? -INFINITY : m[h] * p.c;
+              part[MT * HD + MT + r] = l[h];
+            }
+          }
+        }
+      }
+      first_slot = 1;
+      fresh = true;
+    }
+    cur.next(p);
+  }
+  cp_async_wait<0>();
+}
+
+// Joins the parts of items that the cut between CTAs b - 1 and b goes
+// through first (b = blockIdx.x + 1), four rows of the tile per CTA.
+template <typename C>
+__global__ void __launch_bounds__(kThreads) paged_combine_kernel(const __grid_constant__ Params p) {
+  constexpr int HD = C::HD, MT = C::MT, NT = C::NT;
+  __shared__ long long sh[10];
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const int b = blockIdx.x + 1;
+  const Range rg = plan<MT, NT>(p, b, sh);
+  const long long at = rg.begin;
+  if (at >= rg.total) return;
+  Cursor<MT, NT> cur;
+  cur.seek(p, rg, at);
+  const long long start = at - cur.tile, stop = start + cur.it.tiles;
+  if (start == at || start < at - rg.per) return;  // not cut here, or cut before
+  const int last = (int)((stop - 1) / rg.per);     // parts: CTAs b - 1 .. last
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.y * 4 + warp;
+  if (r >= cur.it.nf) return;
+  auto part = [&](int cta) {
+    const bool head = cta >= b || start == (long long)cta * rg.per;  // the CTA's first item
+    return p.a.part + (2ll * cta + (head ? 0 : 1)) * C::kPartFloats;
+  };
+  float top = -INFINITY;
+  for (int cta = b - 1 + lane; cta <= last; cta += 32) top = fmaxf(top, part(cta)[MT * HD + r]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  const float mc = top == -INFINITY ? 0.f : top;
+  constexpr int PL = HD / 32;  // columns per lane
+  float acc[PL] = {}, l = 0.f;
+  for (int cta = b - 1; cta <= last; ++cta) {
+    const float* x = part(cta);
+    const float w = exp2_fast(x[MT * HD + r] - mc);
+    l += x[MT * HD + MT + r] * w;
+    if (w != 0.f)  // a part of which the row sees nothing
+#pragma unroll
+      for (int e = 0; e < PL / 2; ++e) {
+        const float2 v = *reinterpret_cast<const float2*>(x + r * HD + e * 64 + lane * 2);
+        acc[2 * e] += v.x * w;
+        acc[2 * e + 1] += v.y * w;
+      }
+  }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const int f = cur.it.f0 + r, i = (int)p.group_div.quot(f), head = cur.head * p.a.group + f - i * p.a.group;
+  const long long o = (long long)(cur.it.start + i) * p.a.o_row + (long long)head * p.a.o_head;
+#pragma unroll
+  for (int e = 0; e < PL / 2; ++e) {
+    const int col = e * 64 + lane * 2;
+    if (col >= p.a.c.hd) continue;
+    if constexpr (C::DT == kF32)
+      *reinterpret_cast<float2*>(static_cast<float*>(p.a.out) + o + col) = make_float2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    else
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.a.out) + o + col) =
+          pack<C::DT>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  }
+  if (p.a.lse && lane == 0)
+    p.a.lse[(long long)(cur.it.start + i) * (p.a.c.nkv * p.a.group) + head] =
+        l > 0.f || l != l ? (mc - C::kPShift) * kLn2 + logf(l) : -INFINITY;
+}
+
+template <typename C>
+int resident_ctas() {
+  // Per SM, from shared memory: 228 KB with 1 KB kept for each CTA. (The
+  // registers of 128 threads allow at least three.)
+  const int n = (228 * 1024) / (C::kSmem + 1024 + 512);
+  return n < 1 ? 1 : n > 3 ? 3 : n;
+}
+
+template <typename F>
+auto with_cfg(int dtype, int hd, int rows, F f) {
+#define RAI_MT(DT, HD)                            \
+  (rows <= 16   ? f(Cfg<DT, HD, 16>{})            \
+   : rows <= 32 ? f(Cfg<DT, HD, 32>{})            \
+                : f(Cfg<DT, HD, 64>{}))
+#define RAI_HD(DT) (hd <= 64 ? RAI_MT(DT, 64) : hd <= 128 ? RAI_MT(DT, 128) : RAI_MT(DT, 256))
+  return dtype == kF32 ? RAI_HD(kF32) : dtype == kF16 ? RAI_HD(kF16) : RAI_HD(kBF16);
+#undef RAI_HD
+#undef RAI_MT
+}
+
+// Least tiles of a CTA's range: a cut costs a partial result (a few KB) and
+// its share of the joining kernel.
+constexpr int kMinTiles = 4;
+// Caches of at most this many tiles a sequence are not cut.
+constexpr int kWholeTiles = 8;
+
+template <typename C>
+cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
+  static std::once_flag once[64];
+  static cudaError_t ready[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::call_once(once[dev], [&] {
+    ready[dev] = cudaFuncSetAttribute(paged_attn_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  });
+  if (ready[dev] != cudaSuccess) return ready[dev];
+  Params p;
+  p.a = a;
+  const long long frows = (long long)a.c.max_rows * a.group;
+  p.row_tiles = (int)((frows + C::MT - 1) / C::MT);
+  p.row_tiles_div = FastDiv(p.row_tiles);
+  p.group_div = FastDiv(a.group);
+  p.whole = ((long long)a.c.max_pages * a.c.page.d + C::NT - 1) / C::NT <= kWholeTiles;
+  p.min_tiles = p.whole ? 1 : kMinTiles;
+  p.grid = device_sm_count() * resident_ctas<C>();
+  p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
+  e = launch_pdl(paged_attn_kernel<C>, dim3(p.grid), dim3(kThreads), C::kSmem, s, p);
+  if (e != cudaSuccess || p.whole) return e;
+  return launch_pdl(paged_combine_kernel<C>, dim3(p.grid - 1, C::MT / 4), dim3(kThreads), 0, s, p);
+}
+
+}  // namespace
+
+size_t paged_attention_workspace(const AttnArgs& a) {
+  const long long frows = (long long)a.c.max_rows * a.group;
+  return with_cfg(a.dtype, a.c.hd, (int)(frows < 64 ? frows : 64), [&](auto c) -> size_t {
+    using C = decltype(c);
+    return 2ull * device_sm_count() * resident_ctas<C>() * C::kPartFloats * 4;
+  });
+}
+
+cudaError_t paged_attention(const AttnArgs& a, cudaStream_t s) {
+  const long long frows = (long long)a.c.max_rows * a.group;
+  return with_cfg(a.dtype, a.c.hd, (int)(frows < 64 ? frows : 64), [&](auto c) { return launch<decltype(c)>(a, s); });
+}
+
+}  // namespace rai

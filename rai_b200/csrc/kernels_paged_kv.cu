@@ -1,0 +1,536 @@
+// Filling and keeping a paged cache: rotary positions with the store of k and
+// v, and the page operations (fork, resize with copy on write, compact, copy).
+#include <cuda_runtime.h>
+
+#include "paged.h"
+
+namespace rai {
+
+namespace {
+
+// ---------------------------------------------------------------- elements
+
+template <int DT>
+struct Elt;
+template <>
+struct Elt<kF32> {
+  using T = float;
+  static __device__ __forceinline__ float get(T x) { return x; }
+  static __device__ __forceinline__ T put(float x) { return x; }
+};
+template <>
+struct Elt<kF16> {
+  using T = __half;
+  static __device__ __forceinline__ float get(T x) { return __half2float(x); }
+  static __device__ __forceinline__ T put(float x) { return __float2half_rn(x); }
+};
+template <>
+struct Elt<kBF16> {
+  using T = __nv_bfloat16;
+  static __device__ __forceinline__ float get(T x) { return __bfloat162float(x); }
+  static __device__ __forceinline__ T put(float x) { return __float2bfloat16_rn(x); }
+};
+
+// N elements as 16-byte (or, for the narrower of two types, shorter) vectors.
+template <int DT, int N>
+__device__ __forceinline__ void load_n(const typename Elt<DT>::T* p, float (&x)[N]) {
+  using T = typename Elt<DT>::T;
+  constexpr int kB = N * sizeof(T);
+  alignas(16) T v[N];
+  if constexpr (kB % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < kB / 16; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+    static_assert(kB == 8, "vector width");
+    reinterpret_cast<uint2*>(v)[0] = reinterpret_cast<const uint2*>(p)[0];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = Elt<DT>::get(v[i]);
+}
+template <int DT, int N>
+__device__ __forceinline__ void store_n(typename Elt<DT>::T* p, const float (&x)[N]) {
+  using T = typename Elt<DT>::T;
+  constexpr int kB = N * sizeof(T);
+  alignas(16) T v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = Elt<DT>::put(x[i]);
+  if constexpr (kB % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < kB / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
+  } else {
+    static_assert(kB == 8, "vector width");
+    reinterpret_cast<uint2*>(p)[0] = reinterpret_cast<const uint2*>(v)[0];
+  }
+}
+
+// cos and sin of pos * inv_freq. The product and its reduction by whole
+// turns are in 64 bits (a far position times a frequency has more than 24
+// significant bits above the point); what is left, within half a turn, has a
+// 32-bit sine and cosine.
+__device__ __forceinline__ void turn_of(int pos, float inv_freq, float mscale, float* c, float* s) {
+  const double a = (double)pos * (double)inv_freq;
+  const double n = rint(a * 0.15915494309189533577);
+  // 2 pi as a double and the rest of it.
+  const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.28318530717958647693, a));
+  float sv, cv;
+  sincosf((float)r, &sv, &cv);
+  *c = cv * mscale;
+  *s = sv * mscale;
+}
+
+constexpr int kRopeThreads = 256;
+
+// One CTA per chunk row (looping): the row's angles go to shared memory, then
+// threads take vectors of kV elements of every q, k and v head; a half-split
+// pair's two vectors are one thread's work, so a rotation in place is safe.
+// Bound: HBM, each element read and written once.
+template <int IN, int OUT>
+__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const __grid_constant__ RopeArgs a) {
+  using TI = typename Elt<IN>::T;
+  using TO = typename Elt<OUT>::T;
+  constexpr int kV = IN == kF32 && OUT == kF32 ? 4 : 8;
+  __shared__ float cs[128], sn[128];
+  const PagedChunk& ch = a.c;
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const int half = a.rot / 2;
+  for (int row = blockIdx.x; row < ch.rows; row += gridDim.x) {
+    // The sequence of the row: the last with q_start <= row.
+    int lo = 0, hi = ch.n_seqs;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (ch.q_start[mid] <= row) lo = mid; else hi = mid;
+    }
+    const SeqRows r = seq_rows(ch, lo);
+    if (row < r.start || row >= r.start + r.n) continue;  // behind the last sequence (or before the first)
+    const int pos = r.len - r.n + (row - r.start);
+    __syncthreads();
+    for (int i = threadIdx.x; i < half; i += kRopeThreads)
+      turn_of(pos, a.inv_freq[i], a.mscale, &cs[i], &sn[i]);
+    int page = -1, slot = 0;
+    if (pos >= 0) {
+      const int pi = (int)ch.page.quot(pos);
+      page = page_of(ch, lo, pi);
+      slot = pos - pi * (int)ch.page.d;
+    }
+    __syncthreads();
+    const TI* qr = static_cast<const TI*>(a.q) + (long long)row * a.q_row;
+    const TI* kr = static_cast<const TI*>(a.k) + (long long)row * a.k_row;
+    const TI* vr = static_cast<const TI*>(a.v) + (long long)row * a.v_row;
+    TO* qo = static_cast<TO*>(a.q_out) + (long long)row * a.o_row;
+    TO* ko = static_cast<TO*>(ch.k) + page * ch.k_page + slot * ch.k_slot;
+    TO* vo = static_cast<TO*>(ch.v) + page * ch.v_page + slot * ch.v_slot;
+    if (half % kV) {
+      // Pairs do not fall on vectors: one pair, or one element behind the
+      // rotated part, at a time.
+      const int per = ch.hd - half;
+      for (int x = threadIdx.x; x < (a.heads + 2 * ch.nkv) * per; x += kRopeThreads) {
+        const int head = x / per, e = x - head * per;
+        const bool is_q = head < a.heads, is_k = !is_q && head < a.heads + ch.nkv;
+        if (!is_q && page < 0) continue;
+        const int h = is_q ? head : is_k ? head - a.heads : head - a.heads - ch.nkv;
+        const TI* src = is_q ? qr + (long long)h * a.q_head : is_k ? kr + (long long)h * a.k_head : vr + (long long)h * a.v_head;
+        TO* dst = is_q ? qo + (long long)h * a.o_head : is_k ? ko + (long long)h * ch.k_head : vo + (long long)h * ch.v_head;
+        if (e >= half) {
+          dst[half + e] = Elt<OUT>::put(Elt<IN>::get(src[half + e]));
+          continue;
+        }
+        const int i = a.interleaved ? 2 * e : e, j = a.interleaved ? 2 * e + 1 : e + half;
+        const float x0 = Elt<IN>::get(src[i]), x1 = Elt<IN>::get(src[j]);
+        const float c = is_q || is_k ? cs[e] : 1.f, s = is_q || is_k ? sn[e] : 0.f;
+        dst[i] = Elt<OUT>::put(is_q || is_k ? x0 * c - x1 * s : x0);
+        dst[j] = Elt<OUT>::put(is_q || is_k ? x1 * c + x0 * s : x1);
+      }
+      continue;
+    }
+    const int per = ch.hd / kV;  // vectors of a head
+    const int total = (a.heads + 2 * ch.nkv) * per;
+    for (int x = threadIdx.x; x < total; x += kRopeThreads) {
+      const int head = x / per, d = (x - head * per) * kV;
+      const TI* src;
+      TO* dst;
+      bool rotate = true;
+      if (head < a.heads) {
+        src = qr + (long long)head * a.q_head;
+        dst = qo + (long long)head * a.o_head;
+      } else if (head < a.heads + ch.nkv) {
+        if (page < 0) continue;
+        src = kr + (long long)(head - a.heads) * a.k_head;
+        dst = ko + (long long)(head - a.heads) * ch.k_head;
+      } else {
+        if (page < 0) continue;
+        src = vr + (long long)(head - a.heads - ch.nkv) * a.v_head;
+        dst = vo + (long long)(head - a.heads - ch.nkv) * ch.v_head;
+        rotate = false;
+      }
+      float u[kV], w[kV];
+      if (!rotate || d >= a.rot) {
+        load_n<IN, kV>(src + d, u);
+        store_n<OUT, kV>(dst + d, u);
+      } else if (a.interleaved) {
+        load_n<IN, kV>(src + d, u);
+#pragma unroll
+        for (int i = 0; i < kV; i += 2) {
+          const float c = cs[d / 2 + i / 2], s = sn[d / 2 + i / 2];
+          w[i] = u[i] * c - u[i + 1] * s;
+          w[i + 1] = u[i + 1] * c + u[i] * s;
+        }
+        store_n<OUT, kV>(dst + d, w);
+      } else if (d < half) {
+        load_n<IN, kV>(src + d, u);
+        load_n<IN, kV>(src + d + half, w);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) {
+          const float c = cs[d + i], s = sn[d + i], x0 = u[i], x1 = w[i];
+          u[i] = x0 * c - x1 * s;
+          w[i] = x1 * c + x0 * s;
+        }
+        store_n<OUT, kV>(dst + d, u);
+        store_n<OUT, kV>(dst + d + half, w);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- pages
+
+constexpr int kMetaThreads = 1024;
+
+__device__ __forceinline__ int cells_of(int len, int page_size) { return (len + page_size - 1) / page_size; }
+
+// A sequence's length within its table.
+__device__ __forceinline__ int table_len(const TableArgs& t, const int* lens, int s) {
+  const int v = lens[s], cap = (int)min((long long)t.max_pages * t.page_size, (long long)(INT_MAX - 1024));
+  const int c = min(max(v, 0), cap);
+  if (c != v) atomicOr(t.err, kErrBadInput);
+  return c;
+}
+__device__ __forceinline__ bool good_page(const TableArgs& t, int page) {
+  if ((unsigned)page < (unsigned)t.n_pages) return true;
+  atomicOr(t.err, kErrBadInput);
+  return false;
+}
+
+// CTA i: child i's table row, and parent i's change of references (its
+// children less one for each page). Integer sums: the order does not matter.
+__global__ void __launch_bounds__(256) kv_fork_kernel(TableArgs in, TableArgs out, const int* __restrict__ parents) {
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const int i = blockIdx.x;
+  int mine = 0;
+  for (int x = threadIdx.x; x < out.n_seqs; x += blockDim.x) mine += parents[x] == i;
+  __shared__ int sum[8];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
+  if ((threadIdx.x & 31) == 0) sum[threadIdx.x >> 5] = mine;
+  __syncthreads();
+  int children = 0;
+  for (int w = 0; w < 8; ++w) children += sum[w];
+  if (i < in.n_seqs && children != 1) {
+    const int cells = cells_of(table_len(in, in.lens, i), in.page_size);
+    const int* row = in.table + (long long)i * in.stride;
+    for (int x = threadIdx.x; x < cells; x += blockDim.x)
+      if (good_page(in, row[x])) atomicAdd(in.refs + row[x], children - 1);
+  }
+  if (i < out.n_seqs) {
+    int p = parents[i];
+    if (p < -1 || p >= in.n_seqs) {
+      atomicOr(in.err, kErrBadInput);
+      p = -1;
+    }
+    const int len = p >= 0 ? table_len(in, in.lens, p) : 0, cells = cells_of(len, in.page_size);
+    const int* row = in.table + (long long)p * in.stride;
+    int* to = out.table + (long long)i * out.stride;
+    for (int x = threadIdx.x; x < out.max_pages; x += blockDim.x) to[x] = x < cells ? row[x] : -1;
+    if (threadIdx.x == 0) out.lens[i] = len;
+  }
+}
+
+__device__ __forceinline__ int block_scan(int v, int* sh, int* total) {  // exclusive, kMetaThreads threads
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(~0u, incl, o);
+    if (lane >= o) incl += u;
+  }
+  __syncthreads();
+  if (lane == 31) sh[warp] = incl;
+  __syncthreads();
+  if (warp == 0) {
+    int w = sh[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(~0u, w, o);
+      if (lane >= o) w += u;
+    }
+    sh[lane] = w;
+  }
+  __syncthreads();
+  *total = sh[31];
+  return incl - v + (warp ? sh[warp - 1] : 0);
+}
+
+// One CTA. Releases what shrinks, then gives the sequences that grow the
+// lowest free pages in sequence order: first the copy of a shared last page
+// that is partly filled (all holders but the last copy it), then new pages.
+// Copies are listed as (src, dst) for kv_copy_kernel: ws = [count, src[n],
+// dst[n]].
+__global__ void __launch_bounds__(kMetaThreads) kv_resize_kernel(TableArgs t, const int* __restrict__ new_lens,
+                                                                 int delta, int* status, int* ws) {
+  __shared__ int tail[kMaxTableSeqs];   // page to copy on write, or -1
+  __shared__ int place[kMaxTableSeqs];  // exclusive sum of the pages that sequences take
+  __shared__ int sh[32];
+  pdl_wait_prior();
+  const int n = t.n_seqs, ps = t.page_size;
+  const int cap = (int)min((long long)t.max_pages * ps, (long long)(INT_MAX - 1024));
+  auto want = [&](int s, int len) {
+    long long v = new_lens ? (long long)new_lens[s] : (long long)len + delta;
+    if (v < 0 || v > cap) {
+      if (new_lens || v > cap) atomicOr(t.err, kErrBadInput);
+      v = v < 0 ? 0 : cap;
+    }
+    return (int)v;
+  };
+  // Shrinking sequences release the pages behind their new end.
+  for (int s = threadIdx.x; s < n; s += kMetaThreads) {
+    const int len = table_len(t, t.lens, s), to = want(s, len);
+    tail[s] = -1;
+    int* row = t.table + (long long)s * t.stride;
+    if (to <= len) {
+      for (int x = cells_of(to, ps); x < cells_of(len, ps); ++x) {
+        if (good_page(t, row[x])) atomicSub(t.refs + row[x], 1);
+        row[x] = -1;
+      }
+    } else if (len % ps) {
+      const int page = row[len / ps];
+      if (good_page(t, page)) tail[s] = page;
+    }
+  }
+  __syncthreads();
+  // Growing ones: of the holders of a shared last page the first
+  // refs - 1 copy it.
+  for (int s0 = 0; s0 < n; s0 += kMetaThreads) {
+    const int s = s0 + threadIdx.x;
+    int copies = 0;
+    if (s < n && tail[s] >= 0) {
+      const int refs = *(volatile int*)(t.refs + tail[s]);
+      if (refs > 1) {
+        int before = 0;
+        for (int x = 0; x < s; ++x) before += tail[x] == tail[s];
+        copies = before < refs - 1;
+      }
+    }
+    if (s < n) place[s] = copies;
+  }
+  __syncthreads();
+  int sum = 0;
+  const int per = (n + kMetaThreads - 1) / kMetaThreads;
+  const int s0 = min(n, (int)threadIdx.x * per), s1 = min(n, s0 + per);
+  for (int s = s0; s < s1; ++s) {
+    const int len = table_len(t, t.lens, s), to = want(s, len);
+    if (!place[s]) tail[s] = -1;
+    if (to > len) place[s] += cells_of(to, ps) - cells_of(len, ps);
+    else place[s] = 0;
+    sum += place[s];
+  }
+  int total;
+  int at = block_scan(sum, sh, &total);
+  for (int s = s0; s < s1; ++s) {
+    const int c = place[s];
+    place[s] = at;
+    at += c;
+  }
+  // Free pages, in order: each thread looks at a run of the counts.
+  const int run = (t.n_pages + kMetaThreads - 1) / kMetaThreads;
+  const int p0 = min((long long)t.n_pages, (long long)threadIdx.x * run), p1 = min(t.n_pages, p0 + run);
+  int mine = 0;
+  for (int p = p0; p < p1; ++p) mine += *(volatile int*)(t.refs + p) == 0;
+  int free_total;
+  int rank = block_scan(mine, sh, &free_total);
+  const bool fits = total <= free_total;
+  __shared__ int count;
+  if (threadIdx.x == 0) {
+    count = 0;
+    *status = fits ? 0 : total - free_total;
+  }
+  __syncthreads();
+  if (fits && total > 0) {
+    for (int p = p0; p < p1 && rank < total; ++p) {
+      if (*(volatile int*)(t.refs + p) != 0) continue;
+      // The sequence that takes the rank-th page.
+      int lo = 0, hi = n;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (place[mid] <= rank) lo = mid; else hi = mid;
+      }
+      const int s = lo, len = table_len(t, t.lens, s);
+      int in = rank - place[s], cell = cells_of(len, ps) + in;
+      if (tail[s] >= 0) {
+        --cell;
+        if (in == 0) {
+          const int c = atomicAdd(&count, 1);
+          ws[1 + c] = tail[s];
+          ws[1 + n + c] = p;
+          atomicSub(t.refs + tail[s], 1);
+        }
+      }
+      t.table[(long long)s * t.stride + cell] = p;
+      t.refs[p] = 1;
+      ++rank;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) ws[0] = count;
+  for (int s = threadIdx.x; s < n; s += kMetaThreads) {
+    const int len = table_len(t, t.lens, s), to = want(s, len);
+    if (to <= len || fits) t.lens[s] = to;
+  }
+  __syncthreads();
+  pdl_launch_dependents();
+}
+
+// One CTA. The i-th used page at or above the number of used pages moves to
+// the i-th free page below it. ws = [count, src.., dst..] with room for
+// n_pages / 2 pairs; `moved` is the page's new number.
+__global__ void __launch_bounds__(kMetaThreads) kv_compact_kernel(TableArgs t, int* used_out, int* ws, int* moved) {
+  __shared__ int sh[32];
+  pdl_wait_prior();
+  const int run = (t.n_pages + kMetaThreads - 1) / kMetaThreads;
+  const int p0 = min((long long)t.n_pages, (long long)threadIdx.x * run), p1 = min(t.n_pages, p0 + run);
+  int mine = 0;
+  for (int p = p0; p < p1; ++p) mine += t.refs[p] > 0;
+  int used;
+  block_scan(mine, sh, &used);
+  int holes = 0, highs = 0;
+  for (int p = p0; p < p1; ++p) {
+    const bool held = t.refs[p] > 0;
+    holes += !held && p < used;
+    highs += held && p >= used;
+  }
+  int n_holes, n_highs;
+  int hole = block_scan(holes, sh, &n_holes);
+  int high = block_scan(highs, sh, &n_highs);  // n_highs == n_holes
+  int *src = ws + 1, *dst = ws + 1 + t.n_pages / 2;
+  for (int p = p0; p < p1; ++p) {
+    const bool held = t.refs[p] > 0;
+    if (!held && p < used) dst[hole++] = p;
+    if (held && p >= used) src[high++] = p;
+    moved[p] = p;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n_highs; i += kMetaThreads) {
+    const int a = src[i], b = dst[i];
+    moved[a] = b;
+    t.refs[b] = t.refs[a];
+    t.refs[a] = 0;
+  }
+  if (threadIdx.x == 0) {
+    ws[0] = n_highs;
+    *used_out = used;
+  }
+  __syncthreads();
+  pdl_launch_dependents();
+}
+
+__global__ void __launch_bounds__(256) kv_rename_kernel(TableArgs t, const int* __restrict__ moved) {
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  for (int s = blockIdx.x; s < t.n_seqs; s += gridDim.x) {
+    int* row = t.table + (long long)s * t.stride;
+    const int cells = cells_of(table_len(t, t.lens, s), t.page_size);
+    for (int x = threadIdx.x; x < cells; x += blockDim.x)
+      if (good_page(t, row[x])) row[x] = moved[row[x]];
+  }
+}
+
+// Page data: CTAs walk (pair, plane, piece) with 16-byte vectors, several in
+// flight per thread. Bound: HBM, 2 x bytes moved.
+constexpr int kCopyThreads = 256;
+constexpr int kCopyVecs = 8;
+constexpr long long kPiece = kCopyThreads * kCopyVecs * 16ll;
+__global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(PagePool pool, const int* __restrict__ src,
+                                                               const int* __restrict__ dst,
+                                                               const int* __restrict__ n_dev, int n, uint32_t* err) {
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const int pairs = n_dev ? min(max(*n_dev, 0), n) : n;
+  const long long pieces = (pool.bytes + kPiece - 1) / kPiece;
+  const long long planes = 2ll * pool.layers, total = pairs * planes * pieces;
+  for (long long x = blockIdx.x; x < total; x += gridDim.x) {
+    const long long piece = x % pieces, y = x / pieces;
+    const int plane = (int)(y % planes), pair = (int)(y / planes);
+    const int a = src[pair], b = dst[pair];
+    if ((unsigned)a >= (unsigned)pool.n_pages || (unsigned)b >= (unsigned)pool.n_pages) {
+      if (threadIdx.x == 0) atomicOr(err, kErrBadInput);
+      continue;
+    }
+    const bool is_v = plane >= pool.layers;
+    const int layer = is_v ? plane - pool.layers : plane;
+    char* base = is_v ? pool.v + layer * pool.v_layer : pool.k + layer * pool.k_layer;
+    const long long ps = is_v ? pool.v_page : pool.k_page;
+    const uint4* from = reinterpret_cast<const uint4*>(base + a * ps + piece * kPiece);
+    uint4* to = reinterpret_cast<uint4*>(base + b * ps + piece * kPiece);
+    const int vecs = (int)(min(kPiece, pool.bytes - piece * kPiece) / 16);
+    uint4 v[kCopyVecs];
+#pragma unroll
+    for (int i = 0; i < kCopyVecs; ++i)
+      if (threadIdx.x + i * kCopyThreads < vecs) v[i] = __ldcs(from + threadIdx.x + i * kCopyThreads);
+#pragma unroll
+    for (int i = 0; i < kCopyVecs; ++i)
+      if (threadIdx.x + i * kCopyThreads < vecs) __stcs(to + threadIdx.x + i * kCopyThreads, v[i]);
+  }
+}
+
+}  // namespace
+
+cudaError_t rope_append(const RopeArgs& a, cudaStream_t s) {
+  const int grid = grid_cap(a.c.rows, 8);
+#define RAI_ROPE(I, O)                                                                                   \
+  if (a.in_dtype == I && a.cache_dtype == O)                                                             \
+    return launch_pdl(rope_append_kernel<I, O>, dim3(grid), dim3(kRopeThreads), 0, s, a);
+  RAI_ROPE(kF32, kF32) RAI_ROPE(kF32, kF16) RAI_ROPE(kF32, kBF16)
+  RAI_ROPE(kF16, kF32) RAI_ROPE(kF16, kF16) RAI_ROPE(kF16, kBF16)
+  RAI_ROPE(kBF16, kF32) RAI_ROPE(kBF16, kF16) RAI_ROPE(kBF16, kBF16)
+#undef RAI_ROPE
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t kv_fork(const TableArgs& in, const TableArgs& out, const int* parents, cudaStream_t s) {
+  const int grid = in.n_seqs > out.n_seqs ? in.n_seqs : out.n_seqs;
+  return launch_pdl(kv_fork_kernel, dim3(grid), dim3(256), 0, s, in, out, parents);
+}
+
+cudaError_t kv_copy(const PagePool& pool, const int* src, const int* dst, const int* n_dev, int n, uint32_t* err,
+                    cudaStream_t s) {
+  const long long pieces = (pool.bytes + kPiece - 1) / kPiece;
+  const long long total = n * 2ll * pool.layers * pieces;
+  const int cap = device_sm_count() * 4;
+  return launch_pdl(kv_copy_kernel, dim3((unsigned)(total < cap ? total : cap)), dim3(kCopyThreads), 0, s, pool, src, dst,
+                    n_dev, n, err);
+}
+
+size_t kv_resize_workspace(int n_seqs) { return (1 + 2 * (size_t)n_seqs) * 4; }
+cudaError_t kv_resize(const TableArgs& t, const PagePool& pool, const int* new_lens, int delta, int* status, void* ws,
+                      cudaStream_t s) {
+  int* w = static_cast<int*>(ws);
+  cudaError_t e = launch_pdl(kv_resize_kernel, dim3(1), dim3(kMetaThreads), 0, s, t, new_lens, delta, status, w);
+  if (e != cudaSuccess || (!new_lens && delta <= 0)) return e;  // nothing can grow
+  return kv_copy(pool, w + 1, w + 1 + t.n_seqs, w, t.n_seqs, t.err, s);
+}
+
+size_t kv_compact_workspace(int n_pages) { return (1 + 2 * (size_t)(n_pages / 2) + n_pages) * 4; }
+cudaError_t kv_compact(const TableArgs& t, const PagePool& pool, int* used, void* ws, cudaStream_t s) {
+  int *w = static_cast<int*>(ws), *moved = w + 1 + 2 * (t.n_pages / 2);
+  cudaError_t e = launch_pdl(kv_compact_kernel, dim3(1), dim3(kMetaThreads), 0, s, t, used, w, moved);
+  if (e != cudaSuccess) return e;
+  if (t.n_seqs > 0) {
+    e = launch_pdl(kv_rename_kernel, dim3(grid_cap(t.n_seqs, 4)), dim3(256), 0, s, t, (const int*)moved);
+    if (e != cudaSuccess) return e;
+  }
+  const int most = t.n_pages / 2;
+  if (most == 0) return e;
+  return kv_copy(pool, w + 1, w + 1 + most, w, most, t.err, s);
+}
+
+}  // namespace rai

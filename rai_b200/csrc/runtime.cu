@@ -24,6 +24,7 @@
 
 #include "../../include/rai_gpu.h"
 #include "common.cuh"
+#include "errors.h"
 #include "kernels.h"
 #include "layers.h"
 #include "moe.h"
@@ -1092,6 +1093,11 @@ int static_scratch(void** out) {
 }
 }  // namespace
 
+namespace rai {
+int set_error(int code, const std::string& msg) { return fail(code, msg); }
+int kernel_status_word(uint32_t** out) { return kernel_err_word(out); }
+}  // namespace rai
+
 // ===========================================================================
 extern "C" {
 
@@ -1881,6 +1887,8 @@ int rai_gpu_kernel_status(void* stream) {
   if (e) {
     RAI_CUDA(cudaMemsetAsync(err, 0, 4, s));
     RAI_CUDA(cudaStreamSynchronize(s));
+    if (!(e & rai::kErrWaitTimeout))
+      return fail(RAI_ERR_INVALID, "a kernel-level call met a page number, length or row range outside its tensors");
     return fail(RAI_ERR_TIMEOUT, "a device-side wait of a kernel-level call timed out (its output is incomplete)");
   }
   return RAI_OK;

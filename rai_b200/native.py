@@ -59,6 +59,45 @@ class ModelInfo(C.Structure):
         "experts_per_token", "tied_embeddings", "version")] + [("device_bytes", C.c_uint64)]
 
 
+class PagedChunk(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_int64) for n in (
+        "k_page", "k_head", "k_slot", "v_page", "v_head", "v_slot")] + [
+        ("table", C.c_void_p), ("kv_len", C.c_void_p), ("q_start", C.c_void_p), ("table_stride", C.c_int64)] + [
+        (n, C.c_uint32) for n in ("n_seqs", "max_pages", "n_pages", "page_size", "n_kv_heads", "head_dim", "rows",
+                                  "max_rows", "dtype")]
+
+
+class PagedAttention(C.Structure):
+    _fields_ = [("chunk", PagedChunk), ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p)] + [
+        (n, C.c_int64) for n in ("q_row", "q_head", "out_row", "out_head")] + [
+        ("n_heads", C.c_uint32), ("window", C.c_uint32), ("scale", C.c_float), ("softcap", C.c_float),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class RopeAppend(C.Structure):
+    _fields_ = [("chunk", PagedChunk)] + [(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "inv_freq")] + [
+        (n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "out_row", "out_head")] + [
+        (n, C.c_uint32) for n in ("n_heads", "rot_dim", "interleaved", "in_dtype")] + [("mscale", C.c_float)]
+
+
+class PageTable(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("lens", C.c_void_p), ("refs", C.c_void_p), ("table_stride", C.c_int64)] + [
+        (n, C.c_uint32) for n in ("n_seqs", "max_pages", "n_pages", "page_size")]
+
+
+class PagePool(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_int64) for n in (
+        "k_layer", "k_page", "v_layer", "v_page", "page_bytes")] + [("n_layers", C.c_uint32), ("n_pages", C.c_uint32)]
+
+
+class BeamSelect(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("scores", C.c_void_p), ("row_stride", C.c_int64)] + [(n, C.c_void_p) for n in (
+        "cand_score", "cand_beam", "cand_token", "score", "parent", "token", "history", "hist_len", "out_history",
+        "out_len")] + [("hist_stride", C.c_int64), ("out_hist_stride", C.c_int64)] + [(n, C.c_uint32) for n in (
+            "hist_cap", "batch", "beams", "vocab", "keep")] + [("eos", C.c_int32), ("dtype", C.c_uint32),
+                                                              ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 _lib = None
 P = C.c_void_p
 SZ = C.c_size_t
@@ -117,6 +156,23 @@ def lib() -> C.CDLL:
         L.rai_gpu_w4a8_tol_workspace_bytes.restype = SZ
         L.rai_gpu_w4a8_matmul_tol_prequant.argtypes = [P, P, P, SZ, SZ, SZ, SZ, P, SZ, P]
         L.rai_gpu_attention.argtypes = [P, P, P, P, SZ, SZ, SZ, SZ, SZ, C.c_float, P, P]
+        # Structures go as a pointer to one, or as its bytes.
+        L.rai_gpu_paged_attention_workspace_bytes.argtypes = [P]
+        L.rai_gpu_paged_attention_workspace_bytes.restype = SZ
+        L.rai_gpu_paged_attention.argtypes = [P, P]
+        L.rai_gpu_rope_append.argtypes = [P, P]
+        L.rai_rope_frequencies.argtypes = [C.c_int, C.c_uint32] + [C.c_double] * 5 + [P, C.POINTER(C.c_float)]
+        L.rai_gpu_kv_fork.argtypes = [P, P, P, P]
+        L.rai_gpu_kv_resize_workspace_bytes.argtypes = [C.c_uint32]
+        L.rai_gpu_kv_resize_workspace_bytes.restype = SZ
+        L.rai_gpu_kv_resize.argtypes = [P, P, P, C.c_int32, P, P, SZ, P]
+        L.rai_gpu_kv_compact_workspace_bytes.argtypes = [C.c_uint32]
+        L.rai_gpu_kv_compact_workspace_bytes.restype = SZ
+        L.rai_gpu_kv_compact.argtypes = [P, P, P, P, SZ, P]
+        L.rai_gpu_kv_copy_pages.argtypes = [P, P, P, SZ, P]
+        L.rai_gpu_beam_workspace_bytes.argtypes = [C.c_uint32] * 4
+        L.rai_gpu_beam_workspace_bytes.restype = SZ
+        L.rai_gpu_beam_select.argtypes = [P, P]
         L.rai_rtn_quantize.argtypes = [P, SZ, SZ, C.c_int, SZ, P, P, C.c_int]
         L.rai_synth_normal_f16.argtypes = [C.c_uint64, C.c_uint64, SZ, C.c_float, P, C.c_int]
         L.rai_f64_to_f16.argtypes = [P, SZ, P]

@@ -1,0 +1,334 @@
+"""Paged KV caches on torch tensors: rotary positions with the store into
+pages, attention of a ragged chunk of new tokens, and the page operations
+(fork, resize, compact, copy), over the entry points of include/rai_gpu.h.
+
+A cache is two tensors of pages per layer, K and V, each [pages, kv_heads,
+page_size, head_dim] (any strides whose vectors start on 16 bytes; float32,
+float16 or bfloat16), an int32 table [sequences, max_pages] that names each
+sequence's pages, its int32 lengths, and int32 reference counts [pages]. rai-infer's own
+cache (rai-infer/src/kv_cache.rs:143-304) is one contiguous window per stream.
+
+Everything runs on the current torch stream of the tensors' device, without a
+host synchronisation, and can be captured in a CUDA graph (after one call
+outside of a capture). Wrong arguments raise ValueError or RaiError at the
+call; page numbers, lengths and row ranges on the device that pass the given
+bounds are cut to them and raise at the next `status()`.
+
+    q = rope_append(q, k, v, k_pages, v_pages, table, kv_len, q_start, inv_freq)
+    o = attention(q, k_pages, v_pages, table, kv_len, q_start, max_rows)
+"""
+from __future__ import annotations
+
+import ctypes as C
+import functools
+import struct
+from typing import Optional, Tuple
+
+import numpy as np
+import torch
+
+from . import native
+from .native import check
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_CHUNK = "2Q6q3Qq9I4x"
+_ATTN = struct.Struct(_CHUNK + "3Q4q2I2f2Q")
+_ROPE = struct.Struct(_CHUNK + "5Q8q4If4x")
+_TABLE = struct.Struct("3Qq4I")
+_POOL = struct.Struct("2Q5q2I")
+ROPE_KINDS = {"plain": 0, "linear": 1, "ntk": 2, "llama3": 3, "yarn": 4}
+
+
+def _dtype(t: torch.Tensor, name: str) -> int:
+    d = _DTYPES.get(t.dtype)
+    if d is None:
+        raise ValueError(f"{name}: float32, float16 or bfloat16, not {t.dtype}")
+    return d
+
+
+def _device(*tensors: Tuple[str, torch.Tensor]) -> int:
+    """The CUDA device that all tensors are on."""
+    dev = tensors[0][1].get_device()
+    for name, t in tensors:
+        if t.get_device() != dev or dev < 0:
+            raise ValueError(f"{name}: every tensor has to be on one CUDA device")
+    return dev
+
+
+def _launch(dev: int, fn, *args) -> None:
+    """fn(*args, stream) with the tensors' device current, on its current
+    torch stream."""
+    if dev == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+
+
+def _ints(name: str, t: torch.Tensor, *shape: Optional[int]) -> int:
+    """Address of an int32 tensor of this shape, its last dimension dense."""
+    if t.dtype != torch.int32 or t.dim() != len(shape):
+        raise ValueError(f"{name}: an int32 tensor of {len(shape)} dimension(s)")
+    for got, want in zip(t.shape, shape):
+        if want is not None and got != want:
+            raise ValueError(f"{name}: shape {tuple(t.shape)} does not fit the other arguments")
+    if shape and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last dimension has to be contiguous")
+    return t.data_ptr()
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Row stride of a table; a one-row table may have any."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _rows3(name: str, t: torch.Tensor, heads: Optional[int], dim: int) -> None:
+    if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name}: [rows, heads, head_dim] that fits the pages, not {tuple(t.shape)}")
+    if t.stride(2) != 1 and dim > 1:
+        raise ValueError(f"{name}: head_dim has to be contiguous")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name}: this operator has no gradient; call it under torch.no_grad()")
+
+
+def _chunk(k_pages, v_pages, table, kv_len, q_start, rows: int, max_rows: int, dtype: int):
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise ValueError("k_pages, v_pages: two tensors [pages, kv_heads, page_size, head_dim] of one shape and type")
+    n_pages, nkv, page, hd = k_pages.shape
+    ks, vs = k_pages.stride(), v_pages.stride()
+    if hd > 1 and (ks[3] != 1 or vs[3] != 1):
+        raise ValueError("k_pages, v_pages: head_dim has to be contiguous")
+    n = kv_len.shape[0]
+    return (k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+            _ints("page_table", table, n, None), _ints("kv_len", kv_len, n), _ints("q_start", q_start, n + 1),
+            _row_stride(table), n, table.shape[1], n_pages, page, nkv, hd, rows, max_rows, dtype)
+
+
+@functools.lru_cache(maxsize=256)
+def _attn_workspace(dev: int, dtype: int, hd: int, nkv: int, heads: int, max_rows: int) -> int:
+    a = native.PagedAttention()
+    a.chunk.dtype, a.chunk.head_dim, a.chunk.n_kv_heads, a.chunk.max_rows = dtype, hd, nkv, max_rows
+    a.n_heads = heads
+    with torch.cuda.device(dev):
+        return native.lib().rai_gpu_paged_attention_workspace_bytes(C.byref(a))
+
+
+def attention_workspace_bytes(q: torch.Tensor, k_pages: torch.Tensor, max_rows: int) -> int:
+    """Bytes of the workspace that `attention` takes for these arguments."""
+    return _attn_workspace(q.get_device(), _dtype(k_pages, "k_pages"), k_pages.shape[3], k_pages.shape[1], q.shape[1],
+                           max_rows)
+
+
+def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+              kv_len: torch.Tensor, q_start: torch.Tensor, max_rows: int, *, scale: Optional[float] = None,
+              softcap: float = 0.0, window: int = 0, out: Optional[torch.Tensor] = None,
+              lse: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of each sequence's new rows (q[q_start[s]:q_start[s+1]],
+    the last of its kv_len[s] tokens, at most max_rows of them) over its pages
+    (rai_gpu_paged_attention). q [rows, heads, head_dim] in the pages' type;
+    heads a multiple of the pages' KV heads. softcap > 0 caps the scores by
+    softcap * tanh(s / softcap), window > 0 keeps the last `window` tokens.
+    Rows that no sequence has are left as they are in `out` (undefined when
+    `out` is not given). lse (float32 [rows, heads]) receives the rows'
+    log-sum-exp. A row that sees nothing gives 0 and -inf."""
+    dtype = _dtype(k_pages, "k_pages")
+    hd = k_pages.shape[-1]
+    _rows3("q", q, None, hd)
+    if q.dtype != k_pages.dtype:
+        raise ValueError(f"q: {k_pages.dtype} as the pages, not {q.dtype}")
+    rows, heads = q.shape[0], q.shape[1]
+    if out is None:
+        out = torch.empty((rows, heads, hd), dtype=q.dtype, device=q.device)
+    else:
+        _rows3("out", out, heads, hd)
+        if out.shape[0] != rows or out.dtype != q.dtype:
+            raise ValueError("out: shape and type of q")
+    dev = _device(("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("kv_len", kv_len),
+                  ("q_start", q_start), ("out", out))
+    if rows == 0 or kv_len.shape[0] == 0 or max_rows == 0:
+        return out
+    chunk = _chunk(k_pages, v_pages, page_table, kv_len, q_start, rows, min(max_rows, rows), dtype)
+    lse_at = 0
+    if lse is not None:
+        if lse.dtype != torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous() or lse.get_device() != dev:
+            raise ValueError("lse: contiguous float32 [rows, heads] on q's device")
+        lse_at = lse.data_ptr()
+    if workspace is None:
+        workspace = torch.empty(_attn_workspace(dev, dtype, hd, chunk[16], heads, min(max_rows, rows)), dtype=torch.uint8,
+                                device=q.device)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("workspace: contiguous, on q's device")
+    args = _ATTN.pack(*chunk, q.data_ptr(), out.data_ptr(), lse_at, q.stride(0), q.stride(1), out.stride(0), out.stride(1),
+                      heads, window, hd ** -0.5 if scale is None else scale, softcap, workspace.data_ptr(),
+                      workspace.numel() * workspace.element_size())
+    _launch(dev, native.lib().rai_gpu_paged_attention, args)
+    return out
+
+
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                page_table: torch.Tensor, kv_len: torch.Tensor, q_start: torch.Tensor, inv_freq: torch.Tensor, *,
+                interleaved: bool = False, mscale: float = 1.0, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotate the chunk's q and k rows to their positions and store k and v in
+    the pages (rai_gpu_rope_append). q [rows, heads, head_dim], k and v
+    [rows, kv_heads, head_dim], views of one projection's output as well, in
+    one type; the result and the pages in the pages' type. inv_freq (float32,
+    device) has one frequency per pair; 2 * len(inv_freq) elements of a head
+    turn. q_out may be q itself. Rows as in `attention`, kv_len counting them."""
+    dtype, hd, nkv = _dtype(k_pages, "k_pages"), k_pages.shape[-1], k_pages.shape[1]
+    _rows3("q", q, None, hd)
+    _rows3("k", k, nkv, hd)
+    _rows3("v", v, nkv, hd)
+    rows, heads = q.shape[0], q.shape[1]
+    in_dtype = _dtype(q, "q")
+    if k.dtype != q.dtype or v.dtype != q.dtype or k.shape[0] != rows or v.shape[0] != rows:
+        raise ValueError("q, k, v: one type and one number of rows")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq: a contiguous float32 vector")
+    if q_out is None:
+        q_out = torch.empty((rows, heads, hd), dtype=k_pages.dtype, device=q.device)
+    else:
+        _rows3("q_out", q_out, heads, hd)
+        if q_out.shape[0] != rows or q_out.dtype != k_pages.dtype:
+            raise ValueError("q_out: q's shape in the pages' type")
+    dev = _device(("q", q), ("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table),
+                  ("kv_len", kv_len), ("q_start", q_start), ("inv_freq", inv_freq), ("q_out", q_out))
+    if rows == 0 or kv_len.shape[0] == 0:
+        return q_out
+    args = _ROPE.pack(*_chunk(k_pages, v_pages, page_table, kv_len, q_start, rows, rows, dtype), q.data_ptr(), k.data_ptr(),
+                      v.data_ptr(), q_out.data_ptr(), inv_freq.data_ptr(), q.stride(0), q.stride(1), k.stride(0),
+                      k.stride(1), v.stride(0), v.stride(1), q_out.stride(0), q_out.stride(1), heads,
+                      2 * inv_freq.shape[0], 1 if interleaved else 0, in_dtype, mscale)
+    _launch(dev, native.lib().rai_gpu_rope_append, args)
+    return q_out
+
+
+def rope_frequencies(rot_dim: int, theta: float = 10000.0, kind: str = "plain", *, factor: float = 1.0, low: float = 1.0,
+                     high: float = 4.0, original: float = 8192.0) -> Tuple[np.ndarray, float]:
+    """(inv_freq, mscale) for `rope_append` (rai_rope_frequencies): kind plain,
+    linear, ntk, llama3 (rai-infer/src/layers.rs:760-808) or yarn, for
+    contexts `factor` times the `original` positions."""
+    if kind not in ROPE_KINDS:
+        raise ValueError(f"kind: one of {', '.join(ROPE_KINDS)}")
+    out = np.zeros(max(rot_dim, 0) // 2, np.float32)
+    m = C.c_float()
+    check(native.lib().rai_rope_frequencies(ROPE_KINDS[kind], rot_dim, theta, factor, low, high, original, out.ctypes.data,
+                                            C.byref(m)))
+    return out, m.value
+
+
+def _table(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, page_size: int) -> bytes:
+    n = table.shape[0]
+    return _TABLE.pack(_ints("page_table", table, None, None), _ints("lens", lens, n), _ints("refs", refs, None),
+                       _row_stride(table), n, table.shape[1], refs.shape[0], page_size)
+
+
+def _pool(k: torch.Tensor, v: torch.Tensor):
+    """(bytes of rai_page_pool, page size) of the K and V pages of every
+    layer: [layers, pages, kv_heads, page_size, head_dim], or one layer's four
+    dimensions, a page being one dense block."""
+    if k.dim() == 4:
+        k = k.unsqueeze(0)
+    if v.dim() == 4:
+        v = v.unsqueeze(0)
+    _dtype(k, "k")
+    if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError("k, v: two tensors [layers, pages, kv_heads, page_size, head_dim] of one shape and type")
+    e = k.element_size()
+    for name, t in (("k", k), ("v", v)):
+        # A page's block may order its heads and slots either way.
+        dims = sorted((s, n) for s, n in zip(t.stride()[2:], t.shape[2:]) if n > 1)
+        want = 1
+        for s, n in dims:
+            if s != want:
+                raise ValueError(f"{name}: every page has to be one contiguous block")
+            want *= n
+    n = k.shape[2] * k.shape[3] * k.shape[4] * e
+    one = k.shape[1] == 1  # the stride of a single page or layer means nothing
+    return _POOL.pack(k.data_ptr(), v.data_ptr(), k.stride(0) * e if k.shape[0] > 1 else 0, n if one else k.stride(1) * e,
+                      v.stride(0) * e if v.shape[0] > 1 else 0, n if one else v.stride(1) * e, n, k.shape[0],
+                      k.shape[1]), k.shape[3]
+
+
+def fork(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor, page_size: int, *,
+         out_table: Optional[torch.Tensor] = None, out_lens: Optional[torch.Tensor] = None):
+    """Sequence i of the result takes the pages of sequence parents[i] (-1:
+    none); returns (table, lens), in new memory or in out_table, out_lens
+    (rai_gpu_kv_fork). refs is updated in place: sequences without children
+    are freed, children of one parent share its pages. No page moves."""
+    n = parents.shape[0]
+    if n == 0 or page_table.shape[0] == 0:
+        raise ValueError("fork: no sequences")
+    if out_table is None:
+        out_table = torch.empty((n, page_table.shape[1]), dtype=torch.int32, device=page_table.device)
+    if out_lens is None:
+        out_lens = torch.empty((n,), dtype=torch.int32, device=page_table.device)
+    dev = _device(("page_table", page_table), ("lens", lens), ("refs", refs), ("parents", parents), ("out_table", out_table),
+                  ("out_lens", out_lens))
+    if out_table.dim() != 2 or out_table.shape[0] != n:
+        raise ValueError("out_table: one row per parent")
+    _launch(dev, native.lib().rai_gpu_kv_fork, _table(page_table, lens, refs, page_size),
+            _table(out_table, out_lens, refs, page_size), _ints("parents", parents, n))
+    return out_table, out_lens
+
+
+def resize(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+           delta: int = 0, new_lens: Optional[torch.Tensor] = None,
+           workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Resize every sequence in place to new_lens, or by delta tokens
+    (rai_gpu_kv_resize): what shrinks releases its pages (length 0 frees it),
+    what grows takes the lowest free pages, copying a shared last page first
+    that is partly filled. k, v: the pages of every layer. Returns an int32
+    [1] on the device: 0, or the number of pages missing, when nothing grew."""
+    pool, page = _pool(k, v)
+    dev = _device(("page_table", page_table), ("lens", lens), ("refs", refs), ("k", k), ("v", v),
+                  *((("new_lens", new_lens),) if new_lens is not None else ()))
+    n = page_table.shape[0]
+    status = torch.empty((1,), dtype=torch.int32, device=lens.device)
+    if workspace is None:
+        workspace = torch.empty(native.lib().rai_gpu_kv_resize_workspace_bytes(n), dtype=torch.uint8, device=lens.device)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("workspace: contiguous, on the tables' device")
+    _launch(dev, native.lib().rai_gpu_kv_resize, _table(page_table, lens, refs, page), pool,
+            _ints("new_lens", new_lens, n) if new_lens is not None else None, delta, status.data_ptr(),
+            workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    return status
+
+
+def compact(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+            workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Move the pages in use to the front of the pool, in place; tables and
+    refs follow (rai_gpu_kv_compact). Every sequence that holds pages of the
+    pool has to be in page_table. Returns the number of pages in use, int32
+    [1] on the device."""
+    pool, page = _pool(k, v)
+    dev = _device(("page_table", page_table), ("lens", lens), ("refs", refs), ("k", k), ("v", v))
+    used = torch.empty((1,), dtype=torch.int32, device=refs.device)
+    if workspace is None:
+        workspace = torch.empty(native.lib().rai_gpu_kv_compact_workspace_bytes(refs.shape[0]), dtype=torch.uint8,
+                                device=refs.device)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("workspace: contiguous, on the tables' device")
+    _launch(dev, native.lib().rai_gpu_kv_compact, _table(page_table, lens, refs, page), pool, used.data_ptr(),
+            workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    return used
+
+
+def copy_pages(k: torch.Tensor, v: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Copy page src[i] to page dst[i] in every layer (rai_gpu_kv_copy_pages).
+    No destination may occur twice or be a source."""
+    pool, _ = _pool(k, v)
+    dev = _device(("k", k), ("v", v), ("src", src), ("dst", dst))
+    n = src.shape[0]
+    _launch(dev, native.lib().rai_gpu_kv_copy_pages, pool, _ints("src", src, n), _ints("dst", dst, n), n)
+
+
+def status(device=None) -> None:
+    """Wait for the current stream and raise RaiError if a kernel-level call
+    since the last query met a value on the device outside its tensors, or a
+    device wait that gave up (rai_gpu_kernel_status)."""
+    with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
+        check(native.lib().rai_gpu_kernel_status(torch.cuda.current_stream().cuda_stream))
+
+
+__all__ = ["attention", "attention_workspace_bytes", "compact", "copy_pages", "fork", "resize", "rope_append",
+           "rope_frequencies", "status"]

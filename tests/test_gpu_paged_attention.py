@@ -1,0 +1,266 @@
+"""rai_b200.paged.attention against plain attention in 64 bits: types, head
+layouts, ragged lengths, masks, and what masked places may hold."""
+import itertools
+import math
+
+import pytest
+
+import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def run(cache, q, rows, *, scale=None, softcap=0.0, window=0, first=0, max_rows=None, with_lse=True, **kw):
+    from rai_b200 import paged
+    dev = q.device
+    lse = torch.full(q.shape[:2], 7.0, device=dev) if with_lse else None
+    out = kw.pop("out", None)
+    if out is None:
+        out = torch.full(q.shape, 3.0, dtype=q.dtype, device=dev)
+    got = paged.attention(q, cache.k, cache.v, cache.table, cache.kv_len, ref.starts_of(rows, dev, first),
+                          max(rows) if max_rows is None else max_rows, scale=scale, softcap=softcap, window=window, out=out,
+                          lse=lse, **kw)
+    paged.status()
+    return got, lse
+
+
+def agree(cache, q, rows, got, lse, *, scale=None, softcap=0.0, window=0, first=0):
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    want, bound, wlse = ref.attention(q, cache, rows, scale, softcap, window, first)
+    a, b = first, first + sum(rows)
+    g, w = got[a:b].double(), want[a:b]
+    fine = torch.isfinite(w)
+    assert torch.equal(torch.isfinite(g), fine), "finite where it should not be, or the other way"
+    assert torch.equal(torch.isnan(g), torch.isnan(w))
+    over = torch.where(fine, (g - w).abs() / bound[a:b], 0.0)
+    assert over.max() <= 1.0, f"off by {over.max():.3g} times the bound at {over.argmax()}"
+    if lse is not None:
+        d = (lse[a:b].double() - wlse[a:b])
+        empty = wlse[a:b] == -math.inf
+        assert torch.equal(lse[a:b] == -math.inf, empty)
+        # Scores off by d, sums of up to n terms in f32.
+        tol = 2.0 ** -18 * (1 + wlse[a:b].abs()) + softcap * 2.0 ** -20
+        assert (d[~empty].abs() <= tol[~empty]).all(), d[~empty].abs().max()
+    # Rows of no sequence are left as they were.
+    assert (got[:a] == 3.0).all() and (got[b:] == 3.0).all()
+
+
+def make_q(T, H, D, dtype, dev, seed=1, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (scale * torch.randn((T, H, D), generator=g)).to(dtype).to(dev)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("heads,nkv,hd", [(14, 2, 64), (32, 8, 128), (4, 4, 32), (6, 2, 96), (15, 5, 80), (4, 2, 256),
+                                          (8, 1, 16), (5, 1, 136)])
+def test_shapes_and_lengths(dtype, heads, nkv, hd):
+    dev = torch.device("cuda", 0)
+    rows = [1, 2, 0, 9, 1, 5, 1, 1]
+    lens = [1, 64, 7, 65, 200, 5, 63, 129]
+    c = ref.Cache(lens, nkv, hd, 16, dtype, dev, seed=hd)
+    q = make_q(sum(rows) + 4, heads, hd, dtype, dev)
+    got, lse = run(c, q, rows, first=2)
+    agree(c, q, rows, got, lse, first=2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("page", [1, 3, 16, 100, 256])
+@pytest.mark.parametrize("softcap,window", [(0.0, 0), (20.0, 0), (0.0, 1), (0.0, 70), (5.0, 33)])
+def test_pages_caps_and_windows(dtype, page, softcap, window):
+    dev = torch.device("cuda", 0)
+    rows = [3, 1, 12, 40]
+    lens = [3, 300, 130, 140]
+    c = ref.Cache(lens, 2, 64, page, dtype, dev, seed=page)
+    q = make_q(sum(rows), 6, 64, dtype, dev, scale=2.0)
+    got, lse = run(c, q, rows, softcap=softcap, window=window)
+    agree(c, q, rows, got, lse, softcap=softcap, window=window)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("heads,nkv,hd", [(8, 2, 64), (8, 2, 128), (2, 2, 256)])
+@pytest.mark.parametrize("softcap,window", [(0.0, 0), (30.0, 100)])
+def test_long_chunks(dtype, heads, nkv, hd, softcap, window):
+    """Hundreds of rows: several row tiles, cut over the CTAs."""
+    dev = torch.device("cuda", 0)
+    rows = [300, 1, 129, 64, 257]
+    lens = [300, 900, 700, 64, 1025]
+    c = ref.Cache(lens, nkv, hd, 32, dtype, dev, seed=hd + 1)
+    q = make_q(sum(rows) + 3, heads, hd, dtype, dev)
+    got, lse = run(c, q, rows, softcap=softcap, window=window)
+    agree(c, q, rows, got, lse, softcap=softcap, window=window)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("rows,lens", [([1], [5000]), ([1, 1], [9000, 3]), ([9, 4, 1], [4000, 6500, 2500]),
+                                       ([33], [3000])])
+def test_few_long_sequences_are_cut(dtype, rows, lens):
+    dev = torch.device("cuda", 0)
+    c = ref.Cache(lens, 2, 64, 16, dtype, dev, seed=len(lens))
+    q = make_q(sum(rows), 8, 64, dtype, dev)
+    got, lse = run(c, q, rows)
+    agree(c, q, rows, got, lse)
+    again, _ = run(c, q, rows)
+    assert torch.equal(got, again)  # the same bits every time
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_rows_that_see_nothing(dtype, hd):
+    """kv_len below the row count: the first rows stand before the sequence."""
+    dev = torch.device("cuda", 0)
+    rows, lens = [5, 3, 150, 200], [2, 0, 70, 1]
+    c = ref.Cache(lens, 2, hd, 16, dtype, dev)
+    q = make_q(sum(rows), 4, hd, dtype, dev)
+    got, lse = run(c, q, rows)
+    agree(c, q, rows, got, lse)
+    assert (got[:3] == 0).all() and (lse[5:8] == -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,window", [(6, 0), (6, 40), (160, 0), (300, 90)])
+def test_what_is_masked_does_not_matter(dtype, hd, rows, window):
+    """NaN and infinities in later tokens, in tokens behind the window, in
+    unused slots: only rows that see them change."""
+    dev = torch.device("cuda", 0)
+    n = rows + 300
+    c = ref.Cache([n], 2, hd, 16, dtype, dev, seed=rows)
+    q = make_q(rows, 4, hd, dtype, dev)
+
+    def token(t):
+        return c.rows[0][t // 16], t % 16
+    p, s = token(n - 3)
+    c.v[p, :, s, 5] = math.nan
+    c.k[p, 0, s] = math.inf
+    p, s = token(n - 2)
+    c.v[p, 1, s] = math.inf
+    p, s = token(n - rows // 2)
+    c.v[p, 0, s, :3] = -math.inf
+    if window:
+        p, s = token(10)
+        c.v[p, :, s] = math.nan
+        c.k[p, :, s] = math.nan
+    got, _ = run(c, q, [rows], window=window, with_lse=False)
+    want, bound, _ = ref.attention(q, c, [rows], hd ** -0.5, 0.0, window)
+    # K of KV head 0 at n - 3 is infinite: its rows from there on are NaN or
+    # saturated; the others are held to their bounds.
+    g, w = got.double(), want
+    safe = torch.ones(rows, 4, dtype=torch.bool, device=dev)
+    safe[rows - 3:, :2] = False
+    fine = torch.isfinite(w) & safe[:, :, None]
+    assert ((g - w).abs() <= bound)[fine].all()
+    assert not torch.isfinite(g[(~torch.isfinite(w)) & safe[:, :, None]]).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_scores_of_the_lowest_value_and_large(dtype):
+    """Scores near the largest the type can make, and all equal ones."""
+    dev = torch.device("cuda", 0)
+    c = ref.Cache([90, 90], 1, 64, 16, dtype, dev)
+    q = make_q(2, 2, 64, dtype, dev, scale=60.0)
+    q[1] = 0
+    got, lse = run(c, q, [1, 1], with_lse=False)
+    agree(c, q, [1, 1], got, None)
+
+
+def test_strided_rows_and_slot_major_pages():
+    """q as a view of a projection's output, out in a wider buffer, pages
+    [page, slot, head, dim], a table cut from a wider one."""
+    from rai_b200 import paged
+    dev = torch.device("cuda", 0)
+    rows, lens = [2, 130, 1], [50, 200, 777]
+    for dtype in DTYPES:
+        c = ref.Cache(lens, 2, 64, 16, dtype, dev, nhd=True, wide=4)
+        T = sum(rows)
+        big = make_q(T, 12, 64, dtype, dev)
+        q = big[:, 2:10]
+        store = torch.full((T, 9, 72), 3.0, dtype=dtype, device=dev)
+        out = store[:, :8, :64]
+        got, lse = run(c, q, rows, out=out)
+        agree(c, q, rows, got, lse)
+        assert (store[:, 8] == 3.0).all() and (store[:, :, 64:] == 3.0).all()
+
+
+def test_other_stream_graph_and_shared_workspace():
+    """A captured call replays on new contents; two graphs that share a
+    workspace run one after the other."""
+    from rai_b200 import paged
+    dev = torch.device("cuda", 0)
+    rows, lens = [1, 3], [2000, 900]
+    cs = [ref.Cache(lens, 2, 128, 16, torch.bfloat16, dev, seed=s) for s in (1, 2)]
+    qs = [make_q(4, 8, 128, torch.bfloat16, dev, seed=s) for s in (3, 4)]
+    starts = ref.starts_of(rows, dev)
+    ws = torch.empty(paged.attention_workspace_bytes(qs[0], cs[0].k, 3), dtype=torch.uint8, device=dev)
+    want = [paged.attention(q, c.k, c.v, c.table, c.kv_len, starts, 3) for q, c in zip(qs, cs)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], [torch.zeros_like(q) for q in qs]
+    with torch.cuda.stream(side):
+        for q, c, o in zip(qs, cs, outs):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                paged.attention(q, c.k, c.v, c.table, c.kv_len, starts, 3, out=o, workspace=ws)
+            graphs.append(g)
+        for _ in range(3):
+            for g in graphs:
+                g.replay()
+    side.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
+    # New lengths in the same memory.
+    cs[0].kv_len.copy_(torch.tensor([1500, 40], dtype=torch.int32))
+    cs[0].lens = [1500, 40]
+    with torch.cuda.stream(side):
+        graphs[0].replay()
+    side.synchronize()
+    agree(cs[0], qs[0], rows, outs[0], None)
+
+
+def test_bad_values_on_the_device_are_cut_and_reported():
+    """Page numbers outside the pool read as masked; lengths and row ranges
+    outside the tensors are cut."""
+    import rai_b200
+    from rai_b200 import paged
+    dev = torch.device("cuda", 0)
+    rows, lens = [1, 2], [100, 64]
+    c = ref.Cache(lens, 2, 64, 16, torch.bfloat16, dev)
+    q = make_q(3, 4, 64, torch.bfloat16, dev)
+    starts = ref.starts_of(rows, dev)
+    want = paged.attention(q, c.k, c.v, c.table, c.kv_len, starts, 2)
+    paged.status()
+    for cell in (-1, c.n_pages, 1 << 30):
+        t = c.table.clone()
+        t[0, 2] = cell
+        got = paged.attention(q, c.k, c.v, t, c.kv_len, starts, 2)
+        with pytest.raises(rai_b200.RaiError):
+            paged.status()
+        assert torch.equal(got[1:], want[1:]) and torch.isfinite(got.float()).all()
+    for bad in ([0, 1, 1000], [-5, 1, 3], [2, 1, 3]):
+        paged.attention(q, c.k, c.v, c.table, c.kv_len, torch.tensor(bad, dtype=torch.int32, device=dev), 2)
+        with pytest.raises(rai_b200.RaiError):
+            paged.status()
+    paged.attention(q, c.k, c.v, c.table, torch.tensor([1 << 30, -4], dtype=torch.int32, device=dev), starts, 2)
+    with pytest.raises(rai_b200.RaiError):
+        paged.status()
+    paged.status()  # the query clears it
+
+
+def test_offsets_past_32_bits():
+    """A page whose elements lie beyond 2^32 bytes of the pool."""
+    from rai_b200 import paged
+    dev = torch.device("cuda", 0)
+    pages, nkv, page, hd = 18000, 8, 64, 256  # 4.7 GB a pool
+    k = torch.zeros((pages, nkv, page, hd), dtype=torch.bfloat16, device=dev)
+    v = torch.zeros((pages, nkv, page, hd), dtype=torch.bfloat16, device=dev)
+    c = ref.Cache([130], nkv, hd, page, torch.bfloat16, dev, extra=0)
+    far = [pages - 1, 16500, pages - 7]
+    for j, p in enumerate(far):
+        k[p], v[p] = c.k[c.rows[0][j]], c.v[c.rows[0][j]]
+    q = make_q(1, 8, hd, torch.bfloat16, dev)
+    table = torch.tensor([far], dtype=torch.int32, device=dev)
+    got = paged.attention(q, k, v, table, c.kv_len, ref.starts_of([1], dev), 1)
+    want = paged.attention(q, c.k, c.v, c.table, c.kv_len, ref.starts_of([1], dev), 1)
+    assert torch.equal(got, want)
