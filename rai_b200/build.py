@@ -18,8 +18,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "librai_gpu.so")
 SOURCES = ["kernels_gemm.cu", "kernels_gemm_tc.cu", "kernels_gemm_tol.cu", "kernels_layers.cu", "kernels_moe.cu", "kernels_sample.cu",
-           "kernels_paged_attn.cu", "kernels_paged_kv.cu", "kernels_beam.cu", "paged_api.cu", "runtime.cu", "convert_host.cpp"]
-HEADERS = ["common.cuh", "errors.h", "kernels.h", "layers.h", "moe.h", "paged.h", "quant.cuh", "raimodel_format.h", "tp.cuh"]
+           "kernels_paged_attn.cu", "kernels_paged_tc.cu", "kernels_paged_kv.cu", "kernels_beam.cu", "paged_api.cu", "runtime.cu", "convert_host.cpp"]
+HEADERS = ["common.cuh", "errors.h", "kernels.h", "layers.h", "moe.h", "paged.h", "paged_attn.cuh", "quant.cuh", "raimodel_format.h", "tp.cuh"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,0 +1,542 @@
+// Attention of a chunk over a paged cache on the 5th-generation tensor cores,
+// for many query rows per KV head (prompts, chunks of prompts): f16 / bf16,
+// head sizes up to 128. The mathematics, the masks and the line of tiles cut
+// over the CTAs are those of kernels_paged_attn.cu.
+//
+// A CTA takes row tiles of 256 flattened rows (group heads x chunk rows) of
+// one KV head as two halves, A and B, of 128 rows, and walks the cache in
+// tiles of 128 tokens:
+//   S = Q K^T   tcgen05.mma, Q and K in shared memory, S in TMEM (f32)
+//   P = 2^(c S - c m), row sums   two warpgroups, one row per thread
+//   O += P V    tcgen05.mma, P in TMEM over S, V in shared memory, O in TMEM
+// The halves take turns: while one warpgroup works on its S, the tensor core
+// runs the other half's P V and next Q K^T. Per tile of both halves that is
+// 2,048 cycles of tensor core and, at 16 exponentials a cycle, 2,048 cycles of
+// the special function units for head size 128, so both bound it.
+//
+// The running maximum is lazy: m only moves (and O is only rescaled, in TMEM)
+// when a row's maximum passes it by more than 2^8; until then probabilities
+// grow up to 2^8, which f32 sums and the 16-bit types hold.
+//
+// Warps: 0-3 and 4-7 softmax of halves A and B, 8 TMEM and MMA issue (one
+// thread), 9-10 producers: K, V and Q by 16-byte asynchronous copies (pages of
+// any size and any strides; slots that no row sees are zero filled), written
+// in the 128-byte swizzle the MMA reads: K and V tiles as 64-column blocks of
+// [token][128 bytes], K-major for Q K^T and N-major for P V. Every wait is
+// bounded; on a timeout all roles stop, what is in flight is waited for and
+// the TMEM columns are released.
+#include <cuda_runtime.h>
+
+#include <mutex>
+
+#include "paged_attn.cuh"
+
+namespace rai {
+
+namespace {
+
+using namespace paged_attn;
+
+constexpr int kTcThreads = 12 * 32;
+constexpr int kProducers = 64;
+
+template <int DT_, int HD_>
+struct Tc {
+  static constexpr int DT = DT_, HD = HD_, MT = 256, NT = 128;
+  static constexpr int kTileB = NT * HD * 2;           // a K or V tile
+  static constexpr int kQB = MT * HD * 2;
+  static constexpr int kSlots = HD == 128 ? 5 : 10;
+  static constexpr int kSmem = kQB + kSlots * kTileB + 1024;
+  static constexpr int kPartFloats = MT * (HD + 2);
+  // A probability is at most 2^8 of the kept maximum's: 2^15 with the factor.
+  static constexpr float kPShift = DT == kF16 ? 7.f : 0.f;
+  static constexpr uint32_t kFmt = DT == kBF16 ? 1u : 0u;
+  // Instruction descriptor: D f32 (bits 4-5 = 1), A and B of one type (7-9,
+  // 10-12), B's major-ness (16), N >> 3 (17-22), M >> 4 (24-28).
+  static constexpr uint32_t kIdescQK = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+  static constexpr uint32_t kIdescPV =
+      (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | (((uint32_t)HD >> 3) << 17) | ((128u >> 4) << 24);
+};
+
+constexpr float kLazy = 8.f;  // log2 units
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+// 128-byte swizzle, rows of 128 bytes, 8-row atoms 1024 bytes apart (SBO);
+// lbo: distance of 64-element blocks of an N-major operand.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void tm_ld32(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Bytes of 16-byte chunk `chunk` (0 .. HD / 8 - 1) of row `row` in a tile of
+// `rows` rows: 64-column blocks, 128-byte swizzle.
+__device__ __forceinline__ uint32_t tile_at(int rows, int row, int chunk) {
+  return (uint32_t)((chunk >> 3) * rows * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+
+// Whether some row of the item may not see some token of the tile that
+// begins at t0.
+__device__ __forceinline__ bool tile_masked(const Item& it, int t0, int nt, int window, const FastDiv& group) {
+  const int p0 = it.len - it.n, plo = p0 + (int)group.quot(it.f0), phi = it.hi - 1;
+  return t0 + nt - 1 > plo || t0 < it.lo || (window > 0 && t0 <= phi - window);
+}
+
+template <typename C, bool CAP>
+__global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ Params p) {
+  constexpr int DT = C::DT, HD = C::HD, MT = C::MT, NT = C::NT;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ long long sh[kPlanWords];
+  __shared__ uint64_t kv_full[C::kSlots], kv_empty[C::kSlots], q_full, q_empty, s_full[2], p_full[2], o_done[2], drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int poison[4];  // ordinal + 1 of an item with masked V values that are not finite
+  const uint32_t sq = (smem_u32(smem_raw) + 1023) & ~1023u, skv = sq + C::kQB;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PagedChunk& ch = p.a.c;
+  uint32_t* err = ch.err;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&kv_full[i], kProducers);
+      mbar_init(&kv_empty[i], 1);
+    }
+    mbar_init(&q_full, kProducers);
+    mbar_init(&q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_done[i], 1);
+    }
+    mbar_init(&drained, 1);
+    for (int i = 0; i < 4; ++i) poison[i] = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const Range rg = plan<MT, NT, kTcThreads>(p, blockIdx.x, sh);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
+  const long long begin = rg.begin, end = rg.end;
+
+  // 3 x 168 registers at launch: 208 for each softmax warpgroup, 88 for the
+  // others (208 + 208 + 88 = 504).
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (begin < end && (warp == 9 || warp == 10)) {
+      // ---------------- producers ----------------
+      const int tid = threadIdx.x - 9 * 32;
+      constexpr int kChunks = HD / 8, kRowsPer = kProducers / kChunks;  // rows of 16-byte chunks at a time
+      constexpr int kLag = 2;  // slots in flight before the oldest is handed over
+      const int chunk = tid % kChunks, r0 = tid / kChunks;
+      const bool in_head = chunk * 8 < ch.hd;
+      Cursor<MT, NT> cur;
+      cur.seek(p, rg, begin);
+      int items = 0;
+      uint32_t n = 0, handed = 0;  // K and V tiles fetched, handed over
+      bool ok = true, fresh = true;
+      // Which of the slots in flight holds a V tile to look through.
+      uint32_t look = 0;  // bit i: fetch n - 1 - i
+      auto hand = [&](int age) {  // the fetch `handed` has landed
+        const uint32_t slot = handed % C::kSlots;
+        if (look >> age & 1u) {
+          const uint32_t base = skv + slot * C::kTileB;
+          bool bad = false;
+          for (int i = 0; i < NT / kRowsPer; ++i) {
+            const uint32_t ad = base + tile_at(NT, r0 + i * kRowsPer, chunk);
+            uint4 w;
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(ad));
+            const uint4 f = make_uint4(finite_or_zero<DT>(w.x), finite_or_zero<DT>(w.y), finite_or_zero<DT>(w.z),
+                                       finite_or_zero<DT>(w.w));
+            if (f.x != w.x || f.y != w.y || f.z != w.z || f.w != w.w) {
+              bad = true;
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(ad), "r"(f.x), "r"(f.y), "r"(f.z), "r"(f.w)
+                           : "memory");
+            }
+          }
+          if (bad) *(volatile int*)&poison[items & 3] = items + 1;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&kv_full[slot]);
+        ++handed;
+      };
+      for (long long at = begin; at < end && ok; ++at) {
+        if (fresh) {
+          // A new item: what is in flight is handed over under the old one's
+          // ordinal, then the query rows are fetched.
+          cp_async_wait<0>();
+          while (handed < n) hand((int)(n - 1 - handed));
+          if (at > begin) {
+            ++items;
+            ok = mbar_wait(&q_empty, (items - 1) & 1, err);
+            if (!ok) break;
+          }
+          const Item& it = cur.it;
+          for (int i = 0; i < MT / kRowsPer; ++i) {
+            const int r = r0 + i * kRowsPer, f = it.f0 + r, qi = (int)p.group_div.quot(f), j = f - qi * p.a.group;
+            const bool real = r < it.nf && in_head;
+            const long long o = (long long)(it.start + qi) * p.a.q_row + (long long)(cur.head * p.a.group + j) * p.a.q_head + chunk * 8;
+            cp_async16_or_zero(sq + tile_at(MT, r, chunk), real ? static_cast<const uint16_t*>(p.a.q) + o : p.a.q, real);
+          }
+          cp_async_commit();
+          cp_async_wait<0>();
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          mbar_arrive(&q_full);
+          fresh = false;
+        }
+        const Item& it = cur.it;
+        const int t0 = (it.first + cur.tile) * NT;
+        // Pages of the tile's tokens: each lane looks up four.
+        int pages[NT / 32];
+#pragma unroll
+        for (int i = 0; i < NT / 32; ++i) {
+          const int t = t0 + lane + 32 * i;
+          pages[i] = t >= it.lo && t < it.hi ? page_of(ch, it.seq, (int)ch.page.quot(t)) : -1;
+        }
+#pragma unroll 1
+        for (int kv = 0; kv < 2 && ok; ++kv) {
+          const uint32_t slot = n % C::kSlots, use = n / C::kSlots;
+          if (use > 0 && !mbar_wait(&kv_empty[slot], (use - 1) & 1, err)) {
+            ok = false;
+            break;
+          }
+          const uint32_t base = skv + slot * C::kTileB;
+          const uint16_t* src = static_cast<const uint16_t*>(kv ? ch.v : ch.k) + (long long)cur.head * (kv ? ch.v_head : ch.k_head) + chunk * 8;
+          const long long sp = kv ? ch.v_page : ch.k_page, ss = kv ? ch.v_slot : ch.k_slot;
+#pragma unroll
+          for (int i = 0; i < NT / kRowsPer; ++i) {
+            const int row = r0 + i * kRowsPer, t = t0 + row;
+            const int page = __shfl_sync(~0u, pages[i * kRowsPer / 32], row & 31);
+            const int in = t - (int)ch.page.quot(t) * (int)ch.page.d;
+            const bool real = page >= 0 && in_head;
+            cp_async16_or_zero(base + tile_at(NT, row, chunk), real ? src + page * sp + in * ss : src, real);
+          }
+          cp_async_commit();
+          look = look << 1 | (kv && tile_masked(it, t0, NT, p.a.window, p.group_div) ? 1u : 0u);
+          ++n;
+          if (n - handed > (uint32_t)kLag) {
+            cp_async_wait<kLag>();
+            hand(kLag);
+          }
+        }
+        if (cur.tile + 1 == it.tiles) fresh = true;
+        cur.next(p);
+      }
+      cp_async_wait<0>();
+      if (ok)
+        while (handed < n) hand((int)(n - 1 - handed));
+    } else if (begin < end && warp == 8) {
+      // ---------------- MMA issue ----------------
+      if (lane == 0) {
+        Cursor<MT, NT> cur;
+        cur.seek(p, rg, begin);
+        bool ok = true;
+        int items = 0;
+        auto qk = [&](int half, uint32_t k) {  // S of half for the CTA's k-th tile
+          const uint32_t a0 = sq + half * 128 * 128, b0 = skv + (2 * k) % C::kSlots * C::kTileB;
+#pragma unroll
+          for (int x = 0; x < HD / 16; ++x) {
+            const uint32_t in = (x & 3) * 32;
+            mma_ss(tmem + half * 128, desc_sw128(a0 + (x >> 2) * MT * 128 + in, 16), desc_sw128(b0 + (x >> 2) * NT * 128 + in, 16),
+                   C::kIdescQK, x > 0);
+          }
+          commit(&s_full[half]);
+        };
+        auto pv = [&](int half, uint32_t k, bool add) {
+          const uint32_t b0 = skv + (2 * k + 1) % C::kSlots * C::kTileB;
+#pragma unroll
+          for (int x = 0; x < NT / 16; ++x)
+            mma_ts(tmem + 256 + half * HD, tmem + half * 128 + x * 8, desc_sw128(b0 + x * 2048, NT * 128), C::kIdescPV, add || x > 0);
+          commit(&o_done[half]);
+        };
+        auto wait_kv = [&](uint32_t i) { return mbar_wait(&kv_full[i % C::kSlots], i / C::kSlots & 1, err); };
+        // Queries, K and V of a tile are waited for once each, before the first
+        // MMA that reads them.
+        const uint32_t tiles = (uint32_t)(end - begin);
+        bool first = true;  // tile k is its item's first here
+        ok = mbar_wait(&q_full, 0, err) && wait_kv(0);
+        if (ok) {
+          fence_after();
+          qk(0, 0);
+          qk(1, 0);
+          commit(&kv_empty[0]);
+          if (cur.tile + 1 == cur.it.tiles || tiles == 1) commit(&q_empty);
+        }
+        for (uint32_t k = 0; k < tiles && ok; ++k) {
+          const bool last = cur.tile + 1 == cur.it.tiles, more = k + 1 < tiles;
+          cur.next(p);
+          ok = wait_kv(2 * k + 1) && mbar_wait(&p_full[0], k & 1, err);
+          if (!ok) break;
+          fence_after();
+          pv(0, k, !first);
+          if (more) {
+            if (last) {
+              ++items;
+              ok = mbar_wait(&q_full, items & 1, err);
+            }
+            ok = ok && wait_kv(2 * k + 2);
+            if (!ok) break;
+            fence_after();
+            qk(0, k + 1);
+          }
+          ok = mbar_wait(&p_full[1], k & 1, err);
+          if (!ok) break;
+          fence_after();
+          pv(1, k, !first);
+          commit(&kv_empty[(2 * k + 1) % C::kSlots]);
+          if (more) {
+            qk(1, k + 1);
+            commit(&kv_empty[(2 * k + 2) % C::kSlots]);
+            // Tile k + 1 is its item's last here: the queries may go.
+            if (cur.tile + 1 == cur.it.tiles || k + 2 == tiles) commit(&q_empty);
+          }
+          first = last;
+        }
+        commit(&drained);
+        mbar_wait(&drained, 0, nullptr);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if (begin < end) {
+      // ---------------- softmax, one row per thread ----------------
+      const int half = warp >> 2, row = threadIdx.x & 127;
+      const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+      const uint32_t ts = tmem + half * 128 + lanes, to = tmem + 256 + half * HD + lanes;
+      Cursor<MT, NT> cur;
+      cur.seek(p, rg, begin);
+      int items = 0;
+      bool ok = true;
+      float m = -INFINITY, l = 0.f;  // m: of the raw scores
+      uint32_t k = 0, k_first = 0;
+      for (long long at = begin; at < end; ++at, ++k) {
+        const Item& it = cur.it;
+        const int f = it.f0 + half * 128 + row, qi = (int)p.group_div.quot(f);
+        const bool real = half * 128 + row < it.nf;
+        const int pos = real ? it.len - it.n + qi : -1;
+        const int t0 = (it.first + cur.tile) * NT;
+        ok = __all_sync(~0u, mbar_wait(&s_full[half], k & 1, err));
+        if (!ok) break;
+        fence_after();
+        uint32_t v[128];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tm_ld32(ts + 32 * x, v + 32 * x);
+        tm_wait_ld();
+        if constexpr (CAP) {
+#pragma unroll
+          for (int x = 0; x < 128; ++x) v[x] = __float_as_uint(capped<DT>(__uint_as_float(v[x]), p.a.scale, p.a.softcap));
+        }
+        if (tile_masked(it, t0, NT, p.a.window, p.group_div)) {
+          const int from = max(it.lo, p.a.window > 0 ? pos - p.a.window + 1 : 0) - t0, till = pos - t0;
+#pragma unroll
+          for (int x = 0; x < 128; ++x)
+            if (x > till || x < from) v[x] = 0xff800000u;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < 128; x += 2) top = fmaxf(top, fmaxf(__uint_as_float(v[x]), __uint_as_float(v[x + 1])));
+        const bool move = top > m && (m == -INFINITY || (top - m) * p.c > kLazy);
+        if (__any_sync(~0u, move)) {
+          const float next = move ? top : m;
+          const float fix = move && m != -INFINITY ? exp2_fast((m - next) * p.c) : 1.f;
+          l *= fix;
+          m = next;
+          if (k > k_first) {
+            ok = __all_sync(~0u, mbar_wait(&o_done[half], (k - 1) & 1, err));
+            if (!ok) break;
+            fence_after();
+#pragma unroll 1
+            for (int x = 0; x < HD; x += 32) {
+              uint32_t o[32];
+              tm_ld32(to + x, o);
+              tm_wait_ld();
+#pragma unroll
+              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * fix);
+              tm_st32(to + x, o);
+            }
+          }
+        }
+        const float mc = (m == -INFINITY ? 0.f : m * p.c) - C::kPShift;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 64; ++x) {
+          const float a = exp2_fast(fmaf(__uint_as_float(v[2 * x]), p.c, -mc));
+          const float b = exp2_fast(fmaf(__uint_as_float(v[2 * x + 1]), p.c, -mc));
+          sum[x & 1] += a;
+          sum[2 + (x & 1)] += b;
+          v[x] = pack<DT>(a, b);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tm_st32(ts, v);
+        tm_st32(ts + 32, v + 32);
+        tm_wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[half]);
+
+        if (cur.tile + 1 == it.tiles || at + 1 == end) {
+          // ---- end of the item, or of this CTA's part of it ----
+          ok = __all_sync(~0u, mbar_wait(&o_done[half], k & 1, err));
+          if (!ok) break;
+          fence_after();
+          const long long item_at = at - cur.tile;
+          const bool whole = item_at >= begin && cur.tile + 1 == it.tiles;
+          const bool poisoned = *(volatile int*)&poison[items & 3] == items + 1;
+          const int r = half * 128 + row, j = f - qi * p.a.group, head = cur.head * p.a.group + j;
+          const float inv = !whole ? 1.f : l > 0.f || l != l ? 1.f / l : 0.f;
+          float* part = p.a.part + (2ll * blockIdx.x + (items ? 1 : 0)) * C::kPartFloats;
+          uint16_t* out = static_cast<uint16_t*>(p.a.out) + (long long)(it.start + qi) * p.a.o_row + (long long)head * p.a.o_head;
+#pragma unroll 1
+          for (int x = 0; x < HD; x += 32) {
+            uint32_t o[32];
+            tm_ld32(to + x, o);
+            tm_wait_ld();
+            if (poisoned && real) {
+              // A row that sees a V value which is not finite gets it after all.
+              const int ta = it.first * NT + (int)max(0ll, begin - item_at) * NT, tb = (it.first + cur.tile + 1) * NT;
+              const int from = max(max(ta, it.lo), p.a.window > 0 ? pos - p.a.window + 1 : 0), till = min(min(tb, it.hi), pos + 1);
+              for (int t = from; t < till; ++t) {
+                if (!tile_masked(it, t / NT * NT, NT, p.a.window, p.group_div)) continue;
+                const int pi = (int)ch.page.quot(t), page = page_of(ch, it.seq, pi);
+                if (page < 0) continue;
+                const long long vo = page * ch.v_page + (long long)cur.head * ch.v_head + (t - pi * (int)ch.page.d) * ch.v_slot;
+#pragma unroll
+                for (int y = 0; y < 32; ++y) {
+                  const float w = x + y < ch.hd ? value<DT>(ch.v, vo + x + y) : 0.f;
+                  if (!(fabsf(w) <= 3.4028235e38f)) o[y] = __float_as_uint(__uint_as_float(o[y]) + w);
+                }
+              }
+            }
+            if (!whole) {
+#pragma unroll
+              for (int y = 0; y < 32; y += 4)
+                *reinterpret_cast<uint4*>(part + r * HD + x + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+            } else if (real) {
+#pragma unroll
+              for (int y = 0; y < 32; y += 8) {
+                uint32_t w[4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z)
+                  w[z] = pack<DT>(__uint_as_float(o[y + 2 * z]) * inv, __uint_as_float(o[y + 2 * z + 1]) * inv);
+                if (x + y < ch.hd) *reinterpret_cast<uint4*>(out + x + y) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            }
+          }
+          if (!whole) {
+            part[MT * HD + r] = m == -INFINITY ? -INFINITY : m * p.c;
+            part[MT * HD + MT + r] = l;
+          } else if (real && p.a.lse) {
+            p.a.lse[(long long)(it.start + qi) * (ch.nkv * p.a.group) + head] =
+                l > 0.f || l != l ? (m * p.c - C::kPShift) * kLn2 + logf(l) : -INFINITY;
+          }
+          fence_before();
+          ++items;
+          m = -INFINITY;
+          l = 0.f;
+          k_first = k + 1;
+        }
+        cur.next(p);
+      }
+    }
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 8) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
+template <typename C, bool CAP>
+cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
+  static std::once_flag once[64];
+  static cudaError_t ready[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::call_once(once[dev], [&] {
+    ready[dev] = cudaFuncSetAttribute(paged_attn_tc_kernel<C, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  });
+  if (ready[dev] != cudaSuccess) return ready[dev];
+  Params p;
+  p.a = a;
+  const long long frows = (long long)a.c.max_rows * a.group;
+  p.row_tiles = (int)((frows + C::MT - 1) / C::MT);
+  p.row_tiles_div = FastDiv(p.row_tiles);
+  p.group_div = FastDiv(a.group);
+  p.grid = device_sm_count();
+  p.whole = false;
+  p.min_tiles = 4;
+  p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
+  e = launch_pdl(paged_attn_tc_kernel<C, CAP>, dim3(p.grid), dim3(kTcThreads), C::kSmem, s, p);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(paged_combine_kernel<C>, dim3(p.grid - 1, combine_grid_y(C::MT)), dim3(kCombineThreads), 0, s, p);
+}
+
+}  // namespace
+
+bool paged_attention_tc_takes(const AttnArgs& a) {
+  return a.dtype != kF32 && a.c.hd <= 128 && (long long)a.c.max_rows * a.group > 64;
+}
+
+size_t paged_attention_tc_workspace(const AttnArgs& a) {
+  return 2ull * device_sm_count() * (a.c.hd <= 64 ? Tc<kBF16, 64>::kPartFloats : Tc<kBF16, 128>::kPartFloats) * 4;
+}
+
+cudaError_t paged_attention_tc(const AttnArgs& a, cudaStream_t s) {
+#define RAI_TC(DT, HD) (a.softcap > 0.f ? launch<Tc<DT, HD>, true>(a, s) : launch<Tc<DT, HD>, false>(a, s))
+  if (a.dtype == kF16) return a.c.hd <= 64 ? RAI_TC(kF16, 64) : RAI_TC(kF16, 128);
+  return a.c.hd <= 64 ? RAI_TC(kBF16, 64) : RAI_TC(kBF16, 128);
+#undef RAI_TC
+}
+
+}  // namespace rai
