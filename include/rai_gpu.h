@@ -396,6 +396,7 @@ typedef struct {
   void* workspace;
   size_t workspace_bytes;  /* rai_gpu_paged_attention_workspace_bytes */
 } rai_paged_attention;
+/* By the sizes and types in args alone; may be 0. */
 RAI_API size_t rai_gpu_paged_attention_workspace_bytes(const rai_paged_attention* args);
 RAI_API int rai_gpu_paged_attention(const rai_paged_attention* args, void* stream);
 

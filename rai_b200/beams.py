@@ -13,7 +13,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import native
-from .paged import _device, _dtype, _ints, _launch
+from .paged import _device, _dtype, _ints, _launch, lib
 
 _ARGS = struct.Struct("2Qq6Q4Q2q5IiI4x2Q")
 
@@ -65,8 +65,8 @@ def select(logits: torch.Tensor, scores: torch.Tensor, *, keep: Optional[int] = 
     if b == 0 or n == 0 or v == 0:
         raise ValueError("logits: a size is zero")
     # One allocation for the float outputs, one for the integer ones.
-    fl = torch.empty((b * (keep + n),), dtype=torch.float32, device=logits.device)
-    it = torch.empty((2 * b * (keep + n),), dtype=torch.int32, device=logits.device)
+    fl = scores.new_empty((b * (keep + n),))
+    it = scores.new_empty((2 * b * (keep + n),), dtype=torch.int32)
     cs, sc = fl.split([b * keep, b * n])
     cb, ct, pa, tk = it.split([b * keep, b * keep, b * n, b * n])
     hist = [0, 0, 0, 0, 0, 0, 0]
@@ -81,13 +81,13 @@ def select(logits: torch.Tensor, scores: torch.Tensor, *, keep: Optional[int] = 
         hist = [_ints("history", history, b * n, None), _ints("hist_len", hist_len, b * n), out_h.data_ptr(), out_n.data_ptr(),
                 stride, out_h.stride(0) if b * n > 1 else max(out_h.shape[-1], 1), history.shape[1]]
     if workspace is None:
-        workspace = torch.empty(_workspace(dev, b, n, v, keep), dtype=torch.uint8, device=logits.device)
+        workspace = scores.new_empty((_workspace(dev, b, n, v, keep),), dtype=torch.uint8)
     elif workspace.get_device() != dev or not workspace.is_contiguous():
         raise ValueError("workspace: contiguous, on the logits' device")
     args = _ARGS.pack(logits.data_ptr(), scores.data_ptr(), row, cs.data_ptr(), cb.data_ptr(), ct.data_ptr(), sc.data_ptr(),
                       pa.data_ptr(), tk.data_ptr(), *hist, b, n, v, keep, eos, dtype, workspace.data_ptr(),
                       workspace.numel() * workspace.element_size())
-    _launch(dev, native.lib().rai_gpu_beam_select, args)
+    _launch(dev, lib().rai_gpu_beam_select, args)
     return BeamChoice(cs.view(b, keep), cb.view(b, keep), ct.view(b, keep), sc.view(b, n), pa.view(b, n), tk.view(b, n),
                       out_h, out_n)
 

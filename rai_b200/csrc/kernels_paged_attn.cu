@@ -71,33 +71,45 @@ __device__ __forceinline__ uint32_t swz(int row, int chunk) {  // 16-byte chunk 
   return (uint32_t)row * C::kRowB + (uint32_t)((chunk ^ (row & 7)) << 4);
 }
 
+// K and V of the cursor's tile, from pages looked up a tile ahead. Each lane
+// knows the offsets of NT / 32 tokens; a token's copies get its offset by a
+// shuffle, eight copies' addresses at a time.
 template <typename C>
-__device__ __forceinline__ void load_tile(const Params& p, const Cursor<C::MT, C::NT>& cur, uint32_t sk, uint32_t sv) {
+__device__ __forceinline__ void load_tile(const Params& p, const Cursor<C::MT, C::NT>& cur, TilePages<C::NT>& pages,
+                                          uint32_t sk, uint32_t sv) {
   constexpr int kChunks = C::kRowB / 16;  // per row
-  constexpr int kRowsPer = kThreads / kChunks;
+  constexpr int kRowsPer = kThreads / kChunks, kIter = C::NT / kRowsPer;
   const PagedChunk& c = p.a.c;
-  const int chunk = threadIdx.x % kChunks, r0 = threadIdx.x / kChunks;
+  const int lane = threadIdx.x & 31, chunk = threadIdx.x % kChunks, r0 = threadIdx.x / kChunks;
   const int t0 = (cur.it.first + cur.tile) * C::NT;
   const bool in_head = chunk * 16 < c.hd * C::kElt;
-  const char* k = static_cast<const char*>(c.k) + (long long)cur.head * c.k_head * C::kElt + chunk * 16;
-  const char* v = static_cast<const char*>(c.v) + (long long)cur.head * c.v_head * C::kElt + chunk * 16;
+  pages.check(c, cur.it, t0, lane);
 #pragma unroll
-  for (int i = 0; i < C::NT / kRowsPer; ++i) {
-    const int row = r0 + i * kRowsPer, t = t0 + row;
-    bool real = t >= cur.it.lo && t < cur.it.hi;
-    long long ko = 0, vo = 0;
-    if (real) {
-      const int pi = (int)c.page.quot(t);
-      const int page = page_of(c, cur.it.seq, pi), slot = t - pi * (int)c.page.d;
-      real = page >= 0 && in_head;
-      if (real) {
-        ko = (page * c.k_page + slot * c.k_slot) * C::kElt;
-        vo = (page * c.v_page + slot * c.v_slot) * C::kElt;
+  for (int kv = 0; kv < 2; ++kv) {
+    const char* base = static_cast<const char*>(kv ? c.v : c.k) + (long long)cur.head * (kv ? c.v_head : c.k_head) * C::kElt + chunk * 16;
+    long long off[C::NT / 32];
+    pages.offsets(c, t0, lane, kv ? c.v_page : c.k_page, kv ? c.v_slot : c.k_slot, off);
+    constexpr int kB = kIter < 8 ? kIter : 8;
+#pragma unroll
+    for (int i0 = 0; i0 < kIter; i0 += kB) {
+      long long o[kB];
+#pragma unroll
+      for (int i = 0; i < kB; ++i) {
+        const int row = r0 + (i0 + i) * kRowsPer;
+        // The lane's rows of one pass lie in one half of the tile or in
+        // both (fewer chunks a row than lanes).
+        long long x = __shfl_sync(~0u, off[0], row & 31);
+#pragma unroll
+        for (int y = 1; y < C::NT / 32; ++y) {
+          const long long z = __shfl_sync(~0u, off[y], row & 31);
+          if (row / 32 == y) x = z;
+        }
+        o[i] = in_head ? x : -1;
       }
+#pragma unroll
+      for (int i = 0; i < kB; ++i)
+        cp_async16_or_zero((kv ? sv : sk) + swz<C>(r0 + (i0 + i) * kRowsPer, chunk), o[i] >= 0 ? base + o[i] * C::kElt : base, o[i] >= 0);
     }
-    const uint32_t o = swz<C>(row, chunk);
-    cp_async16_or_zero(sk + o, real ? k + ko : k, real);
-    cp_async16_or_zero(sv + o, real ? v + vo : v, real);
   }
 }
 
@@ -171,18 +183,25 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
   pdl_launch_dependents();
   const Range rg = plan<MT, NT, kThreads>(p, blockIdx.x, sh);
   const long long begin = rg.begin, end = rg.end;
-  if (begin >= end) return;
+  if (begin >= end) {
+    if (threadIdx.x == 0 && !p.whole) reinterpret_cast<Cut*>(p.a.part)[blockIdx.x] = Cut{};
+    return;
+  }
 
   Cursor<MT, NT> ld, cur;
   ld.seek(p, rg, begin);
   cur = ld;
+  if (threadIdx.x == 0 && !p.whole) leave_cut<MT, NT>(p, rg, cur, blockIdx.x);
   long long loaded = begin;
+  TilePages<NT> pages;
+  pages.fetch(ch, ld.it, (ld.it.first + ld.tile) * NT, lane);
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) {
     if (loaded < end) {
-      load_tile<C>(p, ld, base + s * 2 * C::kTileB, base + s * 2 * C::kTileB + C::kTileB);
+      load_tile<C>(p, ld, pages, base + s * 2 * C::kTileB, base + s * 2 * C::kTileB + C::kTileB);
       ++loaded;
       ld.next(p);
+      if (loaded < end) pages.fetch(ch, ld.it, (ld.it.first + ld.tile) * NT, lane);
     }
     cp_async_commit();
   }
@@ -246,9 +265,10 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
     // The stage that the last step read is free: fetch ahead.
     if (loaded < end) {
       const uint32_t st = base + (uint32_t)((loaded - begin) % S) * 2 * C::kTileB;
-      load_tile<C>(p, ld, st, st + C::kTileB);
+      load_tile<C>(p, ld, pages, st, st + C::kTileB);
       ++loaded;
       ld.next(p);
+      if (loaded < end) pages.fetch(ch, ld.it, (ld.it.first + ld.tile) * NT, lane);
     }
     cp_async_commit();
     const uint32_t sk = base + (uint32_t)((at - begin) % S) * 2 * C::kTileB, sv = sk + C::kTileB;
@@ -460,6 +480,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
             const int pi = (int)ch.page.quot(t), page = page_of(ch, it.seq, pi);
             if (page < 0) continue;
             const long long vo = page * ch.v_page + (long long)cur.head * ch.v_head + (t - pi * (int)ch.page.d) * ch.v_slot;
+#pragma unroll
             for (int h = 0; h < 2; ++h) {
               if (t > pos[h] || (p.a.window > 0 && t <= pos[h] - p.a.window)) continue;
 #pragma unroll
@@ -497,7 +518,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
                   l[h] > 0.f || l[h] != l[h] ? (m[h] * p.c - C::kPShift) * kLn2 + logf(l[h]) : -INFINITY;
           }
         } else {
-          float* part = p.a.part + (2ll * blockIdx.x + first_slot) * C::kPartFloats;
+          float* part = part_of(p, C::kPartFloats, blockIdx.x, first_slot);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int r = wm * 16 + g + 8 * h;
@@ -544,6 +565,10 @@ auto with_cfg(int dtype, int hd, int rows, F f) {
 constexpr int kMinTiles = 4;
 // Caches of at most this many tiles a sequence are not cut.
 constexpr int kWholeTiles = 8;
+template <typename C>
+bool whole_items(const AttnArgs& a) {
+  return ((long long)a.c.max_pages * a.c.page.d + C::NT - 1) / C::NT <= kWholeTiles;
+}
 
 template <typename C>
 cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
@@ -563,7 +588,7 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
   p.row_tiles = (int)((frows + C::MT - 1) / C::MT);
   p.row_tiles_div = FastDiv(p.row_tiles);
   p.group_div = FastDiv(a.group);
-  p.whole = ((long long)a.c.max_pages * a.c.page.d + C::NT - 1) / C::NT <= kWholeTiles;
+  p.whole = whole_items<C>(a);
   p.min_tiles = p.whole ? 1 : kMinTiles;
   p.grid = device_sm_count() * resident_ctas<C>();
   p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
@@ -579,7 +604,9 @@ size_t paged_attention_workspace(const AttnArgs& a) {
   const long long frows = (long long)a.c.max_rows * a.group;
   return with_cfg(a.dtype, a.c.hd, (int)(frows < 64 ? frows : 64), [&](auto c) -> size_t {
     using C = decltype(c);
-    return 2ull * device_sm_count() * resident_ctas<C>() * C::kPartFloats * 4;
+    if (whole_items<C>(a)) return 0;  // nothing is cut
+    const int grid = device_sm_count() * resident_ctas<C>();
+    return cut_bytes(grid) + 2ull * grid * C::kPartFloats * 4;
   });
 }
 

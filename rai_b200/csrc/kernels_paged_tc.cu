@@ -110,6 +110,25 @@ __device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* v) {
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Bounded wait (about a second of SM clock), polling: a wait with a suspend
+// hint wakes late.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, uint32_t* err) {
+  const uint32_t a = smem_u32(bar);
+  const long long t0 = clock64();
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (clock64() - t0 > 2000000000ll) break;
+  }
+  if (err) atomicOr(err, kErrWaitTimeout);
+  return false;
+}
+
 // Bytes of 16-byte chunk `chunk` (0 .. HD / 8 - 1) of row `row` in a tile of
 // `rows` rows: 64-column blocks, 128-byte swizzle.
 __device__ __forceinline__ uint32_t tile_at(int rows, int row, int chunk) {
@@ -168,6 +187,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 
   // 3 x 168 registers at launch: 208 for each softmax warpgroup, 88 for the
   // others (208 + 208 + 88 = 504).
+  if (begin >= end && threadIdx.x == 0) reinterpret_cast<Cut*>(p.a.part)[blockIdx.x] = Cut{};
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (begin < end && (warp == 9 || warp == 10)) {
@@ -179,6 +199,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       const bool in_head = chunk * 8 < ch.hd;
       Cursor<MT, NT> cur;
       cur.seek(p, rg, begin);
+      if (tid == 0) leave_cut<MT, NT>(p, rg, cur, blockIdx.x);
+      TilePages<NT> pages;
+      pages.fetch(ch, cur.it, (cur.it.first + cur.tile) * NT, lane);
       int items = 0;
       uint32_t n = 0, handed = 0;  // K and V tiles fetched, handed over
       bool ok = true, fresh = true;
@@ -215,7 +238,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
           while (handed < n) hand((int)(n - 1 - handed));
           if (at > begin) {
             ++items;
-            ok = mbar_wait(&q_empty, (items - 1) & 1, err);
+            ok = wait_bar(&q_empty, (items - 1) & 1, err);
             if (!ok) break;
           }
           const Item& it = cur.it;
@@ -233,30 +256,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         }
         const Item& it = cur.it;
         const int t0 = (it.first + cur.tile) * NT;
-        // Pages of the tile's tokens: each lane looks up four.
-        int pages[NT / 32];
-#pragma unroll
-        for (int i = 0; i < NT / 32; ++i) {
-          const int t = t0 + lane + 32 * i;
-          pages[i] = t >= it.lo && t < it.hi ? page_of(ch, it.seq, (int)ch.page.quot(t)) : -1;
-        }
+        pages.check(ch, it, t0, lane);
 #pragma unroll 1
         for (int kv = 0; kv < 2 && ok; ++kv) {
           const uint32_t slot = n % C::kSlots, use = n / C::kSlots;
-          if (use > 0 && !mbar_wait(&kv_empty[slot], (use - 1) & 1, err)) {
+          if (use > 0 && !wait_bar(&kv_empty[slot], (use - 1) & 1, err)) {
             ok = false;
             break;
           }
           const uint32_t base = skv + slot * C::kTileB;
           const uint16_t* src = static_cast<const uint16_t*>(kv ? ch.v : ch.k) + (long long)cur.head * (kv ? ch.v_head : ch.k_head) + chunk * 8;
-          const long long sp = kv ? ch.v_page : ch.k_page, ss = kv ? ch.v_slot : ch.k_slot;
+          long long off[NT / 32];
+          pages.offsets(ch, t0, lane, kv ? ch.v_page : ch.k_page, kv ? ch.v_slot : ch.k_slot, off);
+          // Eight copies' addresses at a time: their shuffles overlap.
 #pragma unroll
-          for (int i = 0; i < NT / kRowsPer; ++i) {
-            const int row = r0 + i * kRowsPer, t = t0 + row;
-            const int page = __shfl_sync(~0u, pages[i * kRowsPer / 32], row & 31);
-            const int in = t - (int)ch.page.quot(t) * (int)ch.page.d;
-            const bool real = page >= 0 && in_head;
-            cp_async16_or_zero(base + tile_at(NT, row, chunk), real ? src + page * sp + in * ss : src, real);
+          for (int i0 = 0; i0 < NT / kRowsPer; i0 += 8) {
+            long long o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int row = r0 + (i0 + i) * kRowsPer;
+              const long long x = __shfl_sync(~0u, off[(i0 + i) * kRowsPer / 32], row & 31);
+              o[i] = in_head ? x : -1;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              cp_async16_or_zero(base + tile_at(NT, r0 + (i0 + i) * kRowsPer, chunk), o[i] >= 0 ? src + o[i] : src, o[i] >= 0);
           }
           cp_async_commit();
           look = look << 1 | (kv && tile_masked(it, t0, NT, p.a.window, p.group_div) ? 1u : 0u);
@@ -268,6 +292,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         }
         if (cur.tile + 1 == it.tiles) fresh = true;
         cur.next(p);
+        if (at + 1 < end) pages.fetch(ch, cur.it, (cur.it.first + cur.tile) * NT, lane);
       }
       cp_async_wait<0>();
       if (ok)
@@ -296,12 +321,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             mma_ts(tmem + 256 + half * HD, tmem + half * 128 + x * 8, desc_sw128(b0 + x * 2048, NT * 128), C::kIdescPV, add || x > 0);
           commit(&o_done[half]);
         };
-        auto wait_kv = [&](uint32_t i) { return mbar_wait(&kv_full[i % C::kSlots], i / C::kSlots & 1, err); };
+        auto wait_kv = [&](uint32_t i) { return wait_bar(&kv_full[i % C::kSlots], i / C::kSlots & 1, err); };
         // Queries, K and V of a tile are waited for once each, before the first
         // MMA that reads them.
         const uint32_t tiles = (uint32_t)(end - begin);
         bool first = true;  // tile k is its item's first here
-        ok = mbar_wait(&q_full, 0, err) && wait_kv(0);
+        ok = wait_bar(&q_full, 0, err) && wait_kv(0);
         if (ok) {
           fence_after();
           qk(0, 0);
@@ -312,21 +337,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         for (uint32_t k = 0; k < tiles && ok; ++k) {
           const bool last = cur.tile + 1 == cur.it.tiles, more = k + 1 < tiles;
           cur.next(p);
-          ok = wait_kv(2 * k + 1) && mbar_wait(&p_full[0], k & 1, err);
+          ok = wait_kv(2 * k + 1) && wait_bar(&p_full[0], k & 1, err);
           if (!ok) break;
           fence_after();
           pv(0, k, !first);
           if (more) {
             if (last) {
               ++items;
-              ok = mbar_wait(&q_full, items & 1, err);
+              ok = wait_bar(&q_full, items & 1, err);
             }
             ok = ok && wait_kv(2 * k + 2);
             if (!ok) break;
             fence_after();
             qk(0, k + 1);
           }
-          ok = mbar_wait(&p_full[1], k & 1, err);
+          ok = wait_bar(&p_full[1], k & 1, err);
           if (!ok) break;
           fence_after();
           pv(1, k, !first);
@@ -340,7 +365,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
           first = last;
         }
         commit(&drained);
-        mbar_wait(&drained, 0, nullptr);
+        wait_bar(&drained, 0, nullptr);
       }
     }
   } else {
@@ -362,7 +387,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         const bool real = half * 128 + row < it.nf;
         const int pos = real ? it.len - it.n + qi : -1;
         const int t0 = (it.first + cur.tile) * NT;
-        ok = __all_sync(~0u, mbar_wait(&s_full[half], k & 1, err));
+        ok = __all_sync(~0u, wait_bar(&s_full[half], k & 1, err));
         if (!ok) break;
         fence_after();
         uint32_t v[128];
@@ -389,7 +414,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
           l *= fix;
           m = next;
           if (k > k_first) {
-            ok = __all_sync(~0u, mbar_wait(&o_done[half], (k - 1) & 1, err));
+            ok = __all_sync(~0u, wait_bar(&o_done[half], (k - 1) & 1, err));
             if (!ok) break;
             fence_after();
 #pragma unroll 1
@@ -423,7 +448,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 
         if (cur.tile + 1 == it.tiles || at + 1 == end) {
           // ---- end of the item, or of this CTA's part of it ----
-          ok = __all_sync(~0u, mbar_wait(&o_done[half], k & 1, err));
+          ok = __all_sync(~0u, wait_bar(&o_done[half], k & 1, err));
           if (!ok) break;
           fence_after();
           const long long item_at = at - cur.tile;
@@ -431,7 +456,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
           const bool poisoned = *(volatile int*)&poison[items & 3] == items + 1;
           const int r = half * 128 + row, j = f - qi * p.a.group, head = cur.head * p.a.group + j;
           const float inv = !whole ? 1.f : l > 0.f || l != l ? 1.f / l : 0.f;
-          float* part = p.a.part + (2ll * blockIdx.x + (items ? 1 : 0)) * C::kPartFloats;
+          float* part = part_of(p, C::kPartFloats, blockIdx.x, items ? 1 : 0);
           uint16_t* out = static_cast<uint16_t*>(p.a.out) + (long long)(it.start + qi) * p.a.o_row + (long long)head * p.a.o_head;
 #pragma unroll 1
           for (int x = 0; x < HD; x += 32) {
@@ -529,7 +554,7 @@ bool paged_attention_tc_takes(const AttnArgs& a) {
 }
 
 size_t paged_attention_tc_workspace(const AttnArgs& a) {
-  return 2ull * device_sm_count() * (a.c.hd <= 64 ? Tc<kBF16, 64>::kPartFloats : Tc<kBF16, 128>::kPartFloats) * 4;
+  return cut_bytes(device_sm_count()) + 2ull * device_sm_count() * (a.c.hd <= 64 ? Tc<kBF16, 64>::kPartFloats : Tc<kBF16, 128>::kPartFloats) * 4;
 }
 
 cudaError_t paged_attention_tc(const AttnArgs& a, cudaStream_t s) {

@@ -133,6 +133,7 @@ size_t rai_gpu_paged_attention_workspace_bytes(const rai_paged_attention* a) {
   if (!a || !a->chunk.n_kv_heads || !a->n_heads) return 0;
   rai::AttnArgs o;
   o.c.hd = (int)a->chunk.head_dim, o.c.max_rows = (int)a->chunk.max_rows;
+  o.c.max_pages = (int)a->chunk.max_pages, o.c.page.d = a->chunk.page_size;
   o.group = (int)(a->n_heads / a->chunk.n_kv_heads);
   o.dtype = (int)a->chunk.dtype;
   return rai::paged_attention_workspace(o);
@@ -142,7 +143,8 @@ int rai_gpu_paged_attention(const rai_paged_attention* a, void* stream) {
   return guarded([&] {
     rai::AttnArgs o;
     if (int rc = attention_args(a, &o)) return rc;
-    if (!o.part || !aligned(o.part, 16) || o.part_bytes < rai::paged_attention_workspace(o))
+    const size_t need = rai::paged_attention_workspace(o);
+    if (need && (!o.part || !aligned(o.part, 16) || o.part_bytes < need))
       return bad("workspace is too small or not on a 16-byte boundary");
     if (int rc = rai::kernel_status_word(&o.c.err)) return rc;
     return done(rai::paged_attention(o, static_cast<cudaStream_t>(stream)));

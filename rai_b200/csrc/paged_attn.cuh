@@ -137,6 +137,41 @@ struct Cursor {
   }
 };
 
+// The pages of a tile's NT tokens, NT / 32 per lane. fetch() only issues the
+// loads, a tile ahead of their use; check() reports numbers outside the pool
+// and leaves -1 there and for tokens that no row of the item sees.
+template <int NT>
+struct TilePages {
+  int page[NT / 32];
+  __device__ __forceinline__ void fetch(const PagedChunk& c, const Item& it, int t0, int lane) {
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) {
+      const int t = t0 + lane + 32 * i;
+      page[i] = -1;
+      if (t >= it.lo && t < it.hi) page[i] = __ldg(c.table + (long long)it.seq * c.table_stride + c.page.quot(t));
+    }
+  }
+  __device__ __forceinline__ void check(const PagedChunk& c, const Item& it, int t0, int lane) {
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) {
+      const int t = t0 + lane + 32 * i;
+      if (t >= it.lo && t < it.hi && (unsigned)page[i] >= (unsigned)c.n_pages) {
+        atomicOr(c.err, kErrBadInput);
+        page[i] = -1;
+      }
+    }
+  }
+  // Offset in elements of each of the lane's tokens, -1 without a page.
+  __device__ __forceinline__ void offsets(const PagedChunk& c, int t0, int lane, long long page_stride, long long slot_stride,
+                                          long long (&off)[NT / 32]) const {
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) {
+      const int t = t0 + lane + 32 * i, slot = t - (int)c.page.quot(t) * (int)c.page.d;
+      off[i] = page[i] >= 0 ? page[i] * page_stride + slot * slot_stride : -1;
+    }
+  }
+};
+
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
@@ -186,54 +221,82 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
   }
 }
 
-constexpr int kCombineThreads = 128;
-constexpr int combine_grid_y(int mt) { return mt / 4 < 16 ? mt / 4 : 16; }
+// What a CTA of the main kernel leaves for the join: whether the cut at its
+// first tile is the first one through an item, and that item.
+struct Cut {
+  int first;       // 0: nothing to join here
+  int last;        // the item's parts are in CTAs b - 1 .. last
+  int slot0;       // the part's slot in CTA b - 1
+  int start, f0, nf, head, pad;
+};
+constexpr size_t cut_bytes(int grid) { return (size_t)grid * sizeof(Cut); }
 
-// Joins the parts of items that the cut between CTAs b - 1 and b goes
-// through first (b = blockIdx.x + 1); the CTAs of one b share the tile's rows.
+template <int MT, int NT>
+__device__ __forceinline__ void leave_cut(const Params& p, const Range& rg, const Cursor<MT, NT>& cur, int cta) {
+  Cut c = {};
+  if (rg.begin < rg.total && !p.whole && cta > 0) {
+    const long long at = rg.begin, start = at - cur.tile, stop = start + cur.it.tiles;
+    if (start != at && start >= at - rg.per) {
+      c.first = 1;
+      c.last = (int)((stop - 1) / rg.per);
+      c.slot0 = start == at - rg.per ? 0 : 1;
+      c.start = cur.it.start, c.f0 = cur.it.f0, c.nf = cur.it.nf, c.head = cur.head;
+    }
+  }
+  reinterpret_cast<Cut*>(p.a.part)[cta] = c;
+}
+__device__ __forceinline__ float* part_of(const Params& p, int floats, int cta, int slot) {
+  return p.a.part + cut_bytes(p.grid) / 4 + (2ll * cta + slot) * floats;
+}
+
+constexpr int kCombineThreads = 128;
+
+// Joins the parts of the item whose first cut is at the beginning of CTA
+// b = blockIdx.x + 1; each warp takes rows of the tile. Bound by latency: a
+// lane finds the weight of one part, and the parts' loads are independent.
 template <typename C>
 __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const __grid_constant__ Params p) {
-  constexpr int HD = C::HD, MT = C::MT, NT = C::NT;
-  __shared__ long long sh[kPlanWords];
+  constexpr int HD = C::HD, MT = C::MT, PL = HD / 32;  // columns per lane
   pdl_wait_prior();
   pdl_launch_dependents();
   const int b = blockIdx.x + 1;
-  const Range rg = plan<MT, NT, kCombineThreads>(p, b, sh);
-  const long long at = rg.begin;
-  if (at >= rg.total) return;
-  Cursor<MT, NT> cur;
-  cur.seek(p, rg, at);
-  const long long start = at - cur.tile, stop = start + cur.it.tiles;
-  if (start == at || start < at - rg.per) return;  // not cut here, or cut before
-  const int last = (int)((stop - 1) / rg.per);     // parts: CTAs b - 1 .. last
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto part = [&](int cta) {
-    const bool head = cta >= b || start == (long long)cta * rg.per;  // the CTA's first item
-    return p.a.part + (2ll * cta + (head ? 0 : 1)) * C::kPartFloats;
-  };
-  for (int r = blockIdx.y * 4 + warp; r < cur.it.nf; r += gridDim.y * 4) {
+  const Cut cut = reinterpret_cast<const Cut*>(p.a.part)[b];
+  if (!cut.first) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = cut.last - b + 2;
+  auto part = [&](int i) { return part_of(p, C::kPartFloats, b - 1 + i, i == 0 ? cut.slot0 : 0); };
+  for (int r = blockIdx.y * (kCombineThreads / 32) + warp; r < cut.nf; r += gridDim.y * (kCombineThreads / 32)) {
     float top = -INFINITY;
-    for (int cta = b - 1 + lane; cta <= last; cta += 32) top = fmaxf(top, part(cta)[MT * HD + r]);
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, part(i)[MT * HD + r]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
     const float mc = top == -INFINITY ? 0.f : top;
-    constexpr int PL = HD / 32;  // columns per lane
     float acc[PL] = {}, l = 0.f;
-    for (int cta = b - 1; cta <= last; ++cta) {
-      const float* x = part(cta);
-      const float w = exp2_fast(x[MT * HD + r] - mc);
-      l += x[MT * HD + MT + r] * w;
-      if (w != 0.f)  // a part of which the row sees nothing
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+      float mine = 0.f, w = 0.f;
+      if (i0 + lane < parts) {
+        const float* x = part(i0 + lane) + MT * HD + r;
+        w = exp2_fast(x[0] - mc);
+        mine = x[MT] * w;
+      }
+      const int n = min(32, parts - i0);
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float wi = __shfl_sync(~0u, w, i);
+        l += __shfl_sync(~0u, mine, i);
+        const float* x = part(i0 + i) + r * HD;
 #pragma unroll
         for (int e = 0; e < PL / 2; ++e) {
-          const float2 v = *reinterpret_cast<const float2*>(x + r * HD + e * 64 + lane * 2);
-          acc[2 * e] += v.x * w;
-          acc[2 * e + 1] += v.y * w;
+          const float2 v = *reinterpret_cast<const float2*>(x + e * 64 + lane * 2);
+          if (wi != 0.f) {  // else the row sees nothing of the part
+            acc[2 * e] += v.x * wi;
+            acc[2 * e + 1] += v.y * wi;
+          }
         }
+      }
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    const int f = cur.it.f0 + r, i = (int)p.group_div.quot(f), head = cur.head * p.a.group + f - i * p.a.group;
-    const long long o = (long long)(cur.it.start + i) * p.a.o_row + (long long)head * p.a.o_head;
+    const int f = cut.f0 + r, i = (int)p.group_div.quot(f), head = cut.head * p.a.group + f - i * p.a.group;
+    const long long o = (long long)(cut.start + i) * p.a.o_row + (long long)head * p.a.o_head;
 #pragma unroll
     for (int e = 0; e < PL / 2; ++e) {
       const int col = e * 64 + lane * 2;
@@ -245,10 +308,11 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const __
             pack<C::DT>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
     }
     if (p.a.lse && lane == 0)
-      p.a.lse[(long long)(cur.it.start + i) * (p.a.c.nkv * p.a.group) + head] =
+      p.a.lse[(long long)(cut.start + i) * (p.a.c.nkv * p.a.group) + head] =
           l > 0.f || l != l ? (mc - C::kPShift) * kLn2 + logf(l) : -INFINITY;
   }
 }
+constexpr int combine_grid_y(int mt) { return mt / 4 < 32 ? mt / 4 : 32; }
 
 }  // namespace paged_attn
 }  // namespace rai

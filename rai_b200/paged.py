@@ -55,24 +55,41 @@ def _device(*tensors: Tuple[str, torch.Tensor]) -> int:
     return dev
 
 
+_lib = None  # native.lib(), looked up once
+_current_device = torch.cuda.current_device
+# The handle of a device's current stream, without the wrapper object that
+# torch.cuda.current_stream makes (1 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+
+
+def lib():
+    global _lib
+    if _lib is None:
+        _lib = native.lib()
+    return _lib
+
+
 def _launch(dev: int, fn, *args) -> None:
     """fn(*args, stream) with the tensors' device current, on its current
     torch stream."""
-    if dev == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+    if dev == _current_device():
+        rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        check(rc)
 
 
 def _ints(name: str, t: torch.Tensor, *shape: Optional[int]) -> int:
     """Address of an int32 tensor of this shape, its last dimension dense."""
-    if t.dtype != torch.int32 or t.dim() != len(shape):
+    got = t.shape
+    if t.dtype is not torch.int32 or len(got) != len(shape):
         raise ValueError(f"{name}: an int32 tensor of {len(shape)} dimension(s)")
-    for got, want in zip(t.shape, shape):
-        if want is not None and got != want:
-            raise ValueError(f"{name}: shape {tuple(t.shape)} does not fit the other arguments")
-    if shape and t.shape[-1] > 1 and t.stride(-1) != 1:
+    for a, b in zip(got, shape):
+        if b is not None and a != b:
+            raise ValueError(f"{name}: shape {tuple(got)} does not fit the other arguments")
+    if not t.is_contiguous() and got[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name}: the last dimension has to be contiguous")
     return t.data_ptr()
 
@@ -82,41 +99,47 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
 
 
-def _rows3(name: str, t: torch.Tensor, heads: Optional[int], dim: int) -> None:
-    if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name}: [rows, heads, head_dim] that fits the pages, not {tuple(t.shape)}")
-    if t.stride(2) != 1 and dim > 1:
+def _rows3(name: str, t: torch.Tensor, heads: Optional[int], dim: int):
+    """The strides of a tensor of rows."""
+    shape, st = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name}: [rows, heads, head_dim] that fits the pages, not {tuple(shape)}")
+    if st[2] != 1 and dim > 1:
         raise ValueError(f"{name}: head_dim has to be contiguous")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name}: this operator has no gradient; call it under torch.no_grad()")
+    return st
 
 
 def _chunk(k_pages, v_pages, table, kv_len, q_start, rows: int, max_rows: int, dtype: int):
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+    shape = k_pages.shape
+    if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype is not v_pages.dtype:
         raise ValueError("k_pages, v_pages: two tensors [pages, kv_heads, page_size, head_dim] of one shape and type")
-    n_pages, nkv, page, hd = k_pages.shape
+    n_pages, nkv, page, hd = shape
     ks, vs = k_pages.stride(), v_pages.stride()
     if hd > 1 and (ks[3] != 1 or vs[3] != 1):
         raise ValueError("k_pages, v_pages: head_dim has to be contiguous")
     n = kv_len.shape[0]
+    at = _ints("page_table", table, n, None)
     return (k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-            _ints("page_table", table, n, None), _ints("kv_len", kv_len, n), _ints("q_start", q_start, n + 1),
+            at, _ints("kv_len", kv_len, n), _ints("q_start", q_start, n + 1),
             _row_stride(table), n, table.shape[1], n_pages, page, nkv, hd, rows, max_rows, dtype)
 
 
-@functools.lru_cache(maxsize=256)
-def _attn_workspace(dev: int, dtype: int, hd: int, nkv: int, heads: int, max_rows: int) -> int:
+@functools.lru_cache(maxsize=1024)
+def _attn_workspace(dev: int, dtype: int, hd: int, nkv: int, heads: int, max_rows: int, max_pages: int, page: int) -> int:
     a = native.PagedAttention()
     a.chunk.dtype, a.chunk.head_dim, a.chunk.n_kv_heads, a.chunk.max_rows = dtype, hd, nkv, max_rows
+    a.chunk.max_pages, a.chunk.page_size = max_pages, page
     a.n_heads = heads
     with torch.cuda.device(dev):
         return native.lib().rai_gpu_paged_attention_workspace_bytes(C.byref(a))
 
 
-def attention_workspace_bytes(q: torch.Tensor, k_pages: torch.Tensor, max_rows: int) -> int:
+def attention_workspace_bytes(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor, max_rows: int) -> int:
     """Bytes of the workspace that `attention` takes for these arguments."""
     return _attn_workspace(q.get_device(), _dtype(k_pages, "k_pages"), k_pages.shape[3], k_pages.shape[1], q.shape[1],
-                           max_rows)
+                           min(max_rows, q.shape[0]), page_table.shape[1], k_pages.shape[2])
 
 
 def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -133,35 +156,42 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     log-sum-exp. A row that sees nothing gives 0 and -inf."""
     dtype = _dtype(k_pages, "k_pages")
     hd = k_pages.shape[-1]
-    _rows3("q", q, None, hd)
-    if q.dtype != k_pages.dtype:
+    qs = _rows3("q", q, None, hd)
+    if q.dtype is not k_pages.dtype:
         raise ValueError(f"q: {k_pages.dtype} as the pages, not {q.dtype}")
     rows, heads = q.shape[0], q.shape[1]
     if out is None:
-        out = torch.empty((rows, heads, hd), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((rows, heads, hd))
+        os = out.stride()
     else:
-        _rows3("out", out, heads, hd)
-        if out.shape[0] != rows or out.dtype != q.dtype:
+        os = _rows3("out", out, heads, hd)
+        if out.shape[0] != rows or out.dtype is not q.dtype:
             raise ValueError("out: shape and type of q")
     dev = _device(("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("kv_len", kv_len),
                   ("q_start", q_start), ("out", out))
     if rows == 0 or kv_len.shape[0] == 0 or max_rows == 0:
         return out
-    chunk = _chunk(k_pages, v_pages, page_table, kv_len, q_start, rows, min(max_rows, rows), dtype)
+    if max_rows > rows:
+        max_rows = rows
+    chunk = _chunk(k_pages, v_pages, page_table, kv_len, q_start, rows, max_rows, dtype)
     lse_at = 0
     if lse is not None:
         if lse.dtype != torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous() or lse.get_device() != dev:
             raise ValueError("lse: contiguous float32 [rows, heads] on q's device")
         lse_at = lse.data_ptr()
+    ws_at = ws_bytes = 0
     if workspace is None:
-        workspace = torch.empty(_attn_workspace(dev, dtype, hd, chunk[16], heads, min(max_rows, rows)), dtype=torch.uint8,
-                                device=q.device)
-    elif workspace.get_device() != dev or not workspace.is_contiguous():
-        raise ValueError("workspace: contiguous, on q's device")
-    args = _ATTN.pack(*chunk, q.data_ptr(), out.data_ptr(), lse_at, q.stride(0), q.stride(1), out.stride(0), out.stride(1),
-                      heads, window, hd ** -0.5 if scale is None else scale, softcap, workspace.data_ptr(),
-                      workspace.numel() * workspace.element_size())
-    _launch(dev, native.lib().rai_gpu_paged_attention, args)
+        need = _attn_workspace(dev, dtype, hd, chunk[16], heads, max_rows, chunk[13], chunk[15])
+        if need:
+            workspace = q.new_empty((need,), dtype=torch.uint8)
+            ws_at, ws_bytes = workspace.data_ptr(), need
+    else:
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            raise ValueError("workspace: contiguous, on q's device")
+        ws_at, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    args = _ATTN.pack(*chunk, q.data_ptr(), out.data_ptr(), lse_at, qs[0], qs[1], os[0], os[1], heads, window,
+                      hd ** -0.5 if scale is None else scale, softcap, ws_at, ws_bytes)
+    _launch(dev, lib().rai_gpu_paged_attention, args)
     return out
 
 
@@ -175,30 +205,28 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torc
     device) has one frequency per pair; 2 * len(inv_freq) elements of a head
     turn. q_out may be q itself. Rows as in `attention`, kv_len counting them."""
     dtype, hd, nkv = _dtype(k_pages, "k_pages"), k_pages.shape[-1], k_pages.shape[1]
-    _rows3("q", q, None, hd)
-    _rows3("k", k, nkv, hd)
-    _rows3("v", v, nkv, hd)
+    qs, ks, vs = _rows3("q", q, None, hd), _rows3("k", k, nkv, hd), _rows3("v", v, nkv, hd)
     rows, heads = q.shape[0], q.shape[1]
     in_dtype = _dtype(q, "q")
-    if k.dtype != q.dtype or v.dtype != q.dtype or k.shape[0] != rows or v.shape[0] != rows:
+    if k.dtype is not q.dtype or v.dtype is not q.dtype or k.shape[0] != rows or v.shape[0] != rows:
         raise ValueError("q, k, v: one type and one number of rows")
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+    if inv_freq.dtype is not torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq: a contiguous float32 vector")
     if q_out is None:
-        q_out = torch.empty((rows, heads, hd), dtype=k_pages.dtype, device=q.device)
+        q_out = q.new_empty((rows, heads, hd), dtype=k_pages.dtype)
+        os = q_out.stride()
     else:
-        _rows3("q_out", q_out, heads, hd)
-        if q_out.shape[0] != rows or q_out.dtype != k_pages.dtype:
+        os = _rows3("q_out", q_out, heads, hd)
+        if q_out.shape[0] != rows or q_out.dtype is not k_pages.dtype:
             raise ValueError("q_out: q's shape in the pages' type")
     dev = _device(("q", q), ("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table),
                   ("kv_len", kv_len), ("q_start", q_start), ("inv_freq", inv_freq), ("q_out", q_out))
     if rows == 0 or kv_len.shape[0] == 0:
         return q_out
     args = _ROPE.pack(*_chunk(k_pages, v_pages, page_table, kv_len, q_start, rows, rows, dtype), q.data_ptr(), k.data_ptr(),
-                      v.data_ptr(), q_out.data_ptr(), inv_freq.data_ptr(), q.stride(0), q.stride(1), k.stride(0),
-                      k.stride(1), v.stride(0), v.stride(1), q_out.stride(0), q_out.stride(1), heads,
-                      2 * inv_freq.shape[0], 1 if interleaved else 0, in_dtype, mscale)
-    _launch(dev, native.lib().rai_gpu_rope_append, args)
+                      v.data_ptr(), q_out.data_ptr(), inv_freq.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0],
+                      os[1], heads, 2 * inv_freq.shape[0], 1 if interleaved else 0, in_dtype, mscale)
+    _launch(dev, lib().rai_gpu_rope_append, args)
     return q_out
 
 
@@ -230,23 +258,26 @@ def _pool(k: torch.Tensor, v: torch.Tensor):
         k = k.unsqueeze(0)
     if v.dim() == 4:
         v = v.unsqueeze(0)
+    shape = k.shape
     _dtype(k, "k")
-    if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype:
+    if len(shape) != 5 or shape != v.shape or k.dtype is not v.dtype:
         raise ValueError("k, v: two tensors [layers, pages, kv_heads, page_size, head_dim] of one shape and type")
     e = k.element_size()
+    layers, pages, heads, slots, dim = shape
+    n = heads * slots * dim
+    strides = []
     for name, t in (("k", k), ("v", v)):
-        # A page's block may order its heads and slots either way.
-        dims = sorted((s, n) for s, n in zip(t.stride()[2:], t.shape[2:]) if n > 1)
-        want = 1
-        for s, n in dims:
-            if s != want:
-                raise ValueError(f"{name}: every page has to be one contiguous block")
-            want *= n
-    n = k.shape[2] * k.shape[3] * k.shape[4] * e
-    one = k.shape[1] == 1  # the stride of a single page or layer means nothing
-    return _POOL.pack(k.data_ptr(), v.data_ptr(), k.stride(0) * e if k.shape[0] > 1 else 0, n if one else k.stride(1) * e,
-                      v.stride(0) * e if v.shape[0] > 1 else 0, n if one else v.stride(1) * e, n, k.shape[0],
-                      k.shape[1]), k.shape[3]
+        st = t.stride()
+        if st[2:] != (slots * dim, dim, 1):
+            # A page's block may order its heads and slots either way.
+            want = 1
+            for s, m in sorted((s, m) for s, m in zip(st[2:], shape[2:]) if m > 1):
+                if s != want:
+                    raise ValueError(f"{name}: every page has to be one contiguous block")
+                want *= m
+        # The stride of a single page or layer means nothing.
+        strides += [st[0] * e if layers > 1 else 0, st[1] * e if pages > 1 else n * e]
+    return _POOL.pack(k.data_ptr(), v.data_ptr(), *strides, n * e, layers, pages), slots
 
 
 def fork(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor, page_size: int, *,
@@ -259,14 +290,14 @@ def fork(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, paren
     if n == 0 or page_table.shape[0] == 0:
         raise ValueError("fork: no sequences")
     if out_table is None:
-        out_table = torch.empty((n, page_table.shape[1]), dtype=torch.int32, device=page_table.device)
+        out_table = page_table.new_empty((n, page_table.shape[1]))
     if out_lens is None:
-        out_lens = torch.empty((n,), dtype=torch.int32, device=page_table.device)
+        out_lens = lens.new_empty((n,))
     dev = _device(("page_table", page_table), ("lens", lens), ("refs", refs), ("parents", parents), ("out_table", out_table),
                   ("out_lens", out_lens))
     if out_table.dim() != 2 or out_table.shape[0] != n:
         raise ValueError("out_table: one row per parent")
-    _launch(dev, native.lib().rai_gpu_kv_fork, _table(page_table, lens, refs, page_size),
+    _launch(dev, lib().rai_gpu_kv_fork, _table(page_table, lens, refs, page_size),
             _table(out_table, out_lens, refs, page_size), _ints("parents", parents, n))
     return out_table, out_lens
 
@@ -283,12 +314,12 @@ def resize(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, k: 
     dev = _device(("page_table", page_table), ("lens", lens), ("refs", refs), ("k", k), ("v", v),
                   *((("new_lens", new_lens),) if new_lens is not None else ()))
     n = page_table.shape[0]
-    status = torch.empty((1,), dtype=torch.int32, device=lens.device)
+    status = lens.new_empty((1,))
     if workspace is None:
-        workspace = torch.empty(native.lib().rai_gpu_kv_resize_workspace_bytes(n), dtype=torch.uint8, device=lens.device)
+        workspace = lens.new_empty((lib().rai_gpu_kv_resize_workspace_bytes(n),), dtype=torch.uint8)
     elif workspace.get_device() != dev or not workspace.is_contiguous():
         raise ValueError("workspace: contiguous, on the tables' device")
-    _launch(dev, native.lib().rai_gpu_kv_resize, _table(page_table, lens, refs, page), pool,
+    _launch(dev, lib().rai_gpu_kv_resize, _table(page_table, lens, refs, page), pool,
             _ints("new_lens", new_lens, n) if new_lens is not None else None, delta, status.data_ptr(),
             workspace.data_ptr(), workspace.numel() * workspace.element_size())
     return status
@@ -302,13 +333,12 @@ def compact(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, k:
     [1] on the device."""
     pool, page = _pool(k, v)
     dev = _device(("page_table", page_table), ("lens", lens), ("refs", refs), ("k", k), ("v", v))
-    used = torch.empty((1,), dtype=torch.int32, device=refs.device)
+    used = refs.new_empty((1,))
     if workspace is None:
-        workspace = torch.empty(native.lib().rai_gpu_kv_compact_workspace_bytes(refs.shape[0]), dtype=torch.uint8,
-                                device=refs.device)
+        workspace = refs.new_empty((lib().rai_gpu_kv_compact_workspace_bytes(refs.shape[0]),), dtype=torch.uint8)
     elif workspace.get_device() != dev or not workspace.is_contiguous():
         raise ValueError("workspace: contiguous, on the tables' device")
-    _launch(dev, native.lib().rai_gpu_kv_compact, _table(page_table, lens, refs, page), pool, used.data_ptr(),
+    _launch(dev, lib().rai_gpu_kv_compact, _table(page_table, lens, refs, page), pool, used.data_ptr(),
             workspace.data_ptr(), workspace.numel() * workspace.element_size())
     return used
 
@@ -319,7 +349,7 @@ def copy_pages(k: torch.Tensor, v: torch.Tensor, src: torch.Tensor, dst: torch.T
     pool, _ = _pool(k, v)
     dev = _device(("k", k), ("v", v), ("src", src), ("dst", dst))
     n = src.shape[0]
-    _launch(dev, native.lib().rai_gpu_kv_copy_pages, pool, _ints("src", src, n), _ints("dst", dst, n), n)
+    _launch(dev, lib().rai_gpu_kv_copy_pages, pool, _ints("src", src, n), _ints("dst", dst, n), n)
 
 
 def status(device=None) -> None:

@@ -193,7 +193,7 @@ def test_other_stream_graph_and_shared_workspace():
     cs = [ref.Cache(lens, 2, 128, 16, torch.bfloat16, dev, seed=s) for s in (1, 2)]
     qs = [make_q(4, 8, 128, torch.bfloat16, dev, seed=s) for s in (3, 4)]
     starts = ref.starts_of(rows, dev)
-    ws = torch.empty(paged.attention_workspace_bytes(qs[0], cs[0].k, 3), dtype=torch.uint8, device=dev)
+    ws = torch.empty(paged.attention_workspace_bytes(qs[0], cs[0].k, cs[0].table, 3), dtype=torch.uint8, device=dev)
     want = [paged.attention(q, c.k, c.v, c.table, c.kv_len, starts, 3) for q, c in zip(qs, cs)]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
