@@ -43,6 +43,48 @@ bool paged_attention_tc_takes(const AttnArgs& a);
 size_t paged_attention_tc_workspace(const AttnArgs& a);
 cudaError_t paged_attention_tc(const AttnArgs& a, cudaStream_t s);
 
+namespace paged_attn {
+
+bool make_maps(const PagedChunk& c, int dtype, int box, KvMaps* maps) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess) {
+      (void)cudaGetLastError();
+      f = nullptr;
+    }
+    return reinterpret_cast<Encode>(f);
+  }();
+  if (!encode) return false;
+  const int elt = dtype == kF32 ? 4 : 2;
+  const CUtensorMapDataType type = dtype == kF32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const cuuint64_t dims[4] = {(cuuint64_t)c.hd, c.page.d, (cuuint64_t)c.nkv, (cuuint64_t)c.n_pages};
+  const cuuint32_t boxes[4] = {128u / elt, (cuuint32_t)box, 1, 1}, ones[4] = {1, 1, 1, 1};
+  for (int kv = 0; kv < 2; ++kv) {
+    long long st[3] = {kv ? c.v_slot : c.k_slot, kv ? c.v_head : c.k_head, kv ? c.v_page : c.k_page};
+    cuuint64_t strides[3];
+    for (int i = 0; i < 3; ++i) {
+      // The stride of a dimension of one means nothing, but has to be valid.
+      if (dims[i + 1] == 1) st[i] = 16 / elt;
+      strides[i] = (cuuint64_t)st[i] * elt;
+      if (st[i] <= 0 || strides[i] >= (1ull << 40)) return false;
+    }
+    if (encode(kv ? &maps->v : &maps->k, type, 4, kv ? c.v : c.k, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+  }
+  return true;
+}
+
+}  // namespace paged_attn
+
 namespace {
 
 using namespace paged_attn;
@@ -189,19 +231,19 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
   }
 
   Cursor<MT, NT> ld, cur;
-  ld.seek(p, rg, begin);
+  ld.seek(p, rg);
   cur = ld;
   if (threadIdx.x == 0 && !p.whole) leave_cut<MT, NT>(p, rg, cur, blockIdx.x);
-  long long loaded = begin;
+  uint32_t loaded = 0, done = 0;  // tiles
   TilePages<NT> pages;
   pages.fetch(ch, ld.it, (ld.it.first + ld.tile) * NT, lane);
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) {
-    if (loaded < end) {
+    if (ld.pos < end) {
       load_tile<C>(p, ld, pages, base + s * 2 * C::kTileB, base + s * 2 * C::kTileB + C::kTileB);
       ++loaded;
       ld.next(p);
-      if (loaded < end) pages.fetch(ch, ld.it, (ld.it.first + ld.tile) * NT, lane);
+      if (ld.pos < end) pages.fetch(ch, ld.it, (ld.it.first + ld.tile) * NT, lane);
     }
     cp_async_commit();
   }
@@ -212,7 +254,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
   int pos[2];  // position of the thread's two rows, below 0: none
   bool poison = false, fresh = true;
   int first_slot = 0;  // of the workspace: 0 for the CTA's first item, 1 for its last
-  for (long long at = begin; at < end; ++at) {
+  for (; cur.pos < end; ++done) {
     const Item& it = cur.it;
     if (fresh) {
       // The item's rows: query fragments, positions, empty sums.
@@ -263,15 +305,15 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
     cp_async_wait<S - 2>();
     __syncthreads();
     // The stage that the last step read is free: fetch ahead.
-    if (loaded < end) {
-      const uint32_t st = base + (uint32_t)((loaded - begin) % S) * 2 * C::kTileB;
+    if (ld.pos < end) {
+      const uint32_t st = base + (loaded % S) * 2 * C::kTileB;
       load_tile<C>(p, ld, pages, st, st + C::kTileB);
       ++loaded;
       ld.next(p);
-      if (loaded < end) pages.fetch(ch, ld.it, (ld.it.first + ld.tile) * NT, lane);
+      if (ld.pos < end) pages.fetch(ch, ld.it, (ld.it.first + ld.tile) * NT, lane);
     }
     cp_async_commit();
-    const uint32_t sk = base + (uint32_t)((at - begin) % S) * 2 * C::kTileB, sv = sk + C::kTileB;
+    const uint32_t sk = base + (done % S) * 2 * C::kTileB, sv = sk + C::kTileB;
     const int t0 = (it.first + cur.tile) * NT;
     const int p0 = it.len - it.n;
     const int plo = p0 + (int)p.group_div.quot(it.f0), phi = it.hi - 1;
@@ -410,7 +452,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
     }
 
     // ---- end of the item, or of this CTA's part of it ----
-    if (cur.tile + 1 == it.tiles || at + 1 == end) {
+    if (cur.ends(end)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         l[h] += __shfl_xor_sync(~0u, l[h], 1);
@@ -470,7 +512,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
         }
       }
       if (wn == 0) {
-        const long long item_at = at - cur.tile;  // where the item begins on the line
+        const long long item_at = cur.pos - cur.tile;  // of its first tile
         if (poison) {
           // Rows that see a V value which is not finite get it after all.
           const int ta = it.first * NT + (int)max(0ll, begin - item_at) * NT, tb = (it.first + cur.tile + 1) * NT;
@@ -494,7 +536,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
             }
           }
         }
-        const bool whole = item_at >= begin && cur.tile + 1 == it.tiles;
+        const bool whole = item_at >= begin && cur.last_of_item();
         if (whole) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -563,6 +605,7 @@ auto with_cfg(int dtype, int hd, int rows, F f) {
 // Least tiles of a CTA's range: a cut costs a partial result (a few KB) and
 // its share of the joining kernel.
 constexpr int kMinTiles = 4;
+constexpr int kItemCost = 1;  // tiles
 // Caches of at most this many tiles a sequence are not cut.
 constexpr int kWholeTiles = 8;
 template <typename C>
@@ -590,6 +633,7 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
   p.group_div = FastDiv(a.group);
   p.whole = whole_items<C>(a);
   p.min_tiles = p.whole ? 1 : kMinTiles;
+  p.item_cost = kItemCost;
   p.grid = device_sm_count() * resident_ctas<C>();
   p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
   e = launch_pdl(paged_attn_kernel<C>, dim3(p.grid), dim3(kThreads), C::kSmem, s, p);

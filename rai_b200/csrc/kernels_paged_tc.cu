@@ -19,12 +19,13 @@
 // grow up to 2^8, which f32 sums and the 16-bit types hold.
 //
 // Warps: 0-3 and 4-7 softmax of halves A and B, 8 TMEM and MMA issue (one
-// thread), 9-10 producers: K, V and Q by 16-byte asynchronous copies (pages of
-// any size and any strides; slots that no row sees are zero filled), written
-// in the 128-byte swizzle the MMA reads: K and V tiles as 64-column blocks of
-// [token][128 bytes], K-major for Q K^T and N-major for P V. Every wait is
-// bounded; on a timeout all roles stop, what is in flight is waited for and
-// the TMEM columns are released.
+// thread), 9 K and V by TMA, a piece of a page per lane, 10-11 the queries and
+// the hand-over of V tiles (in masked tiles they are looked through first).
+// Pages that TMA cannot fetch (sizes that are not 8 x 2^i or whole tiles) come
+// by 16-byte copies of warps 10-11. Tiles lie in the 128-byte swizzle the MMA
+// reads, K-major for Q K^T and N-major for P V. Every wait is bounded; on a
+// timeout all roles stop, what is in flight is waited for and the TMEM columns
+// are released.
 #include <cuda_runtime.h>
 
 #include <mutex>
@@ -59,6 +60,7 @@ struct Tc {
 };
 
 constexpr float kLazy = 8.f;  // log2 units
+constexpr int kItemCost = 3;  // tiles
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -129,12 +131,6 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, uint32_
   return false;
 }
 
-// Bytes of 16-byte chunk `chunk` (0 .. HD / 8 - 1) of row `row` in a tile of
-// `rows` rows: 64-column blocks, 128-byte swizzle.
-__device__ __forceinline__ uint32_t tile_at(int rows, int row, int chunk) {
-  return (uint32_t)((chunk >> 3) * rows * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
-}
-
 // Whether some row of the item may not see some token of the tile that
 // begins at t0.
 __device__ __forceinline__ bool tile_masked(const Item& it, int t0, int nt, int window, const FastDiv& group) {
@@ -142,12 +138,63 @@ __device__ __forceinline__ bool tile_masked(const Item& it, int t0, int nt, int 
   return t0 + nt - 1 > plo || t0 < it.lo || (window > 0 && t0 <= phi - window);
 }
 
-template <typename C, bool CAP>
-__global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ Params p) {
+// Replaces the values of this thread's chunks of a V tile that are not finite
+// by zero; whether there were any.
+template <typename C>
+__device__ __forceinline__ bool look_through(uint32_t base, int tid) {
+  constexpr int kChunks = C::HD / 8, kRowsPer = kProducers / kChunks;
+  const int chunk = tid % kChunks, r0 = tid / kChunks;
+  bool bad = false;
+#pragma unroll 4
+  for (int i = 0; i < C::NT / kRowsPer; ++i) {
+    const uint32_t ad = base + tile_at(C::NT, r0 + i * kRowsPer, chunk);
+    uint4 w;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(ad));
+    const uint4 f = make_uint4(finite_or_zero<C::DT>(w.x), finite_or_zero<C::DT>(w.y), finite_or_zero<C::DT>(w.z),
+                               finite_or_zero<C::DT>(w.w));
+    if (f.x != w.x || f.y != w.y || f.z != w.z || f.w != w.w) {
+      bad = true;
+      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(ad), "r"(f.x), "r"(f.y), "r"(f.z), "r"(f.w) : "memory");
+    }
+  }
+  return bad;
+}
+
+// The item's query rows, by kProducers threads; waits until they are there.
+template <typename C>
+__device__ __forceinline__ void load_queries(const Params& p, const Item& it, int kv_head, uint32_t sq, int tid) {
+  constexpr int kChunks = C::HD / 8, kRowsPer = kProducers / kChunks;
+  const int chunk = tid % kChunks, r0 = tid / kChunks;
+  const bool in_head = chunk * 8 < p.a.c.hd;
+  const uint16_t* q = static_cast<const uint16_t*>(p.a.q) + (long long)it.start * p.a.q_row + (long long)kv_head * p.a.group * p.a.q_head + chunk * 8;
+#pragma unroll 1
+  for (int i0 = 0; i0 < C::MT / kRowsPer; i0 += 8) {
+    const uint16_t* src[8];
+    bool real[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + (i0 + i) * kRowsPer, f = it.f0 + r, qi = (int)p.group_div.quot(f), j = f - qi * p.a.group;
+      real[i] = r < it.nf && in_head;
+      src[i] = real[i] ? q + qi * p.a.q_row + j * p.a.q_head : q;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) cp_async16_or_zero(sq + tile_at(C::MT, r0 + (i0 + i) * kRowsPer, chunk), src[i], real[i]);
+  }
+  cp_async_commit();
+  cp_async_wait<0>();
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+constexpr int kLanded = 8;  // V tiles between their landing and their hand-over
+
+template <typename C, bool CAP, bool TMA>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    paged_attn_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ KvMaps maps, int box) {
   constexpr int DT = C::DT, HD = C::HD, MT = C::MT, NT = C::NT;
   extern __shared__ uint8_t smem_raw[];
   __shared__ long long sh[kPlanWords];
   __shared__ uint64_t kv_full[C::kSlots], kv_empty[C::kSlots], q_full, q_empty, s_full[2], p_full[2], o_done[2], drained;
+  __shared__ uint64_t landed[kLanded];
   __shared__ uint32_t tmem_slot;
   __shared__ int poison[4];  // ordinal + 1 of an item with masked V values that are not finite
   const uint32_t sq = (smem_u32(smem_raw) + 1023) & ~1023u, skv = sq + C::kQB;
@@ -157,7 +204,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kSlots; ++i) {
-      mbar_init(&kv_full[i], kProducers);
+      mbar_init(&kv_full[i], TMA ? 1 : kProducers);
       mbar_init(&kv_empty[i], 1);
     }
     mbar_init(&q_full, kProducers);
@@ -168,6 +215,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       mbar_init(&o_done[i], 1);
     }
     mbar_init(&drained, 1);
+    for (int i = 0; i < kLanded; ++i) mbar_init(&landed[i], 1);
     for (int i = 0; i < 4; ++i) poison[i] = 0;
     fence_barrier_init();
   }
@@ -190,67 +238,102 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   if (begin >= end && threadIdx.x == 0) reinterpret_cast<Cut*>(p.a.part)[blockIdx.x] = Cut{};
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (begin < end && (warp == 9 || warp == 10)) {
-      // ---------------- producers ----------------
-      const int tid = threadIdx.x - 9 * 32;
+    if (begin < end && TMA && warp == 9) {
+      // ---------------- K and V by TMA ----------------
+      Cursor<MT, NT> cur;
+      cur.seek(p, rg);
+      TilePieces<NT, HD / 64, 2> pieces;
+      pieces.fetch(ch, cur.it, (cur.it.first + cur.tile) * NT, box, lane);
+      uint32_t issued = 0;
+      bool ok = true;
+      for (uint32_t k = 0; cur.pos < end && ok; ++k) {
+        const Item& it = cur.it;
+        const int t0 = (it.first + cur.tile) * NT;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint32_t n = 2 * k + kv, slot = n % C::kSlots, use = n / C::kSlots;
+          if (ok && use > 0) ok = __all_sync(~0u, wait_bar(&kv_empty[slot], (use - 1) & 1, err));
+          if (ok) {
+            pieces.load(ch, it, t0, box, lane, kv ? &maps.v : &maps.k, cur.head, skv + slot * C::kTileB,
+                        kv ? &landed[k % kLanded] : &kv_full[slot]);
+            ++issued;
+          }
+        }
+        cur.next(p);
+        if (cur.pos < end) pieces.fetch(ch, cur.it, (cur.it.first + cur.tile) * NT, box, lane);
+      }
+      // What was requested lands before the CTA ends.
+      for (uint32_t n = issued > C::kSlots ? issued - C::kSlots : 0; n < issued; ++n) {
+        if (n & 1) wait_bar(&landed[n / 2 % kLanded], n / 2 / kLanded & 1, nullptr);
+        else wait_bar(&kv_full[n % C::kSlots], n / C::kSlots & 1, nullptr);
+      }
+    } else if (begin < end && TMA && warp >= 10) {
+      // ---------------- queries; V tiles handed over ----------------
+      const int tid = threadIdx.x - 10 * 32;
+      Cursor<MT, NT> cur;
+      cur.seek(p, rg);
+      if (tid == 0) leave_cut<MT, NT>(p, rg, cur, blockIdx.x);
+      int items = 0;
+      bool fresh = true;
+      for (uint32_t k = 0; cur.pos < end; ++k) {
+        const Item& it = cur.it;
+        if (fresh) {
+          if (k > 0 && !__all_sync(~0u, wait_bar(&q_empty, (items - 1) & 1, err))) break;
+          load_queries<C>(p, it, cur.head, sq, tid);
+          mbar_arrive(&q_full);
+          fresh = false;
+        }
+        if (!__all_sync(~0u, wait_bar(&landed[k % kLanded], k / kLanded & 1, err))) break;
+        const uint32_t slot = (2 * k + 1) % C::kSlots;
+        if (tile_masked(it, (it.first + cur.tile) * NT, NT, p.a.window, p.group_div)) {
+          if (look_through<C>(skv + slot * C::kTileB, tid)) *(volatile int*)&poison[items & 3] = items + 1;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          asm volatile("bar.sync 1, 64;" ::: "memory");
+        }
+        if (tid == 0) mbar_arrive(&kv_full[slot]);
+        if (cur.last_of_item()) {
+          fresh = true;
+          ++items;
+        }
+        cur.next(p);
+      }
+    } else if (begin < end && !TMA && warp >= 10) {
+      // ---------------- K, V and queries by 16-byte copies ----------------
+      const int tid = threadIdx.x - 10 * 32;
       constexpr int kChunks = HD / 8, kRowsPer = kProducers / kChunks;  // rows of 16-byte chunks at a time
-      constexpr int kLag = 2;  // slots in flight before the oldest is handed over
+      constexpr int kLag = 2;  // tiles in flight before the oldest is handed over
       const int chunk = tid % kChunks, r0 = tid / kChunks;
       const bool in_head = chunk * 8 < ch.hd;
       Cursor<MT, NT> cur;
-      cur.seek(p, rg, begin);
+      cur.seek(p, rg);
       if (tid == 0) leave_cut<MT, NT>(p, rg, cur, blockIdx.x);
       TilePages<NT> pages;
       pages.fetch(ch, cur.it, (cur.it.first + cur.tile) * NT, lane);
       int items = 0;
       uint32_t n = 0, handed = 0;  // K and V tiles fetched, handed over
       bool ok = true, fresh = true;
-      // Which of the slots in flight holds a V tile to look through.
-      uint32_t look = 0;  // bit i: fetch n - 1 - i
+      uint32_t look = 0;  // bit i: fetch n - 1 - i is a V tile to look through
       auto hand = [&](int age) {  // the fetch `handed` has landed
         const uint32_t slot = handed % C::kSlots;
-        if (look >> age & 1u) {
-          const uint32_t base = skv + slot * C::kTileB;
-          bool bad = false;
-          for (int i = 0; i < NT / kRowsPer; ++i) {
-            const uint32_t ad = base + tile_at(NT, r0 + i * kRowsPer, chunk);
-            uint4 w;
-            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(ad));
-            const uint4 f = make_uint4(finite_or_zero<DT>(w.x), finite_or_zero<DT>(w.y), finite_or_zero<DT>(w.z),
-                                       finite_or_zero<DT>(w.w));
-            if (f.x != w.x || f.y != w.y || f.z != w.z || f.w != w.w) {
-              bad = true;
-              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(ad), "r"(f.x), "r"(f.y), "r"(f.z), "r"(f.w)
-                           : "memory");
-            }
-          }
-          if (bad) *(volatile int*)&poison[items & 3] = items + 1;
-        }
+        if ((look >> age & 1u) && look_through<C>(skv + slot * C::kTileB, tid)) *(volatile int*)&poison[items & 3] = items + 1;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mbar_arrive(&kv_full[slot]);
         ++handed;
       };
-      for (long long at = begin; at < end && ok; ++at) {
+      bool first = true;
+      while (cur.pos < end && ok) {
         if (fresh) {
           // A new item: what is in flight is handed over under the old one's
           // ordinal, then the query rows are fetched.
           cp_async_wait<0>();
           while (handed < n) hand((int)(n - 1 - handed));
-          if (at > begin) {
+          if (!first) {
             ++items;
             ok = wait_bar(&q_empty, (items - 1) & 1, err);
             if (!ok) break;
           }
-          const Item& it = cur.it;
-          for (int i = 0; i < MT / kRowsPer; ++i) {
-            const int r = r0 + i * kRowsPer, f = it.f0 + r, qi = (int)p.group_div.quot(f), j = f - qi * p.a.group;
-            const bool real = r < it.nf && in_head;
-            const long long o = (long long)(it.start + qi) * p.a.q_row + (long long)(cur.head * p.a.group + j) * p.a.q_head + chunk * 8;
-            cp_async16_or_zero(sq + tile_at(MT, r, chunk), real ? static_cast<const uint16_t*>(p.a.q) + o : p.a.q, real);
-          }
-          cp_async_commit();
-          cp_async_wait<0>();
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          first = false;
+          load_queries<C>(p, cur.it, cur.head, sq, tid);
           mbar_arrive(&q_full);
           fresh = false;
         }
@@ -290,9 +373,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             hand(kLag);
           }
         }
-        if (cur.tile + 1 == it.tiles) fresh = true;
+        if (cur.last_of_item()) fresh = true;
         cur.next(p);
-        if (at + 1 < end) pages.fetch(ch, cur.it, (cur.it.first + cur.tile) * NT, lane);
+        if (cur.pos < end) pages.fetch(ch, cur.it, (cur.it.first + cur.tile) * NT, lane);
       }
       cp_async_wait<0>();
       if (ok)
@@ -301,7 +384,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       // ---------------- MMA issue ----------------
       if (lane == 0) {
         Cursor<MT, NT> cur;
-        cur.seek(p, rg, begin);
+        cur.seek(p, rg);
         bool ok = true;
         int items = 0;
         auto qk = [&](int half, uint32_t k) {  // S of half for the CTA's k-th tile
@@ -324,19 +407,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         auto wait_kv = [&](uint32_t i) { return wait_bar(&kv_full[i % C::kSlots], i / C::kSlots & 1, err); };
         // Queries, K and V of a tile are waited for once each, before the first
         // MMA that reads them.
-        const uint32_t tiles = (uint32_t)(end - begin);
         bool first = true;  // tile k is its item's first here
-        ok = wait_bar(&q_full, 0, err) && wait_kv(0);
+        ok = cur.pos < end && wait_bar(&q_full, 0, err) && wait_kv(0);
         if (ok) {
           fence_after();
           qk(0, 0);
           qk(1, 0);
           commit(&kv_empty[0]);
-          if (cur.tile + 1 == cur.it.tiles || tiles == 1) commit(&q_empty);
+          if (cur.ends(end)) commit(&q_empty);
         }
-        for (uint32_t k = 0; k < tiles && ok; ++k) {
-          const bool last = cur.tile + 1 == cur.it.tiles, more = k + 1 < tiles;
+        for (uint32_t k = 0; cur.pos < end && ok; ++k) {
+          const bool last = cur.last_of_item();
           cur.next(p);
+          const bool more = cur.pos < end;
           ok = wait_kv(2 * k + 1) && wait_bar(&p_full[0], k & 1, err);
           if (!ok) break;
           fence_after();
@@ -359,8 +442,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
           if (more) {
             qk(1, k + 1);
             commit(&kv_empty[(2 * k + 2) % C::kSlots]);
-            // Tile k + 1 is its item's last here: the queries may go.
-            if (cur.tile + 1 == cur.it.tiles || k + 2 == tiles) commit(&q_empty);
+            if (cur.ends(end)) commit(&q_empty);  // tile k + 1 is its item's last here: the queries may go
           }
           first = last;
         }
@@ -376,12 +458,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
       const uint32_t ts = tmem + half * 128 + lanes, to = tmem + 256 + half * HD + lanes;
       Cursor<MT, NT> cur;
-      cur.seek(p, rg, begin);
+      cur.seek(p, rg);
       int items = 0;
       bool ok = true;
       float m = -INFINITY, l = 0.f;  // m: of the raw scores
       uint32_t k = 0, k_first = 0;
-      for (long long at = begin; at < end; ++at, ++k) {
+      for (; cur.pos < end; ++k) {
         const Item& it = cur.it;
         const int f = it.f0 + half * 128 + row, qi = (int)p.group_div.quot(f);
         const bool real = half * 128 + row < it.nf;
@@ -404,9 +486,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
           for (int x = 0; x < 128; ++x)
             if (x > till || x < from) v[x] = 0xff800000u;
         }
-        float top = -INFINITY;
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int x = 0; x < 128; x += 2) top = fmaxf(top, fmaxf(__uint_as_float(v[x]), __uint_as_float(v[x + 1])));
+        for (int x = 0; x < 128; x += 2)
+          tops[x / 2 & 3] = fmaxf(tops[x / 2 & 3], fmaxf(__uint_as_float(v[x]), __uint_as_float(v[x + 1])));
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const bool move = top > m && (m == -INFINITY || (top - m) * p.c > kLazy);
         if (__any_sync(~0u, move)) {
           const float next = move ? top : m;
@@ -446,13 +530,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[half]);
 
-        if (cur.tile + 1 == it.tiles || at + 1 == end) {
+        if (cur.ends(end)) {
           // ---- end of the item, or of this CTA's part of it ----
           ok = __all_sync(~0u, wait_bar(&o_done[half], k & 1, err));
           if (!ok) break;
           fence_after();
-          const long long item_at = at - cur.tile;
-          const bool whole = item_at >= begin && cur.tile + 1 == it.tiles;
+          const long long item_at = cur.pos - cur.tile;  // of its first tile
+          const bool whole = item_at >= begin && cur.last_of_item();
           const bool poisoned = *(volatile int*)&poison[items & 3] == items + 1;
           const int r = half * 128 + row, j = f - qi * p.a.group, head = cur.head * p.a.group + j;
           const float inv = !whole ? 1.f : l > 0.f || l != l ? 1.f / l : 0.f;
@@ -520,8 +604,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   }
 }
 
-template <typename C, bool CAP>
-cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
+template <typename C, bool CAP, bool TMA>
+cudaError_t launch(const AttnArgs& a, const KvMaps& maps, int box, cudaStream_t s) {
   static std::once_flag once[64];
   static cudaError_t ready[64];
   int dev = 0;
@@ -529,7 +613,7 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   std::call_once(once[dev], [&] {
-    ready[dev] = cudaFuncSetAttribute(paged_attn_tc_kernel<C, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    ready[dev] = cudaFuncSetAttribute(paged_attn_tc_kernel<C, CAP, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   });
   if (ready[dev] != cudaSuccess) return ready[dev];
   Params p;
@@ -540,9 +624,13 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
   p.group_div = FastDiv(a.group);
   p.grid = device_sm_count();
   p.whole = false;
-  p.min_tiles = 4;
+  p.min_tiles = 8;
+  p.item_cost = kItemCost;
   p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
-  e = launch_pdl(paged_attn_tc_kernel<C, CAP>, dim3(p.grid), dim3(kTcThreads), C::kSmem, s, p);
+  // Not launched ahead of its predecessor's end: its CTAs would share the SMs
+  // with the last call's join and run unevenly.
+  paged_attn_tc_kernel<C, CAP, TMA><<<p.grid, kTcThreads, C::kSmem, s>>>(p, maps, box);
+  e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return launch_pdl(paged_combine_kernel<C>, dim3(p.grid - 1, combine_grid_y(C::MT)), dim3(kCombineThreads), 0, s, p);
 }
@@ -558,7 +646,13 @@ size_t paged_attention_tc_workspace(const AttnArgs& a) {
 }
 
 cudaError_t paged_attention_tc(const AttnArgs& a, cudaStream_t s) {
-#define RAI_TC(DT, HD) (a.softcap > 0.f ? launch<Tc<DT, HD>, true>(a, s) : launch<Tc<DT, HD>, false>(a, s))
+  KvMaps maps;
+  const int box = tma_box((int)a.c.page.d, 128);
+  const bool tma = box && make_maps(a.c, a.dtype, box, &maps);
+#define RAI_TC(DT, HD)                                                                                                   \
+  (a.softcap > 0.f ? (tma ? launch<Tc<DT, HD>, true, true>(a, maps, box, s) : launch<Tc<DT, HD>, true, false>(a, maps, box, s)) \
+                   : (tma ? launch<Tc<DT, HD>, false, true>(a, maps, box, s)                                             \
+                          : launch<Tc<DT, HD>, false, false>(a, maps, box, s)))
   if (a.dtype == kF16) return a.c.hd <= 64 ? RAI_TC(kF16, 64) : RAI_TC(kF16, 128);
   return a.c.hd <= 64 ? RAI_TC(kBF16, 64) : RAI_TC(kBF16, 128);
 #undef RAI_TC

@@ -1,6 +1,7 @@
 // What the two kernels of paged attention share: the line of token tiles and
-// its cuts, the join of cut items, and elements.
+// its cuts, the fetching of pages, the join of cut items, and elements.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include "paged.h"
@@ -12,9 +13,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kPlanWords = 22;
 
+// All (sequence, row tile, KV head) items lie one after the other on a line,
+// each item_cost + tiles long: tile i of an item that begins at s is at
+// s + item_cost + i. Cut in equal ranges, one per CTA, the line gives CTAs with
+// many short items fewer tiles (an item costs its queries' load, the filling
+// of the pipeline and its output beside its tiles).
 struct Params {
   AttnArgs a;
-  int row_tiles, min_tiles, grid;
+  int row_tiles, min_tiles, item_cost, grid;
   bool whole;  // items are short: none is cut
   float c;  // log2(e) * scale, or log2(e) when the scores are capped
   FastDiv row_tiles_div, group_div;
@@ -52,13 +58,16 @@ __device__ __forceinline__ Item item_of(const Params& p, int unit) {
   return it;
 }
 
-// The CTA's range [begin, end) of the line of tiles and the unit it starts
-// in. Every thread sums a run of units; a block scan places the runs. With
-// p.whole the cuts move down to the starts of the items they fall in.
+__device__ __forceinline__ int length_of(const Params& p, const Item& it) { return it.tiles ? it.tiles + p.item_cost : 0; }
+
+// The CTA's range [begin, end) of the line and the unit (sequence, row tile)
+// it starts in. Every thread sums a run of units; a block scan places the
+// runs. With p.whole the cuts move down to the starts of the items they fall
+// in.
 struct Range {
   long long total, per, begin, end;
   int unit;          // unit of `begin`
-  long long before;  // tiles of one KV head before it
+  long long before;  // length of one KV head's line before it
 };
 template <int MT, int NT, int THREADS>
 __device__ __forceinline__ Range plan(const Params& p, long long cta, long long (&sh)[kPlanWords]) {
@@ -66,7 +75,7 @@ __device__ __forceinline__ Range plan(const Params& p, long long cta, long long 
   const int per = (units + THREADS - 1) / THREADS;
   const int u0 = min(units, (int)threadIdx.x * per), u1 = min(units, u0 + per);
   long long own = 0;
-  for (int u = u0; u < u1; ++u) own += item_of<MT, NT>(p, u).tiles;
+  for (int u = u0; u < u1; ++u) own += length_of(p, item_of<MT, NT>(p, u));
   long long incl = own;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -95,7 +104,7 @@ __device__ __forceinline__ Range plan(const Params& p, long long cta, long long 
     } else if (own && at >= excl * nkv && at < incl * nkv) {
       int u = u0, t;
       for (;; ++u) {
-        t = item_of<MT, NT>(p, u).tiles;
+        t = length_of(p, item_of<MT, NT>(p, u));
         if (at < (excl + t) * nkv) break;
         excl += t;
       }
@@ -112,21 +121,28 @@ __device__ __forceinline__ Range plan(const Params& p, long long cta, long long 
   return r;
 }
 
-// Walks the line of tiles.
+// Walks the line's tiles; done when pos reaches the end of the range.
 template <int MT, int NT>
 struct Cursor {
   Item it;
   int unit, head, tile;
-  __device__ __forceinline__ void seek(const Params& p, const Range& r, long long at) {
+  long long pos;
+  // To the first tile at or behind the range's beginning.
+  __device__ __forceinline__ void seek(const Params& p, const Range& r) {
     unit = r.unit;
     it = item_of<MT, NT>(p, unit);
-    const long long in = at - r.before * p.a.c.nkv;
-    head = (int)(in / it.tiles);
-    tile = (int)(in - (long long)head * it.tiles);
+    const long long in = r.begin - r.before * p.a.c.nkv;
+    const int len = length_of(p, it);
+    head = (int)(in / len);
+    const int off = (int)(in - (long long)head * len);
+    tile = max(0, off - p.item_cost);
+    pos = r.begin + max(0, p.item_cost - off);
   }
   __device__ __forceinline__ void next(const Params& p) {
+    ++pos;
     if (++tile < it.tiles) return;
     tile = 0;
+    pos += p.item_cost;
     if (++head < p.a.c.nkv) return;
     head = 0;
     const int units = p.a.c.n_seqs * p.row_tiles;
@@ -135,6 +151,9 @@ struct Cursor {
       it = item_of<MT, NT>(p, unit);
     } while (it.tiles == 0);
   }
+  __device__ __forceinline__ bool last_of_item() const { return tile + 1 == it.tiles; }
+  // The CTA's last tile of the item.
+  __device__ __forceinline__ bool ends(long long end) const { return tile + 1 == it.tiles || pos + 1 >= end; }
 };
 
 // The pages of a tile's NT tokens, NT / 32 per lane. fetch() only issues the
@@ -169,6 +188,77 @@ struct TilePages {
       const int t = t0 + lane + 32 * i, slot = t - (int)c.page.quot(t) * (int)c.page.d;
       off[i] = page[i] >= 0 ? page[i] * page_stride + slot * slot_stride : -1;
     }
+  }
+};
+
+// Tiles of tokens in shared memory: 128-byte column blocks of [token][128
+// bytes] under the 128-byte swizzle (16-byte chunk c of a row at c ^ (row &
+// 7)), as TMA writes them and tcgen05 and (conflict free) ldmatrix read them.
+__device__ __forceinline__ uint32_t tile_at(int rows, int row, int chunk) {
+  return (uint32_t)((chunk >> 3) * rows * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+
+// Pages as TMA tensors (element, slot, head, page). A tile of NT tokens is
+// fetched in pieces of `box` slots of one page by one 128-byte column block,
+// one copy per lane of a warp: pages of 8 x 2^i slots, or of whole tiles.
+struct KvMaps {
+  CUtensorMap k, v;
+};
+// Slots of a piece, 0 where TMA cannot fetch such pages.
+inline int tma_box(int page, int nt) {
+  if (page % 8 == 0 && page <= nt && nt % page == 0) return page;
+  return page % nt == 0 ? nt : 0;
+}
+// Whether the maps could be made (kernels_paged_attn.cu).
+bool make_maps(const PagedChunk& c, int dtype, int box, KvMaps* maps);
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page,
+                                         uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+
+template <int NT, int BLOCKS, int ELT>
+struct TilePieces {
+  int page;  // of the lane's piece of the next tile
+  __device__ __forceinline__ bool mine(int box, int lane, int* block, int* piece) const {
+    const int pieces = NT / box;
+    *block = lane / pieces;
+    *piece = lane - *block * pieces;
+    return *block < BLOCKS;
+  }
+  // Only issues the load, a tile ahead of its use.
+  __device__ __forceinline__ void fetch(const PagedChunk& c, const Item& it, int t0, int box, int lane) {
+    int block, piece;
+    page = -1;
+    if (!mine(box, lane, &block, &piece)) return;
+    const int t = t0 + piece * box;
+    if (t < it.hi && t + box > it.lo) page = __ldg(c.table + (long long)it.seq * c.table_stride + c.page.quot(t));
+  }
+  // One tile of K or V into dst, completing on bar (one arrival). Pieces that
+  // no row sees are left out: their slots hold what they held. A page outside
+  // the pool is reported and its slots are zeros.
+  __device__ __forceinline__ void load(const PagedChunk& c, const Item& it, int t0, int box, int lane, const CUtensorMap* map,
+                                       int head, uint32_t dst, uint64_t* bar) const {
+    int block, piece;
+    const bool any = mine(box, lane, &block, &piece);
+    const int t = t0 + piece * box;
+    const bool want = any && t < it.hi && t + box > it.lo;
+    const bool good = want && (unsigned)page < (unsigned)c.n_pages;
+    const uint32_t at = dst + block * (NT * 128) + piece * box * 128;
+    if (want && !good) {
+      atomicOr(c.err, kErrBadInput);
+      for (int i = 0; i < box * 8; ++i)
+        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at + i * 16), "r"(0) : "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    const uint32_t n = __popc(__ballot_sync(~0u, good));
+    if (lane == 0) mbar_arrive_expect_tx(bar, n * box * 128);
+    __syncwarp();
+    if (good) tma_load(at, map, block * (128 / ELT), t - (int)c.page.quot(t) * (int)c.page.d, head, page, bar);
   }
 };
 
@@ -235,11 +325,11 @@ template <int MT, int NT>
 __device__ __forceinline__ void leave_cut(const Params& p, const Range& rg, const Cursor<MT, NT>& cur, int cta) {
   Cut c = {};
   if (rg.begin < rg.total && !p.whole && cta > 0) {
-    const long long at = rg.begin, start = at - cur.tile, stop = start + cur.it.tiles;
-    if (start != at && start >= at - rg.per) {
+    const long long tile0 = cur.pos - cur.tile, before = rg.begin - rg.per;  // where CTA b - 1 begins
+    if (tile0 < rg.begin && tile0 >= before) {
       c.first = 1;
-      c.last = (int)((stop - 1) / rg.per);
-      c.slot0 = start == at - rg.per ? 0 : 1;
+      c.last = (int)((tile0 + cur.it.tiles - 1) / rg.per);
+      c.slot0 = tile0 - p.item_cost <= before ? 0 : 1;  // the first item of CTA b - 1?
       c.start = cur.it.start, c.f0 = cur.it.f0, c.nf = cur.it.nf, c.head = cur.head;
     }
   }
