@@ -1,31 +1,39 @@
-// Attention of a chunk over a paged cache on the 5th-generation tensor cores,
-// for many query rows per KV head (prompts, chunks of prompts): f16 / bf16,
-// head sizes up to 128. The mathematics, the masks and the line of tiles cut
-// over the CTAs are those of kernels_paged_attn.cu.
+// Attention of a chunk over a paged cache on the 5th-generation tensor cores:
+// f16 / bf16, head sizes up to 128. The mathematics, the masks and the line of
+// tiles cut over the CTAs are those of kernels_paged_attn.cu.
 //
-// A CTA takes row tiles of 256 flattened rows (group heads x chunk rows) of
-// one KV head as two halves, A and B, of 128 rows, and walks the cache in
-// tiles of 128 tokens:
+// A CTA walks a row tile of one KV head through the cache in tiles of 128
+// tokens:
 //   S = Q K^T   tcgen05.mma, Q and K in shared memory, S in TMEM (f32)
 //   P = 2^(c S - c m), row sums   two warpgroups, one row per thread
 //   O += P V    tcgen05.mma, P in TMEM over S, V in shared memory, O in TMEM
-// The halves take turns: while one warpgroup works on its S, the tensor core
-// runs the other half's P V and next Q K^T. Per tile of both halves that is
-// 2,048 cycles of tensor core and, at 16 exponentials a cycle, 2,048 cycles of
-// the special function units for head size 128, so both bound it.
+// with two S and O in TMEM, halves A and B, that take turns: while a
+// warpgroup works on its S, the tensor core runs the other half's P V and next
+// Q K^T. With many query rows (prompts) the halves are the upper and lower
+// 128 of 256 flattened rows (group heads x chunk rows). With up to 128 (DUO:
+// decoding, draft verification) both take the same rows, A the even and B the
+// odd tiles of an item, and A joins the two at the item's end.
+//
+// Per tile of 256 rows and head size 128 that is 2,048 cycles of tensor core
+// and, at 16 exponentials a cycle, 2,048 cycles of the special function units,
+// so both bound it. With few rows HBM bounds it: a tile's K and V are 64 KB,
+// 1.45 us of an SM's share of the bandwidth, against 0.55 us of tensor core;
+// warps whose rows do not exist skip the softmax.
 //
 // The running maximum is lazy: m only moves (and O is only rescaled, in TMEM)
 // when a row's maximum passes it by more than 2^8; until then probabilities
 // grow up to 2^8, which f32 sums and the 16-bit types hold.
 //
 // Warps: 0-3 and 4-7 softmax of halves A and B, 8 TMEM and MMA issue (one
-// thread), 9 K and V by TMA, a piece of a page per lane, 10-11 the queries and
-// the hand-over of V tiles (in masked tiles they are looked through first).
-// Pages that TMA cannot fetch (sizes that are not 8 x 2^i or whole tiles) come
-// by 16-byte copies of warps 10-11. Tiles lie in the 128-byte swizzle the MMA
-// reads, K-major for Q K^T and N-major for P V. Every wait is bounded; on a
-// timeout all roles stop, what is in flight is waited for and the TMEM columns
-// are released.
+// thread; the MMAs of one thread run in issue order, so the next Q K^T may be
+// issued over a P that P V still reads), 9 K and V by TMA, a piece of a page
+// per lane (DUO: and the queries, two buffers), 10-11 the hand-over of V tiles
+// (in masked tiles they are looked through first) and the queries. Pages that
+// TMA cannot fetch (sizes that are not 8 x 2^i or whole tiles) come by 16-byte
+// copies of warps 10-11. Tiles lie in the 128-byte swizzle the MMA reads,
+// K-major for Q K^T and N-major for P V. Every wait is bounded; on a timeout
+// all roles stop, what is in flight is waited for and the TMEM columns are
+// released.
 #include <cuda_runtime.h>
 
 #include <mutex>
@@ -41,11 +49,13 @@ using namespace paged_attn;
 constexpr int kTcThreads = 12 * 32;
 constexpr int kProducers = 64;
 
-template <int DT_, int HD_>
+template <int DT_, int HD_, bool DUO_>
 struct Tc {
-  static constexpr int DT = DT_, HD = HD_, MT = 256, NT = 128;
-  static constexpr int kTileB = NT * HD * 2;           // a K or V tile
-  static constexpr int kQB = MT * HD * 2;
+  static constexpr int DT = DT_, HD = HD_, NT = 128;
+  static constexpr bool DUO = DUO_;
+  static constexpr int MT = DUO ? 128 : 256;
+  static constexpr int kTileB = NT * HD * 2;  // a K or V tile
+  static constexpr int kQB = 256 * HD * 2;    // DUO: two buffers
   static constexpr int kSlots = HD == 128 ? 5 : 10;
   static constexpr int kSmem = kQB + kSlots * kTileB + 1024;
   static constexpr int kPartFloats = MT * (HD + 2);
@@ -60,7 +70,9 @@ struct Tc {
 };
 
 constexpr float kLazy = 8.f;  // log2 units
-constexpr int kItemCost = 3;  // tiles
+// Few rows: from how many tokens a sequence can have this kernel is the faster
+// one.
+constexpr long long kTcFewRowsTokens = 1024;
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -68,24 +80,25 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
 }
-// 128-byte swizzle, rows of 128 bytes, 8-row atoms 1024 bytes apart (SBO);
-// lbo: distance of 64-element blocks of an N-major operand.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// Operand descriptors: 128-byte swizzle, rows of 128 bytes, 8-row atoms 1024
+// bytes apart (SBO); in the low word the address and the distance of the
+// 64-element blocks of an N-major operand (LBO), the high word is constant.
+// The issuing thread is on every tile's critical path, so a step of K costs it
+// one addition to each low word.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return ((addr & 0x3FFFFu) >> 4) | ((lbo >> 4) << 16); }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(kDescHi)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 y, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(kDescHi)
       : "memory");
 }
 __device__ __forceinline__ void tm_ld32(uint32_t taddr, uint32_t* v) {
@@ -112,23 +125,27 @@ __device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* v) {
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ bool try_bar(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Bounded wait (about a second of SM clock), polling: a wait with a suspend
 // hint wakes late.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, uint32_t* err) {
   const uint32_t a = smem_u32(bar);
+  if (try_bar(a, parity)) return true;
   const long long t0 = clock64();
-  for (;;) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(a), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if (clock64() - t0 > 2000000000ll) break;
-  }
-  if (err) atomicOr(err, kErrWaitTimeout);
-  return false;
+  while (!try_bar(a, parity))
+    if (clock64() - t0 > 2000000000ll) {
+      if (err) atomicOr(err, kErrWaitTimeout);
+      return false;
+    }
+  return true;
 }
 
 // Whether some row of the item may not see some token of the tile that
@@ -160,41 +177,58 @@ __device__ __forceinline__ bool look_through(uint32_t base, int tid) {
   return bad;
 }
 
-// The item's query rows, by kProducers threads; waits until they are there.
-template <typename C>
+// Requests the item's query rows, by THREADS threads. Rows that do not exist
+// keep what they held: no row of S depends on another's.
+template <typename C, int THREADS>
 __device__ __forceinline__ void load_queries(const Params& p, const Item& it, int kv_head, uint32_t sq, int tid) {
-  constexpr int kChunks = C::HD / 8, kRowsPer = kProducers / kChunks;
+  constexpr int kChunks = C::HD / 8, kRowsPer = THREADS / kChunks;
   const int chunk = tid % kChunks, r0 = tid / kChunks;
   const bool in_head = chunk * 8 < p.a.c.hd;
   const uint16_t* q = static_cast<const uint16_t*>(p.a.q) + (long long)it.start * p.a.q_row + (long long)kv_head * p.a.group * p.a.q_head + chunk * 8;
 #pragma unroll 1
-  for (int i0 = 0; i0 < C::MT / kRowsPer; i0 += 8) {
+  for (int i0 = 0; i0 * kRowsPer < it.nf; i0 += 8) {
     const uint16_t* src[8];
-    bool real[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int r = r0 + (i0 + i) * kRowsPer, f = it.f0 + r, qi = (int)p.group_div.quot(f), j = f - qi * p.a.group;
-      real[i] = r < it.nf && in_head;
-      src[i] = real[i] ? q + qi * p.a.q_row + j * p.a.q_head : q;
+      const int f = it.f0 + r0 + (i0 + i) * kRowsPer, qi = (int)p.group_div.quot(f), j = f - qi * p.a.group;
+      src[i] = in_head ? q + qi * p.a.q_row + j * p.a.q_head : q;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) cp_async16_or_zero(sq + tile_at(C::MT, r0 + (i0 + i) * kRowsPer, chunk), src[i], real[i]);
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + (i0 + i) * kRowsPer;
+      if (r < it.nf) cp_async16_or_zero(sq + tile_at(C::MT, r, chunk), src[i], in_head);
+    }
   }
   cp_async_commit();
-  cp_async_wait<0>();
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 constexpr int kLanded = 8;  // V tiles between their landing and their hand-over
+
+// What the issuing thread has to know of a tile: it is the last of its item;
+// the last of its item here; the last of the CTA.
+enum : uint32_t { kLastOfItem = 1, kLastHere = 2, kLastOfCta = 4 };
+template <int MT, int NT>
+__device__ __forceinline__ uint32_t flags_of(const Params& p, const Cursor<MT, NT>& cur, long long end) {
+  uint32_t f = (cur.last_of_item() ? kLastOfItem : 0) | (cur.ends(end) ? kLastHere : 0);
+  // The next tile of the line lies behind the next item's cost.
+  if (cur.pos + 1 + (cur.last_of_item() ? p.item_cost : 0) >= end) f |= kLastOfCta;
+  return f;
+}
 
 template <typename C, bool CAP, bool TMA>
 __global__ void __launch_bounds__(kTcThreads, 1)
     paged_attn_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ KvMaps maps, int box) {
   constexpr int DT = C::DT, HD = C::HD, MT = C::MT, NT = C::NT;
+  constexpr bool DUO = C::DUO;
+  constexpr int kQThreads = DUO ? 32 : kProducers;
   extern __shared__ uint8_t smem_raw[];
   __shared__ long long sh[kPlanWords];
-  __shared__ uint64_t kv_full[C::kSlots], kv_empty[C::kSlots], q_full, q_empty, s_full[2], p_full[2], o_done[2], drained;
+  __shared__ uint64_t kv_full[C::kSlots], kv_empty[C::kSlots], q_full[2], q_empty[2], s_full[2], p_full[2], o_done[2], drained;
+  __shared__ uint64_t b_ready, b_read;  // DUO: half B's sums are there, were read
+  __shared__ float2 b_sums[DUO ? 128 : 1];  // half B's (m, l)
   __shared__ uint64_t landed[kLanded];
+  __shared__ uint32_t flags[C::kSlots];  // of the tile whose K is in the slot
   __shared__ uint32_t tmem_slot;
   __shared__ int poison[4];  // ordinal + 1 of an item with masked V values that are not finite
   const uint32_t sq = (smem_u32(smem_raw) + 1023) & ~1023u, skv = sq + C::kQB;
@@ -207,9 +241,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&kv_full[i], TMA ? 1 : kProducers);
       mbar_init(&kv_empty[i], 1);
     }
-    mbar_init(&q_full, kProducers);
-    mbar_init(&q_empty, 1);
+    mbar_init(&b_ready, 4);
+    mbar_init(&b_read, 4);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], kQThreads);
+      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_done[i], 1);
@@ -245,20 +281,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       TilePieces<NT, HD / 64, 2> pieces;
       pieces.fetch(ch, cur.it, (cur.it.first + cur.tile) * NT, box, lane);
       uint32_t issued = 0;
-      bool ok = true;
+      int items = 0;
+      bool ok = true, fresh = true;
       for (uint32_t k = 0; cur.pos < end && ok; ++k) {
         const Item& it = cur.it;
         const int t0 = (it.first + cur.tile) * NT;
+        const bool queries = DUO && fresh;
+        if (queries) {
+          if (items >= 2) ok = __all_sync(~0u, wait_bar(&q_empty[items & 1], (items / 2 - 1) & 1, err));
+          if (!ok) break;
+          load_queries<C, 32>(p, it, cur.head, sq + (items & 1) * MT * HD * 2, lane);
+        }
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           const uint32_t n = 2 * k + kv, slot = n % C::kSlots, use = n / C::kSlots;
           if (ok && use > 0) ok = __all_sync(~0u, wait_bar(&kv_empty[slot], (use - 1) & 1, err));
           if (ok) {
+            if (kv == 0 && lane == 0) flags[slot] = flags_of<MT, NT>(p, cur, end);
             pieces.load(ch, it, t0, box, lane, kv ? &maps.v : &maps.k, cur.head, skv + slot * C::kTileB,
                         kv ? &landed[k % kLanded] : &kv_full[slot]);
             ++issued;
           }
         }
+        if (queries) {
+          cp_async_wait<0>();
+          fence_async();
+          mbar_arrive(&q_full[items & 1]);
+          ++items;
+        }
+        fresh = cur.last_of_item();
         cur.next(p);
         if (cur.pos < end) pieces.fetch(ch, cur.it, (cur.it.first + cur.tile) * NT, box, lane);
       }
@@ -277,17 +328,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       bool fresh = true;
       for (uint32_t k = 0; cur.pos < end; ++k) {
         const Item& it = cur.it;
-        if (fresh) {
-          if (k > 0 && !__all_sync(~0u, wait_bar(&q_empty, (items - 1) & 1, err))) break;
-          load_queries<C>(p, it, cur.head, sq, tid);
-          mbar_arrive(&q_full);
+        if (!DUO && fresh) {
+          if (k > 0 && !__all_sync(~0u, wait_bar(&q_empty[0], (items - 1) & 1, err))) break;
+          load_queries<C, kProducers>(p, it, cur.head, sq, tid);
+          cp_async_wait<0>();
+          fence_async();
+          mbar_arrive(&q_full[0]);
           fresh = false;
         }
         if (!__all_sync(~0u, wait_bar(&landed[k % kLanded], k / kLanded & 1, err))) break;
         const uint32_t slot = (2 * k + 1) % C::kSlots;
         if (tile_masked(it, (it.first + cur.tile) * NT, NT, p.a.window, p.group_div)) {
           if (look_through<C>(skv + slot * C::kTileB, tid)) *(volatile int*)&poison[items & 3] = items + 1;
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          fence_async();
           asm volatile("bar.sync 1, 64;" ::: "memory");
         }
         if (tid == 0) mbar_arrive(&kv_full[slot]);
@@ -316,7 +369,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       auto hand = [&](int age) {  // the fetch `handed` has landed
         const uint32_t slot = handed % C::kSlots;
         if ((look >> age & 1u) && look_through<C>(skv + slot * C::kTileB, tid)) *(volatile int*)&poison[items & 3] = items + 1;
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        fence_async();
         mbar_arrive(&kv_full[slot]);
         ++handed;
       };
@@ -329,12 +382,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           while (handed < n) hand((int)(n - 1 - handed));
           if (!first) {
             ++items;
-            ok = wait_bar(&q_empty, (items - 1) & 1, err);
+            ok = wait_bar(&q_empty[0], (items - 1) & 1, err);
             if (!ok) break;
           }
           first = false;
-          load_queries<C>(p, cur.it, cur.head, sq, tid);
-          mbar_arrive(&q_full);
+          load_queries<C, kProducers>(p, cur.it, cur.head, sq, tid);
+          cp_async_wait<0>();
+          fence_async();
+          mbar_arrive(&q_full[0]);
           fresh = false;
         }
         const Item& it = cur.it;
@@ -366,6 +421,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               cp_async16_or_zero(base + tile_at(NT, r0 + (i0 + i) * kRowsPer, chunk), o[i] >= 0 ? src + o[i] : src, o[i] >= 0);
           }
           cp_async_commit();
+          if (kv == 0 && tid == 0) flags[slot] = flags_of<MT, NT>(p, cur, end);
           look = look << 1 | (kv && tile_masked(it, t0, NT, p.a.window, p.group_div) ? 1u : 0u);
           ++n;
           if (n - handed > (uint32_t)kLag) {
@@ -383,68 +439,118 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     } else if (begin < end && warp == 8) {
       // ---------------- MMA issue ----------------
       if (lane == 0) {
-        Cursor<MT, NT> cur;
-        cur.seek(p, rg);
+        // K of tile k is fetch 2k, V is fetch 2k + 1, fetch n in slot n % kSlots.
+        struct Slot {
+          uint32_t i, phase;
+          __device__ __forceinline__ void skip() {  // two fetches on
+            i += 2;
+            if (i >= (uint32_t)C::kSlots) i -= C::kSlots, phase ^= 1;
+          }
+        } ks = {0, 0}, vs = {1, 0};
         bool ok = true;
         int items = 0;
-        auto qk = [&](int half, uint32_t k) {  // S of half for the CTA's k-th tile
-          const uint32_t a0 = sq + half * 128 * 128, b0 = skv + (2 * k) % C::kSlots * C::kTileB;
+        uint32_t k = 0;
+        auto qk = [&](int half) {
+          const uint32_t a0 = desc_lo(sq + (DUO ? (items & 1) * MT * HD * 2 : half * 128 * 128), 16);
+          const uint32_t b0 = desc_lo(skv + ks.i * C::kTileB, 16);
 #pragma unroll
           for (int x = 0; x < HD / 16; ++x) {
-            const uint32_t in = (x & 3) * 32;
-            mma_ss(tmem + half * 128, desc_sw128(a0 + (x >> 2) * MT * 128 + in, 16), desc_sw128(b0 + (x >> 2) * NT * 128 + in, 16),
-                   C::kIdescQK, x > 0);
+            const uint32_t in = (x & 3) * 2;
+            mma_ss(tmem + half * 128, a0 + (x >> 2) * (MT * 8) + in, b0 + (x >> 2) * (NT * 8) + in, C::kIdescQK, x > 0);
           }
           commit(&s_full[half]);
         };
-        auto pv = [&](int half, uint32_t k, bool add) {
-          const uint32_t b0 = skv + (2 * k + 1) % C::kSlots * C::kTileB;
+        auto pv = [&](int half, bool add) {
+          const uint32_t b0 = desc_lo(skv + vs.i * C::kTileB, NT * 128);
 #pragma unroll
           for (int x = 0; x < NT / 16; ++x)
-            mma_ts(tmem + 256 + half * HD, tmem + half * 128 + x * 8, desc_sw128(b0 + x * 2048, NT * 128), C::kIdescPV, add || x > 0);
+            mma_ts(tmem + 256 + half * HD, tmem + half * 128 + x * 8, b0 + x * 128, C::kIdescPV, add || x > 0);
           commit(&o_done[half]);
         };
-        auto wait_kv = [&](uint32_t i) { return wait_bar(&kv_full[i % C::kSlots], i / C::kSlots & 1, err); };
-        // Queries, K and V of a tile are waited for once each, before the first
-        // MMA that reads them.
-        bool first = true;  // tile k is its item's first here
-        ok = cur.pos < end && wait_bar(&q_full, 0, err) && wait_kv(0);
-        if (ok) {
-          fence_after();
-          qk(0, 0);
-          qk(1, 0);
-          commit(&kv_empty[0]);
-          if (cur.ends(end)) commit(&q_empty);
-        }
-        for (uint32_t k = 0; cur.pos < end && ok; ++k) {
-          const bool last = cur.last_of_item();
-          cur.next(p);
-          const bool more = cur.pos < end;
-          ok = wait_kv(2 * k + 1) && wait_bar(&p_full[0], k & 1, err);
-          if (!ok) break;
-          fence_after();
-          pv(0, k, !first);
-          if (more) {
-            if (last) {
-              ++items;
-              ok = wait_bar(&q_full, items & 1, err);
-            }
-            ok = ok && wait_kv(2 * k + 2);
+        if constexpr (!DUO) {
+          bool first = true;  // tile k is its item's first here
+          uint32_t now = 0, next = 0;
+          ok = wait_bar(&q_full[0], 0, err) && wait_bar(&kv_full[0], 0, err);
+          if (ok) {
+            fence_after();
+            next = flags[0];
+            qk(0);
+            qk(1);
+            commit(&kv_empty[0]);
+            ks.skip();
+            if (next & kLastHere) commit(&q_empty[0]);
+          }
+          for (; ok; ++k) {
+            now = next;
+            ok = wait_bar(&kv_full[vs.i], vs.phase, err) && wait_bar(&p_full[0], k & 1, err);
             if (!ok) break;
             fence_after();
-            qk(0, k + 1);
+            pv(0, !first);
+            if (!(now & kLastOfCta)) {
+              if (now & kLastOfItem) {
+                ++items;
+                ok = wait_bar(&q_full[0], items & 1, err);
+              }
+              ok = ok && wait_bar(&kv_full[ks.i], ks.phase, err);
+              if (!ok) break;
+              fence_after();
+              next = flags[ks.i];
+              qk(0);
+            }
+            ok = wait_bar(&p_full[1], k & 1, err);
+            if (!ok) break;
+            fence_after();
+            pv(1, !first);
+            commit(&kv_empty[vs.i]);
+            vs.skip();
+            if (now & kLastOfCta) break;
+            qk(1);
+            commit(&kv_empty[ks.i]);
+            ks.skip();
+            if (next & kLastHere) commit(&q_empty[0]);  // tile k + 1 is its item's last here: the queries may go
+            first = now & kLastOfItem;
           }
-          ok = wait_bar(&p_full[1], k & 1, err);
-          if (!ok) break;
-          fence_after();
-          pv(1, k, !first);
-          commit(&kv_empty[(2 * k + 1) % C::kSlots]);
-          if (more) {
-            qk(1, k + 1);
-            commit(&kv_empty[(2 * k + 2) % C::kSlots]);
-            if (cur.ends(end)) commit(&q_empty);  // tile k + 1 is its item's last here: the queries may go
+        } else {
+          // Q K^T runs ahead of P V by one S of each half, in the line's order.
+          bool q_fresh = true, q_more = true;
+          int q_half = 0, v_half = 0, v_in = 0;
+          uint32_t phase = 0, busy = 0;  // bit per half
+          uint32_t ahead = 0, n_ahead = 0;  // flags of the tiles between, 4 bits each
+          while (ok) {
+            while (ok && q_more && !(busy >> q_half & 1u)) {
+              if (q_fresh) ok = wait_bar(&q_full[items & 1], items >> 1 & 1, err);
+              ok = ok && wait_bar(&kv_full[ks.i], ks.phase, err);
+              if (!ok) break;
+              fence_after();
+              const uint32_t f = flags[ks.i];
+              if (q_half == 0) qk(0); else qk(1);
+              commit(&kv_empty[ks.i]);
+              ks.skip();
+              busy |= 1u << q_half;
+              ahead |= f << (4 * n_ahead++);
+              q_more = !(f & kLastOfCta);
+              q_fresh = f & kLastHere;
+              if (q_fresh) {
+                commit(&q_empty[items & 1]);
+                ++items;
+              }
+              q_half = f & kLastOfItem ? 0 : q_half ^ 1;
+            }
+            if (!ok) break;
+            ok = wait_bar(&kv_full[vs.i], vs.phase, err) && wait_bar(&p_full[v_half], phase >> v_half & 1u, err);
+            if (!ok) break;
+            phase ^= 1u << v_half;
+            busy &= ~(1u << v_half);
+            fence_after();
+            if (v_half == 0) pv(0, v_in >= 2); else pv(1, v_in >= 2);
+            commit(&kv_empty[vs.i]);
+            vs.skip();
+            const uint32_t f = ahead & 15u;
+            ahead >>= 4, --n_ahead;
+            if (f & kLastOfCta) break;
+            v_in = f & kLastOfItem ? 0 : v_in + 1;
+            v_half = f & kLastOfItem ? 0 : v_half ^ 1;
           }
-          first = last;
         }
         commit(&drained);
         wait_bar(&drained, 0, nullptr);
@@ -459,137 +565,195 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint32_t ts = tmem + half * 128 + lanes, to = tmem + 256 + half * HD + lanes;
       Cursor<MT, NT> cur;
       cur.seek(p, rg);
-      int items = 0;
+      int items = 0, in = 0;  // in: tiles of the item so far
       bool ok = true;
       float m = -INFINITY, l = 0.f;  // m: of the raw scores
-      uint32_t k = 0, k_first = 0;
-      for (; cur.pos < end; ++k) {
+      uint32_t k = 0, k_first = 0;   // this half's tiles; the item's first
+      for (; cur.pos < end; ++in) {
         const Item& it = cur.it;
-        const int f = it.f0 + half * 128 + row, qi = (int)p.group_div.quot(f);
-        const bool real = half * 128 + row < it.nf;
+        const int r = DUO ? row : half * 128 + row;
+        const int f = it.f0 + r, qi = (int)p.group_div.quot(f);
+        const bool real = r < it.nf;
+        const bool idle = __all_sync(~0u, !real);
         const int pos = real ? it.len - it.n + qi : -1;
-        const int t0 = (it.first + cur.tile) * NT;
-        ok = __all_sync(~0u, wait_bar(&s_full[half], k & 1, err));
-        if (!ok) break;
-        fence_after();
-        uint32_t v[128];
+        if (!DUO || (in & 1) == half) {
+          ok = __all_sync(~0u, wait_bar(&s_full[half], k & 1, err));
+          if (!ok) break;
+          if (!idle) {
+            const int t0 = (it.first + cur.tile) * NT;
+            fence_after();
+            uint32_t v[128];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) tm_ld32(ts + 32 * x, v + 32 * x);
-        tm_wait_ld();
-        if constexpr (CAP) {
+            for (int x = 0; x < 4; ++x) tm_ld32(ts + 32 * x, v + 32 * x);
+            tm_wait_ld();
+            if constexpr (CAP) {
 #pragma unroll
-          for (int x = 0; x < 128; ++x) v[x] = __float_as_uint(capped<DT>(__uint_as_float(v[x]), p.a.scale, p.a.softcap));
+              for (int x = 0; x < 128; ++x) v[x] = __float_as_uint(capped<DT>(__uint_as_float(v[x]), p.a.scale, p.a.softcap));
+            }
+            if (tile_masked(it, t0, NT, p.a.window, p.group_div)) {
+              const int from = max(it.lo, p.a.window > 0 ? pos - p.a.window + 1 : 0) - t0, till = pos - t0;
+#pragma unroll
+              for (int x = 0; x < 128; ++x)
+                if (x > till || x < from) v[x] = 0xff800000u;
+            }
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int x = 0; x < 128; x += 2)
+              tops[x / 2 & 3] = fmaxf(tops[x / 2 & 3], fmaxf(__uint_as_float(v[x]), __uint_as_float(v[x + 1])));
+            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+            const bool move = top > m && (m == -INFINITY || (top - m) * p.c > kLazy);
+            if (__any_sync(~0u, move)) {
+              const float next = move ? top : m;
+              const float fix = move && m != -INFINITY ? exp2_fast((m - next) * p.c) : 1.f;
+              l *= fix;
+              m = next;
+              if (k > k_first) {
+                ok = __all_sync(~0u, wait_bar(&o_done[half], (k - 1) & 1, err));
+                if (!ok) break;
+                fence_after();
+#pragma unroll 1
+                for (int x = 0; x < HD; x += 32) {
+                  uint32_t o[32];
+                  tm_ld32(to + x, o);
+                  tm_wait_ld();
+#pragma unroll
+                  for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * fix);
+                  tm_st32(to + x, o);
+                }
+              }
+            }
+            const float mc = (m == -INFINITY ? 0.f : m * p.c) - C::kPShift;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < 64; ++x) {
+              const float a = exp2_fast(fmaf(__uint_as_float(v[2 * x]), p.c, -mc));
+              const float b = exp2_fast(fmaf(__uint_as_float(v[2 * x + 1]), p.c, -mc));
+              sum[x & 1] += a;
+              sum[2 + (x & 1)] += b;
+              v[x] = pack<DT>(a, b);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tm_st32(ts, v);
+            tm_st32(ts + 32, v + 32);
+            tm_wait_st();
+            fence_before();
+          }
+          // Half B's O of the last item has been read before it is written anew.
+          if (DUO && half == 1 && in == 1 && items > 0) {
+            ok = __all_sync(~0u, wait_bar(&b_read, (items - 1) & 1, err));
+            if (!ok) break;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[half]);
+          ++k;
         }
-        if (tile_masked(it, t0, NT, p.a.window, p.group_div)) {
-          const int from = max(it.lo, p.a.window > 0 ? pos - p.a.window + 1 : 0) - t0, till = pos - t0;
-#pragma unroll
-          for (int x = 0; x < 128; ++x)
-            if (x > till || x < from) v[x] = 0xff800000u;
-        }
-        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int x = 0; x < 128; x += 2)
-          tops[x / 2 & 3] = fmaxf(tops[x / 2 & 3], fmaxf(__uint_as_float(v[x]), __uint_as_float(v[x + 1])));
-        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        const bool move = top > m && (m == -INFINITY || (top - m) * p.c > kLazy);
-        if (__any_sync(~0u, move)) {
-          const float next = move ? top : m;
-          const float fix = move && m != -INFINITY ? exp2_fast((m - next) * p.c) : 1.f;
-          l *= fix;
-          m = next;
+
+        if (cur.ends(end)) {
+          // ---- end of the item, or of this CTA's part of it ----
           if (k > k_first) {
             ok = __all_sync(~0u, wait_bar(&o_done[half], (k - 1) & 1, err));
             if (!ok) break;
             fence_after();
-#pragma unroll 1
-            for (int x = 0; x < HD; x += 32) {
-              uint32_t o[32];
-              tm_ld32(to + x, o);
-              tm_wait_ld();
-#pragma unroll
-              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * fix);
-              tm_st32(to + x, o);
-            }
           }
-        }
-        const float mc = (m == -INFINITY ? 0.f : m * p.c) - C::kPShift;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int x = 0; x < 64; ++x) {
-          const float a = exp2_fast(fmaf(__uint_as_float(v[2 * x]), p.c, -mc));
-          const float b = exp2_fast(fmaf(__uint_as_float(v[2 * x + 1]), p.c, -mc));
-          sum[x & 1] += a;
-          sum[2 + (x & 1)] += b;
-          v[x] = pack<DT>(a, b);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tm_st32(ts, v);
-        tm_st32(ts + 32, v + 32);
-        tm_wait_st();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[half]);
-
-        if (cur.ends(end)) {
-          // ---- end of the item, or of this CTA's part of it ----
-          ok = __all_sync(~0u, wait_bar(&o_done[half], k & 1, err));
-          if (!ok) break;
-          fence_after();
-          const long long item_at = cur.pos - cur.tile;  // of its first tile
-          const bool whole = item_at >= begin && cur.last_of_item();
-          const bool poisoned = *(volatile int*)&poison[items & 3] == items + 1;
-          const int r = half * 128 + row, j = f - qi * p.a.group, head = cur.head * p.a.group + j;
-          const float inv = !whole ? 1.f : l > 0.f || l != l ? 1.f / l : 0.f;
-          float* part = part_of(p, C::kPartFloats, blockIdx.x, items ? 1 : 0);
-          uint16_t* out = static_cast<uint16_t*>(p.a.out) + (long long)(it.start + qi) * p.a.o_row + (long long)head * p.a.o_head;
+          if (DUO && half == 1) {
+            // Half A joins: it reads these sums, and O from the TMEM lanes that
+            // its warps share with this half's.
+            if (items > 0) {
+              ok = __all_sync(~0u, wait_bar(&b_read, (items - 1) & 1, err));
+              if (!ok) break;
+            }
+            b_sums[row] = make_float2(m, l);
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b_ready);
+          } else {
+            float fix_a = 1.f, fix_b = 0.f;
+            if (DUO) {
+              ok = __all_sync(~0u, wait_bar(&b_ready, items & 1, err));
+              if (!ok) break;
+              fence_after();
+              const float2 o = b_sums[row];
+              const float top = fmaxf(m, o.x), ref = top == -INFINITY ? 0.f : top;
+              fix_a = exp2_fast((m - ref) * p.c);
+              fix_b = exp2_fast((o.x - ref) * p.c);
+              l = l * fix_a + o.y * fix_b;
+              m = top;
+            }
+            const bool two = DUO && in >= 1;  // half B has had a tile
+            if (!idle) {
+              const long long item_at = cur.pos - cur.tile;  // of its first tile
+              const bool whole = item_at >= begin && cur.last_of_item();
+              const bool poisoned = *(volatile int*)&poison[items & 3] == items + 1;
+              const int j = f - qi * p.a.group, head = cur.head * p.a.group + j;
+              const float inv = !whole ? 1.f : l > 0.f || l != l ? 1.f / l : 0.f;
+              float* part = part_of(p, C::kPartFloats, blockIdx.x, items ? 1 : 0);
+              uint16_t* out = static_cast<uint16_t*>(p.a.out) + (long long)(it.start + qi) * p.a.o_row + (long long)head * p.a.o_head;
 #pragma unroll 1
-          for (int x = 0; x < HD; x += 32) {
-            uint32_t o[32];
-            tm_ld32(to + x, o);
-            tm_wait_ld();
-            if (poisoned && real) {
-              // A row that sees a V value which is not finite gets it after all.
-              const int ta = it.first * NT + (int)max(0ll, begin - item_at) * NT, tb = (it.first + cur.tile + 1) * NT;
-              const int from = max(max(ta, it.lo), p.a.window > 0 ? pos - p.a.window + 1 : 0), till = min(min(tb, it.hi), pos + 1);
-              for (int t = from; t < till; ++t) {
-                if (!tile_masked(it, t / NT * NT, NT, p.a.window, p.group_div)) continue;
-                const int pi = (int)ch.page.quot(t), page = page_of(ch, it.seq, pi);
-                if (page < 0) continue;
-                const long long vo = page * ch.v_page + (long long)cur.head * ch.v_head + (t - pi * (int)ch.page.d) * ch.v_slot;
+              for (int x = 0; x < HD; x += 32) {
+                uint32_t o[32];
+                __syncwarp();
+                tm_ld32(to + x, o);
+                tm_wait_ld();
+                if (DUO) {
+                  uint32_t ob[32];
+                  if (two) tm_ld32(to + HD + x, ob);
+                  tm_wait_ld();
 #pragma unroll
-                for (int y = 0; y < 32; ++y) {
-                  const float w = x + y < ch.hd ? value<DT>(ch.v, vo + x + y) : 0.f;
-                  if (!(fabsf(w) <= 3.4028235e38f)) o[y] = __float_as_uint(__uint_as_float(o[y]) + w);
+                  for (int y = 0; y < 32; ++y) {
+                    float w = __uint_as_float(o[y]) * fix_a;
+                    if (two && fix_b != 0.f) w += __uint_as_float(ob[y]) * fix_b;
+                    o[y] = __float_as_uint(w);
+                  }
+                }
+                if (poisoned && real) {
+                  // A row that sees a V value which is not finite gets it after all.
+                  const int ta = it.first * NT + (int)max(0ll, begin - item_at) * NT, tb = (it.first + cur.tile + 1) * NT;
+                  const int from = max(max(ta, it.lo), p.a.window > 0 ? pos - p.a.window + 1 : 0), till = min(min(tb, it.hi), pos + 1);
+                  for (int t = from; t < till; ++t) {
+                    if (!tile_masked(it, t / NT * NT, NT, p.a.window, p.group_div)) continue;
+                    const int pi = (int)ch.page.quot(t), page = page_of(ch, it.seq, pi);
+                    if (page < 0) continue;
+                    const long long vo = page * ch.v_page + (long long)cur.head * ch.v_head + (t - pi * (int)ch.page.d) * ch.v_slot;
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) {
+                      const float w = x + y < ch.hd ? value<DT>(ch.v, vo + x + y) : 0.f;
+                      if (!(fabsf(w) <= 3.4028235e38f)) o[y] = __float_as_uint(__uint_as_float(o[y]) + w);
+                    }
+                  }
+                }
+                if (!real) continue;
+                if (!whole) {
+#pragma unroll
+                  for (int y = 0; y < 32; y += 4)
+                    *reinterpret_cast<uint4*>(part + r * HD + x + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+                } else {
+#pragma unroll
+                  for (int y = 0; y < 32; y += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int z = 0; z < 4; ++z)
+                      w[z] = pack<DT>(__uint_as_float(o[y + 2 * z]) * inv, __uint_as_float(o[y + 2 * z + 1]) * inv);
+                    if (x + y < ch.hd) *reinterpret_cast<uint4*>(out + x + y) = make_uint4(w[0], w[1], w[2], w[3]);
+                  }
                 }
               }
-            }
-            if (!whole) {
-#pragma unroll
-              for (int y = 0; y < 32; y += 4)
-                *reinterpret_cast<uint4*>(part + r * HD + x + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
-            } else if (real) {
-#pragma unroll
-              for (int y = 0; y < 32; y += 8) {
-                uint32_t w[4];
-#pragma unroll
-                for (int z = 0; z < 4; ++z)
-                  w[z] = pack<DT>(__uint_as_float(o[y + 2 * z]) * inv, __uint_as_float(o[y + 2 * z + 1]) * inv);
-                if (x + y < ch.hd) *reinterpret_cast<uint4*>(out + x + y) = make_uint4(w[0], w[1], w[2], w[3]);
+              if (real && !whole) {
+                part[MT * HD + r] = m == -INFINITY ? -INFINITY : m * p.c;
+                part[MT * HD + MT + r] = l;
+              } else if (real && p.a.lse) {
+                p.a.lse[(long long)(it.start + qi) * (ch.nkv * p.a.group) + head] =
+                    l > 0.f || l != l ? (m * p.c - C::kPShift) * kLn2 + logf(l) : -INFINITY;
               }
             }
+            fence_before();
+            __syncwarp();
+            if (DUO && lane == 0) mbar_arrive(&b_read);
           }
-          if (!whole) {
-            part[MT * HD + r] = m == -INFINITY ? -INFINITY : m * p.c;
-            part[MT * HD + MT + r] = l;
-          } else if (real && p.a.lse) {
-            p.a.lse[(long long)(it.start + qi) * (ch.nkv * p.a.group) + head] =
-                l > 0.f || l != l ? (m * p.c - C::kPShift) * kLn2 + logf(l) : -INFINITY;
-          }
-          fence_before();
           ++items;
+          in = -1;
           m = -INFINITY;
           l = 0.f;
-          k_first = k + 1;
+          k_first = k;
         }
         cur.next(p);
       }
@@ -624,8 +788,8 @@ cudaError_t launch(const AttnArgs& a, const KvMaps& maps, int box, cudaStream_t 
   p.group_div = FastDiv(a.group);
   p.grid = device_sm_count();
   p.whole = false;
-  p.min_tiles = 8;
-  p.item_cost = kItemCost;
+  p.min_tiles = C::DUO ? 6 : 8;
+  p.item_cost = C::DUO ? 2 : 3;
   p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
   // Not launched ahead of its predecessor's end: its CTAs would share the SMs
   // with the last call's join and run unevenly.
@@ -635,27 +799,33 @@ cudaError_t launch(const AttnArgs& a, const KvMaps& maps, int box, cudaStream_t 
   return launch_pdl(paged_combine_kernel<C>, dim3(p.grid - 1, combine_grid_y(C::MT)), dim3(kCombineThreads), 0, s, p);
 }
 
-}  // namespace
-
-bool paged_attention_tc_takes(const AttnArgs& a) {
-  return a.dtype != kF32 && a.c.hd <= 128 && (long long)a.c.max_rows * a.group > 64;
-}
-
-size_t paged_attention_tc_workspace(const AttnArgs& a) {
-  return cut_bytes(device_sm_count()) + 2ull * device_sm_count() * (a.c.hd <= 64 ? Tc<kBF16, 64>::kPartFloats : Tc<kBF16, 128>::kPartFloats) * 4;
-}
-
-cudaError_t paged_attention_tc(const AttnArgs& a, cudaStream_t s) {
+template <int DT, int HD>
+cudaError_t choose(const AttnArgs& a, cudaStream_t s) {
   KvMaps maps;
   const int box = tma_box((int)a.c.page.d, 128);
   const bool tma = box && make_maps(a.c, a.dtype, box, &maps);
-#define RAI_TC(DT, HD)                                                                                                   \
-  (a.softcap > 0.f ? (tma ? launch<Tc<DT, HD>, true, true>(a, maps, box, s) : launch<Tc<DT, HD>, true, false>(a, maps, box, s)) \
-                   : (tma ? launch<Tc<DT, HD>, false, true>(a, maps, box, s)                                             \
-                          : launch<Tc<DT, HD>, false, false>(a, maps, box, s)))
-  if (a.dtype == kF16) return a.c.hd <= 64 ? RAI_TC(kF16, 64) : RAI_TC(kF16, 128);
-  return a.c.hd <= 64 ? RAI_TC(kBF16, 64) : RAI_TC(kBF16, 128);
-#undef RAI_TC
+  const bool duo = (long long)a.c.max_rows * a.group <= 128, cap = a.softcap > 0.f;
+  if (!tma) return cap ? launch<Tc<DT, HD, false>, true, false>(a, maps, box, s) : launch<Tc<DT, HD, false>, false, false>(a, maps, box, s);
+  if (duo) return cap ? launch<Tc<DT, HD, true>, true, true>(a, maps, box, s) : launch<Tc<DT, HD, true>, false, true>(a, maps, box, s);
+  return cap ? launch<Tc<DT, HD, false>, true, true>(a, maps, box, s) : launch<Tc<DT, HD, false>, false, true>(a, maps, box, s);
+}
+
+}  // namespace
+
+bool paged_attention_tc_takes(const AttnArgs& a) {
+  if (a.dtype == kF32 || a.c.hd > 128) return false;
+  if ((long long)a.c.max_rows * a.group > 64) return true;
+  return tma_box((int)a.c.page.d, 128) && (long long)a.c.max_pages * a.c.page.d >= kTcFewRowsTokens;
+}
+
+size_t paged_attention_tc_workspace(const AttnArgs& a) {
+  return cut_bytes(device_sm_count()) +
+         2ull * device_sm_count() * (a.c.hd <= 64 ? Tc<kBF16, 64, false>::kPartFloats : Tc<kBF16, 128, false>::kPartFloats) * 4;
+}
+
+cudaError_t paged_attention_tc(const AttnArgs& a, cudaStream_t s) {
+  if (a.dtype == kF16) return a.c.hd <= 64 ? choose<kF16, 64>(a, s) : choose<kF16, 128>(a, s);
+  return a.c.hd <= 64 ? choose<kBF16, 64>(a, s) : choose<kBF16, 128>(a, s);
 }
 
 }  // namespace rai

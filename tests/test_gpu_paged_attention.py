@@ -56,11 +56,14 @@ def make_q(T, H, D, dtype, dev, seed=1, scale=1.0):
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("heads,nkv,hd", [(14, 2, 64), (32, 8, 128), (4, 4, 32), (6, 2, 96), (15, 5, 80), (4, 2, 256),
                                           (8, 1, 16), (5, 1, 136)])
-def test_shapes_and_lengths(dtype, heads, nkv, hd):
+@pytest.mark.parametrize("wide", [0, 150])
+def test_shapes_and_lengths(dtype, heads, nkv, hd, wide):
+    """A table for longer sequences than there are (wide) may choose another
+    kernel."""
     dev = torch.device("cuda", 0)
     rows = [1, 2, 0, 9, 1, 5, 1, 1]
     lens = [1, 64, 7, 65, 200, 5, 63, 129]
-    c = ref.Cache(lens, nkv, hd, 16, dtype, dev, seed=hd)
+    c = ref.Cache(lens, nkv, hd, 16, dtype, dev, seed=hd, wide=wide)
     q = make_q(sum(rows) + 4, heads, hd, dtype, dev)
     got, lse = run(c, q, rows, first=2)
     agree(c, q, rows, got, lse, first=2)
@@ -69,11 +72,11 @@ def test_shapes_and_lengths(dtype, heads, nkv, hd):
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("page", [1, 3, 16, 100, 256])
 @pytest.mark.parametrize("softcap,window", [(0.0, 0), (20.0, 0), (0.0, 1), (0.0, 70), (5.0, 33)])
-def test_pages_caps_and_windows(dtype, page, softcap, window):
+@pytest.mark.parametrize("rows", [[3, 1, 12, 40], [3, 1, 12, 20]], ids=["many", "few"])
+def test_pages_caps_and_windows(dtype, page, softcap, window, rows):
     dev = torch.device("cuda", 0)
-    rows = [3, 1, 12, 40]
     lens = [3, 300, 130, 140]
-    c = ref.Cache(lens, 2, 64, page, dtype, dev, seed=page)
+    c = ref.Cache(lens, 2, 64, page, dtype, dev, seed=page, wide=1 + 2000 // page)
     q = make_q(sum(rows), 6, 64, dtype, dev, scale=2.0)
     got, lse = run(c, q, rows, softcap=softcap, window=window)
     agree(c, q, rows, got, lse, softcap=softcap, window=window)
@@ -95,7 +98,7 @@ def test_long_chunks(dtype, heads, nkv, hd, softcap, window):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("rows,lens", [([1], [5000]), ([1, 1], [9000, 3]), ([9, 4, 1], [4000, 6500, 2500]),
-                                       ([33], [3000])])
+                                       ([33], [3000]), ([1] * 40, list(range(200, 4200, 100))), ([2, 1, 3] * 9, [1500, 1100, 4000] * 9)])
 def test_few_long_sequences_are_cut(dtype, rows, lens):
     dev = torch.device("cuda", 0)
     c = ref.Cache(lens, 2, 64, 16, dtype, dev, seed=len(lens))
@@ -108,11 +111,13 @@ def test_few_long_sequences_are_cut(dtype, rows, lens):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("hd", [64, 128])
-def test_rows_that_see_nothing(dtype, hd):
+@pytest.mark.parametrize("rows", [[5, 3, 150, 200], [5, 3, 40, 7]], ids=["many", "few"])
+@pytest.mark.parametrize("wide", [0, 150])
+def test_rows_that_see_nothing(dtype, hd, rows, wide):
     """kv_len below the row count: the first rows stand before the sequence."""
     dev = torch.device("cuda", 0)
-    rows, lens = [5, 3, 150, 200], [2, 0, 70, 1]
-    c = ref.Cache(lens, 2, hd, 16, dtype, dev)
+    lens = [2, 0, 30, 1]
+    c = ref.Cache(lens, 2, hd, 16, dtype, dev, wide=wide)
     q = make_q(sum(rows), 4, hd, dtype, dev)
     got, lse = run(c, q, rows)
     agree(c, q, rows, got, lse)
@@ -122,12 +127,13 @@ def test_rows_that_see_nothing(dtype, hd):
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("rows,window", [(6, 0), (6, 40), (160, 0), (300, 90)])
-def test_what_is_masked_does_not_matter(dtype, hd, rows, window):
+@pytest.mark.parametrize("wide", [0, 100])
+def test_what_is_masked_does_not_matter(dtype, hd, rows, window, wide):
     """NaN and infinities in later tokens, in tokens behind the window, in
     unused slots: only rows that see them change."""
     dev = torch.device("cuda", 0)
     n = rows + 300
-    c = ref.Cache([n], 2, hd, 16, dtype, dev, seed=rows)
+    c = ref.Cache([n], 2, hd, 16, dtype, dev, seed=rows, wide=wide)
     q = make_q(rows, 4, hd, dtype, dev)
 
     def token(t):
