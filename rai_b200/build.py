@@ -8,6 +8,7 @@ include/rai_gpu.h.
 """
 from __future__ import annotations
 
+import concurrent.futures
 import hashlib
 import os
 import subprocess
@@ -83,16 +84,19 @@ def build(force: bool = False, verbose: bool = False) -> str:
         with open(stamp) as fh:
             if fh.read().strip() == digest:
                 return LIB
-    objs = []
     bdir = os.path.join(HERE, "_build")
     os.makedirs(bdir, exist_ok=True)
-    for src in SOURCES:
+
+    def compile_one(src: str) -> str:
         obj = os.path.join(bdir, os.path.splitext(src)[0] + ".o")
         cmd = [NVCC, *FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
         subprocess.run(cmd, check=True)
-        objs.append(obj)
+        return obj
+
+    with concurrent.futures.ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+        objs = list(pool.map(compile_one, SOURCES))
     tmp = LIB + ".tmp"
     subprocess.run([NVCC, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", tmp, *objs,
                     "-Xcompiler", "-fPIC"], check=True)

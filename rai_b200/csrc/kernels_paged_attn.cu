@@ -96,22 +96,18 @@ struct Cfg {
   static constexpr int DT = DT_, HD = HD_, MT = MT_;
   static constexpr int kElt = DT == kF32 ? 4 : 2;
   static constexpr int kRowB = HD * kElt;
-  static constexpr int NT = DT == kF32 && HD >= 128 ? 32 : 64;
+  static constexpr int NT = DT == kF32 ? (HD >= 128 ? 32 : 64) : HD == 64 ? 128 : 64;
   static constexpr int kTileB = NT * kRowB;
-  static constexpr int kStages = HD == 256 ? 2 : HD == 128 ? 3 : 4;
+  static constexpr int kStages = HD == 256 ? 2 : 3;
   static constexpr int WM = MT / 16, WN = 4 / WM, NTW = NT / WN;
   static constexpr bool kQReg = DT != kF32 && HD <= 128;  // query fragments stay in registers
   static constexpr int kQB = kQReg ? 0 : MT * kRowB;
   static constexpr int kMergeB = WN > 1 ? 2 * 16 * (HD + 4) * 4 + 4 * 16 * 8 : 0;
-  static constexpr int kSmem = kStages * 2 * kTileB + kQB + kMergeB + 128;
+  static constexpr int kBlocks = kRowB / 128;  // 128-byte column blocks
+  static constexpr int kSmem = kStages * 2 * kTileB + kQB + kMergeB + 1024;
   static constexpr int kPartFloats = MT * (HD + 2);
   static constexpr float kPShift = DT == kF16 ? 10.f : 0.f;
 };
-
-template <typename C>
-__device__ __forceinline__ uint32_t swz(int row, int chunk) {  // 16-byte chunk of a row, conflict free by rows of 8
-  return (uint32_t)row * C::kRowB + (uint32_t)((chunk ^ (row & 7)) << 4);
-}
 
 // K and V of the cursor's tile, from pages looked up a tile ahead. Each lane
 // knows the offsets of NT / 32 tokens; a token's copies get its offset by a
@@ -150,7 +146,7 @@ __device__ __forceinline__ void load_tile(const Params& p, const Cursor<C::MT, C
       }
 #pragma unroll
       for (int i = 0; i < kB; ++i)
-        cp_async16_or_zero((kv ? sv : sk) + swz<C>(r0 + (i0 + i) * kRowsPer, chunk), o[i] >= 0 ? base + o[i] * C::kElt : base, o[i] >= 0);
+        cp_async16_or_zero((kv ? sv : sk) + tile_at(C::NT, r0 + (i0 + i) * kRowsPer, chunk), o[i] >= 0 ? base + o[i] * C::kElt : base, o[i] >= 0);
     }
   }
 }
@@ -208,12 +204,14 @@ __device__ __forceinline__ float lds_f32(uint32_t a) {
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
   return v;
 }
-template <typename C>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_constant__ Params p) {
+template <typename C, bool TMA>
+__global__ void __launch_bounds__(kThreads)
+    paged_attn_kernel(const __grid_constant__ Params p, const __grid_constant__ KvMaps maps, int box) {
   constexpr int DT = C::DT, HD = C::HD, MT = C::MT, NT = C::NT, WN = C::WN, NTW = C::NTW, S = C::kStages;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   __shared__ long long sh[kPlanWords];
-  const uint32_t base = (smem_u32(smem_raw) + 127) & ~127u;
+  __shared__ uint64_t full[S], empty[S];  // TMA: a stage has landed, every warp is done with it
+  const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
   const uint32_t sq = base + S * 2 * C::kTileB;
   float* merge = reinterpret_cast<float*>(smem_raw + (sq + C::kQB - smem_u32(smem_raw)));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -221,9 +219,16 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
   const int g = lane >> 2, t4 = lane & 3;
   const PagedChunk& ch = p.a.c;
 
+  if (TMA && threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kThreads / 32);
+    }
+    fence_barrier_init();
+  }
   pdl_wait_prior();
   pdl_launch_dependents();
-  const Range rg = plan<MT, NT, kThreads>(p, blockIdx.x, sh);
+  const Range rg = plan<MT, NT, kThreads>(p, blockIdx.x, sh);  // (with barriers of the CTA)
   const long long begin = rg.begin, end = rg.end;
   if (begin >= end) {
     if (threadIdx.x == 0 && !p.whole) reinterpret_cast<Cut*>(p.a.part)[blockIdx.x] = Cut{};
@@ -236,16 +241,33 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
   if (threadIdx.x == 0 && !p.whole) leave_cut<MT, NT>(p, rg, cur, blockIdx.x);
   uint32_t loaded = 0, done = 0;  // tiles
   TilePages<NT> pages;
-  pages.fetch(ch, ld.it, (ld.it.first + ld.tile) * NT, lane);
-#pragma unroll
-  for (int s = 0; s < S - 1; ++s) {
-    if (ld.pos < end) {
-      load_tile<C>(p, ld, pages, base + s * 2 * C::kTileB, base + s * 2 * C::kTileB + C::kTileB);
-      ++loaded;
-      ld.next(p);
-      if (ld.pos < end) pages.fetch(ch, ld.it, (ld.it.first + ld.tile) * NT, lane);
+  TilePieces<NT, C::kBlocks, C::kElt> pieces;
+  // The next tile of K and V (TMA: by warp 0 alone).
+  auto fetch = [&] {
+    if (ld.pos >= end) return;
+    if constexpr (TMA) pieces.fetch(ch, ld.it, (ld.it.first + ld.tile) * NT, box, lane);
+    else pages.fetch(ch, ld.it, (ld.it.first + ld.tile) * NT, lane);
+  };
+  auto load = [&] {
+    const uint32_t i = loaded % S, st = base + i * 2 * C::kTileB;
+    if constexpr (TMA) {
+      const int t0 = (ld.it.first + ld.tile) * NT;
+      pieces.load2(ch, ld.it, t0, box, lane, &maps.k, &maps.v, ld.head, st, st + C::kTileB, &full[i]);
+    } else {
+      load_tile<C>(p, ld, pages, st, st + C::kTileB);
     }
-    cp_async_commit();
+    ++loaded;
+    ld.next(p);
+    fetch();
+  };
+  bool ok = true;
+  if (!TMA || warp == 0) {
+    fetch();
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) {
+      if (ld.pos < end) load();
+      if (!TMA) cp_async_commit();
+    }
   }
 
   uint32_t qf[C::kQReg ? HD / 16 : 1][4];
@@ -290,10 +312,11 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
           const long long o = (long long)(it.start + i) * p.a.q_row + (long long)(cur.head * p.a.group + j) * p.a.q_head;
           uint4 w = make_uint4(0, 0, 0, 0);
           if (real) w = *reinterpret_cast<const uint4*>(static_cast<const char*>(q) + o * C::kElt + chunk * 16);
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(sq + swz<C>(r, chunk)), "r"(w.x), "r"(w.y),
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(sq + tile_at(MT, r, chunk)), "r"(w.x), "r"(w.y),
                        "r"(w.z), "r"(w.w)
                        : "memory");
         }
+        __syncthreads();
       }
 #pragma unroll
       for (int x = 0; x < HD / 8; ++x)
@@ -302,17 +325,21 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
       poison = false;
       fresh = false;
     }
-    cp_async_wait<S - 2>();
-    __syncthreads();
-    // The stage that the last step read is free: fetch ahead.
-    if (ld.pos < end) {
-      const uint32_t st = base + (loaded % S) * 2 * C::kTileB;
-      load_tile<C>(p, ld, pages, st, st + C::kTileB);
-      ++loaded;
-      ld.next(p);
-      if (ld.pos < end) pages.fetch(ch, ld.it, (ld.it.first + ld.tile) * NT, lane);
+    if constexpr (TMA) {
+      if (warp == 0 && ld.pos < end) {
+        // The stage of the last tile is free once every warp is done with it.
+        if (done > 0) ok = __all_sync(~0u, wait_bar(&empty[(done - 1) % S], (done - 1) / S & 1, ch.err));
+        if (ok) load();
+      }
+      ok = __all_sync(~0u, ok && wait_bar(&full[done % S], done / S & 1, ch.err));
+      if (!ok) break;
+    } else {
+      cp_async_wait<S - 2>();
+      __syncthreads();
+      // The stage that the last step read is free: fetch ahead.
+      if (ld.pos < end) load();
+      cp_async_commit();
     }
-    cp_async_commit();
     const uint32_t sk = base + (done % S) * 2 * C::kTileB, sv = sk + C::kTileB;
     const int t0 = (it.first + cur.tile) * NT;
     const int p0 = it.len - it.n;
@@ -336,6 +363,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
         }
       }
       if (__syncthreads_or(bad)) poison = true;
+      if (TMA) fence_async();  // the stage is TMA's again after this
     }
 
     // ---- S = Q K^T over this warp's tokens ----
@@ -353,27 +381,32 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
 #pragma unroll
           for (int e = 0; e < 4; ++e) a[e] = qf[kk][e];
         } else {
-          ldsm4(a, sq + swz<C>(wm * 16 + (lane & 15), kk * 2 + (lane >> 4)));
+          ldsm4(a, sq + tile_at(MT, wm * 16 + (lane & 15), kk * 2 + (lane >> 4)));
         }
 #pragma unroll
         for (int x = 0; x < NTW / 16; ++x) {
           uint32_t b[4];
-          ldsm4(b, sk + swz<C>(w0 + x * 16 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
+          ldsm4(b, sk + tile_at(NT, w0 + x * 16 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
           mma16<DT>(s[2 * x], a, b[0], b[1]);
           mma16<DT>(s[2 * x + 1], a, b[2], b[3]);
         }
       }
     } else {
+      // The tensor core truncates as it adds, so each step's products get an
+      // accumulator of their own and join the sum rounded to nearest.
 #pragma unroll 4
       for (int kk = 0; kk < HD / 8; ++kk) {
         uint32_t ah[4], al[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          split(lds_f32(sq + swz<C>(wm * 16 + g + 8 * (e & 1), kk * 2 + (e >> 1)) + 4 * t4), ah[e], al[e]);
+          split(lds_f32(sq + tile_at(MT, wm * 16 + g + 8 * (e & 1), kk * 2 + (e >> 1)) + 4 * t4), ah[e], al[e]);
 #pragma unroll
         for (int x = 0; x < NTW / 8; ++x) {
           const int tk = w0 + x * 8 + g;
-          mma8x3(s[x], ah, al, lds_f32(sk + swz<C>(tk, kk * 2) + 4 * t4), lds_f32(sk + swz<C>(tk, kk * 2 + 1) + 4 * t4));
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          mma8x3(d, ah, al, lds_f32(sk + tile_at(NT, tk, kk * 2) + 4 * t4), lds_f32(sk + tile_at(NT, tk, kk * 2 + 1) + 4 * t4));
+#pragma unroll
+          for (int y = 0; y < 4; ++y) s[x][y] += d[y];
         }
       }
     }
@@ -428,27 +461,38 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
 #pragma unroll
         for (int x = 0; x < HD / 16; ++x) {
           uint32_t b[4];
-          ldsm4t(b, sv + swz<C>(w0 + kk * 16 + (lane & 15), x * 2 + (lane >> 4)));
+          ldsm4t(b, sv + tile_at(NT, w0 + kk * 16 + (lane & 15), x * 2 + (lane >> 4)));
           mma16<DT>(acc[2 * x], a, b[0], b[1]);
           mma16<DT>(acc[2 * x + 1], a, b[2], b[3]);
         }
       }
     } else {
+      // Column k of A is token 2k (k < 4) or 2 (k - 4) + 1, as the scores lie.
+      uint32_t ah[NTW / 8][4], al[NTW / 8][4];
 #pragma unroll
       for (int kk = 0; kk < NTW / 8; ++kk) {
-        // Column k of A is token 2k (k < 4) or 2 (k - 4) + 1, as the scores lie.
-        uint32_t ah[4], al[4];
-        split(s[kk][0], ah[0], al[0]);
-        split(s[kk][2], ah[1], al[1]);
-        split(s[kk][1], ah[2], al[2]);
-        split(s[kk][3], ah[3], al[3]);
-        const int tk = w0 + kk * 8 + 2 * t4;
-#pragma unroll
-        for (int x = 0; x < HD / 8; ++x) {
-          const int chunk = x * 2 + (g >> 2), off = 4 * (g & 3);
-          mma8x3(acc[x], ah, al, lds_f32(sv + swz<C>(tk, chunk) + off), lds_f32(sv + swz<C>(tk + 1, chunk) + off));
-        }
+        split(s[kk][0], ah[kk][0], al[kk][0]);
+        split(s[kk][2], ah[kk][1], al[kk][1]);
+        split(s[kk][1], ah[kk][2], al[kk][2]);
+        split(s[kk][3], ah[kk][3], al[kk][3]);
       }
+#pragma unroll
+      for (int x = 0; x < HD / 8; ++x) {
+        const int chunk = x * 2 + (g >> 2), off = 4 * (g & 3);
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < NTW / 8; ++kk) {
+          const int tk = w0 + kk * 8 + 2 * t4;
+          mma8x3(d, ah[kk], al[kk], lds_f32(sv + tile_at(NT, tk, chunk) + off), lds_f32(sv + tile_at(NT, tk + 1, chunk) + off));
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) acc[x][y] += d[y];
+      }
+    }
+
+    if constexpr (TMA) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[done % S]);
     }
 
     // ---- end of the item, or of this CTA's part of it ----
@@ -579,7 +623,13 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
     }
     cur.next(p);
   }
-  cp_async_wait<0>();
+  if constexpr (TMA) {
+    // After a timeout: what was requested lands before the CTA ends.
+    if (warp == 0 && !ok)
+      for (uint32_t i = done; i < loaded; ++i) wait_bar(&full[i % S], i / S & 1, nullptr);
+  } else {
+    cp_async_wait<0>();
+  }
 }
 
 template <typename C>
@@ -613,8 +663,8 @@ bool whole_items(const AttnArgs& a) {
   return ((long long)a.c.max_pages * a.c.page.d + C::NT - 1) / C::NT <= kWholeTiles;
 }
 
-template <typename C>
-cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
+template <typename C, bool TMA>
+cudaError_t launch_main(const Params& p, const KvMaps& maps, int box, cudaStream_t s) {
   static std::once_flag once[64];
   static cudaError_t ready[64];
   int dev = 0;
@@ -622,9 +672,14 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   std::call_once(once[dev], [&] {
-    ready[dev] = cudaFuncSetAttribute(paged_attn_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    ready[dev] = cudaFuncSetAttribute(paged_attn_kernel<C, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   });
   if (ready[dev] != cudaSuccess) return ready[dev];
+  return launch_pdl(paged_attn_kernel<C, TMA>, dim3(p.grid), dim3(kThreads), C::kSmem, s, p, maps, box);
+}
+
+template <typename C>
+cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
   Params p;
   p.a = a;
   const long long frows = (long long)a.c.max_rows * a.group;
@@ -636,7 +691,10 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
   p.item_cost = kItemCost;
   p.grid = device_sm_count() * resident_ctas<C>();
   p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
-  e = launch_pdl(paged_attn_kernel<C>, dim3(p.grid), dim3(kThreads), C::kSmem, s, p);
+  KvMaps maps;
+  const int box = tma_box((int)a.c.page.d, C::NT);
+  const bool tma = box && make_maps(a.c, a.dtype, box, &maps);
+  cudaError_t e = tma ? launch_main<C, true>(p, maps, box, s) : launch_main<C, false>(p, maps, box, s);
   if (e != cudaSuccess || p.whole) return e;
   return launch_pdl(paged_combine_kernel<C>, dim3(p.grid - 1, combine_grid_y(C::MT)), dim3(kCombineThreads), 0, s, p);
 }

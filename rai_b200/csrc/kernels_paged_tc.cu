@@ -70,9 +70,9 @@ struct Tc {
 };
 
 constexpr float kLazy = 8.f;  // log2 units
-// Few rows: from how many tokens a sequence can have this kernel is the faster
-// one.
-constexpr long long kTcFewRowsTokens = 1024;
+// Few rows and heads wider than 64: from how many tokens a sequence can have
+// this kernel is the faster one.
+constexpr long long kTcFewRowsTokens = 1536;
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -125,36 +125,6 @@ __device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* v) {
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ bool try_bar(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Bounded wait (about a second of SM clock), polling: a wait with a suspend
-// hint wakes late.
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, uint32_t* err) {
-  const uint32_t a = smem_u32(bar);
-  if (try_bar(a, parity)) return true;
-  const long long t0 = clock64();
-  while (!try_bar(a, parity))
-    if (clock64() - t0 > 2000000000ll) {
-      if (err) atomicOr(err, kErrWaitTimeout);
-      return false;
-    }
-  return true;
-}
-
-// Whether some row of the item may not see some token of the tile that
-// begins at t0.
-__device__ __forceinline__ bool tile_masked(const Item& it, int t0, int nt, int window, const FastDiv& group) {
-  const int p0 = it.len - it.n, plo = p0 + (int)group.quot(it.f0), phi = it.hi - 1;
-  return t0 + nt - 1 > plo || t0 < it.lo || (window > 0 && t0 <= phi - window);
-}
-
 // Replaces the values of this thread's chunks of a V tile that are not finite
 // by zero; whether there were any.
 template <typename C>
@@ -201,7 +171,6 @@ __device__ __forceinline__ void load_queries(const Params& p, const Item& it, in
   }
   cp_async_commit();
 }
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 constexpr int kLanded = 8;  // V tiles between their landing and their hand-over
 
@@ -815,7 +784,7 @@ cudaError_t choose(const AttnArgs& a, cudaStream_t s) {
 bool paged_attention_tc_takes(const AttnArgs& a) {
   if (a.dtype == kF32 || a.c.hd > 128) return false;
   if ((long long)a.c.max_rows * a.group > 64) return true;
-  return tma_box((int)a.c.page.d, 128) && (long long)a.c.max_pages * a.c.page.d >= kTcFewRowsTokens;
+  return a.c.hd > 64 && tma_box((int)a.c.page.d, 128) && (long long)a.c.max_pages * a.c.page.d >= kTcFewRowsTokens;
 }
 
 size_t paged_attention_tc_workspace(const AttnArgs& a) {

@@ -198,6 +198,38 @@ __device__ __forceinline__ uint32_t tile_at(int rows, int row, int chunk) {
   return (uint32_t)((chunk >> 3) * rows * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
 }
 
+__device__ __forceinline__ bool try_bar(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded wait (about a second of SM clock), polling: a wait with a suspend
+// hint wakes late.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, uint32_t* err) {
+  const uint32_t a = smem_u32(bar);
+  if (try_bar(a, parity)) return true;
+  const long long t0 = clock64();
+  while (!try_bar(a, parity))
+    if (clock64() - t0 > 2000000000ll) {
+      if (err) atomicOr(err, kErrWaitTimeout);
+      return false;
+    }
+  return true;
+}
+
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Whether some row of the item may not see some token of the tile that
+// begins at t0.
+__device__ __forceinline__ bool tile_masked(const Item& it, int t0, int nt, int window, const FastDiv& group) {
+  const int p0 = it.len - it.n, plo = p0 + (int)group.quot(it.f0), phi = it.hi - 1;
+  return t0 + nt - 1 > plo || t0 < it.lo || (window > 0 && t0 <= phi - window);
+}
+
 // Pages as TMA tensors (element, slot, head, page). A tile of NT tokens is
 // fetched in pieces of `box` slots of one page by one 128-byte column block,
 // one copy per lane of a warp: pages of 8 x 2^i slots, or of whole tiles.
@@ -243,22 +275,33 @@ struct TilePieces {
   // the pool is reported and its slots are zeros.
   __device__ __forceinline__ void load(const PagedChunk& c, const Item& it, int t0, int box, int lane, const CUtensorMap* map,
                                        int head, uint32_t dst, uint64_t* bar) const {
+    load2(c, it, t0, box, lane, map, nullptr, head, dst, 0, bar);
+  }
+  // With map2: both, K into dst and V into dst2, on one barrier.
+  __device__ __forceinline__ void load2(const PagedChunk& c, const Item& it, int t0, int box, int lane, const CUtensorMap* map,
+                                        const CUtensorMap* map2, int head, uint32_t dst, uint32_t dst2, uint64_t* bar) const {
     int block, piece;
     const bool any = mine(box, lane, &block, &piece);
     const int t = t0 + piece * box;
     const bool want = any && t < it.hi && t + box > it.lo;
     const bool good = want && (unsigned)page < (unsigned)c.n_pages;
-    const uint32_t at = dst + block * (NT * 128) + piece * box * 128;
+    const uint32_t at = block * (NT * 128) + piece * box * 128;
     if (want && !good) {
       atomicOr(c.err, kErrBadInput);
-      for (int i = 0; i < box * 8; ++i)
-        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at + i * 16), "r"(0) : "memory");
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      for (int i = 0; i < box * 8; ++i) {
+        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(dst + at + i * 16), "r"(0) : "memory");
+        if (map2) asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(dst2 + at + i * 16), "r"(0) : "memory");
+      }
+      fence_async();
     }
     const uint32_t n = __popc(__ballot_sync(~0u, good));
-    if (lane == 0) mbar_arrive_expect_tx(bar, n * box * 128);
+    if (lane == 0) mbar_arrive_expect_tx(bar, (map2 ? 2 : 1) * n * box * 128);
     __syncwarp();
-    if (good) tma_load(at, map, block * (128 / ELT), t - (int)c.page.quot(t) * (int)c.page.d, head, page, bar);
+    if (good) {
+      const int slot = t - (int)c.page.quot(t) * (int)c.page.d;
+      tma_load(dst + at, map, block * (128 / ELT), slot, head, page, bar);
+      if (map2) tma_load(dst2 + at, map2, block * (128 / ELT), slot, head, page, bar);
+    }
   }
 };
 
