@@ -350,18 +350,7 @@ __global__ void __launch_bounds__(kThreads)
       // V values that are not finite, where a row may not see them.
       bool bad = false;
 #pragma unroll 4
-      for (int x = threadIdx.x; x < C::kTileB / 16; x += kThreads) {
-        const uint32_t ad = sv + x * 16;
-        uint4 w;
-        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(ad));
-        const uint4 f = make_uint4(finite_or_zero<DT>(w.x), finite_or_zero<DT>(w.y), finite_or_zero<DT>(w.z),
-                                   finite_or_zero<DT>(w.w));
-        if (f.x != w.x || f.y != w.y || f.z != w.z || f.w != w.w) {
-          bad = true;
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(ad), "r"(f.x), "r"(f.y), "r"(f.z), "r"(f.w)
-                       : "memory");
-        }
-      }
+      for (int x = threadIdx.x; x < C::kTileB / 16; x += kThreads) bad |= clean_chunk<DT>(sv + x * 16, t0 + x / 8 % NT, it);
       if (__syncthreads_or(bad)) poison = true;
       if (TMA) fence_async();  // the stage is TMA's again after this
     }

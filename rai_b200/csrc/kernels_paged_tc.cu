@@ -125,24 +125,16 @@ __device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* v) {
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Replaces the values of this thread's chunks of a V tile that are not finite
-// by zero; whether there were any.
+// clean_chunk() of this thread's share of the V tile that begins at token t0.
 template <typename C>
-__device__ __forceinline__ bool look_through(uint32_t base, int tid) {
+__device__ __forceinline__ bool look_through(uint32_t base, int t0, const Item& it, int tid) {
   constexpr int kChunks = C::HD / 8, kRowsPer = kProducers / kChunks;
   const int chunk = tid % kChunks, r0 = tid / kChunks;
   bool bad = false;
 #pragma unroll 4
   for (int i = 0; i < C::NT / kRowsPer; ++i) {
-    const uint32_t ad = base + tile_at(C::NT, r0 + i * kRowsPer, chunk);
-    uint4 w;
-    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(ad));
-    const uint4 f = make_uint4(finite_or_zero<C::DT>(w.x), finite_or_zero<C::DT>(w.y), finite_or_zero<C::DT>(w.z),
-                               finite_or_zero<C::DT>(w.w));
-    if (f.x != w.x || f.y != w.y || f.z != w.z || f.w != w.w) {
-      bad = true;
-      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(ad), "r"(f.x), "r"(f.y), "r"(f.z), "r"(f.w) : "memory");
-    }
+    const int row = r0 + i * kRowsPer;
+    bad |= clean_chunk<C::DT>(base + tile_at(C::NT, row, chunk), t0 + row, it);
   }
   return bad;
 }
@@ -307,8 +299,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (!__all_sync(~0u, wait_bar(&landed[k % kLanded], k / kLanded & 1, err))) break;
         const uint32_t slot = (2 * k + 1) % C::kSlots;
-        if (tile_masked(it, (it.first + cur.tile) * NT, NT, p.a.window, p.group_div)) {
-          if (look_through<C>(skv + slot * C::kTileB, tid)) *(volatile int*)&poison[items & 3] = items + 1;
+        const int t0 = (it.first + cur.tile) * NT;
+        if (tile_masked(it, t0, NT, p.a.window, p.group_div)) {
+          if (look_through<C>(skv + slot * C::kTileB, t0, it, tid)) *(volatile int*)&poison[items & 3] = items + 1;
           fence_async();
           asm volatile("bar.sync 1, 64;" ::: "memory");
         }
@@ -335,9 +328,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       uint32_t n = 0, handed = 0;  // K and V tiles fetched, handed over
       bool ok = true, fresh = true;
       uint32_t look = 0;  // bit i: fetch n - 1 - i is a V tile to look through
+      Item seen = cur.it;  // the item of the fetches in flight
+      int look_t0[2] = {0, 0};  // first tokens of the V tiles in flight
       auto hand = [&](int age) {  // the fetch `handed` has landed
         const uint32_t slot = handed % C::kSlots;
-        if ((look >> age & 1u) && look_through<C>(skv + slot * C::kTileB, tid)) *(volatile int*)&poison[items & 3] = items + 1;
+        if ((look >> age & 1u) && look_through<C>(skv + slot * C::kTileB, handed / 2 & 1 ? look_t0[1] : look_t0[0], seen, tid))
+          *(volatile int*)&poison[items & 3] = items + 1;
         fence_async();
         mbar_arrive(&kv_full[slot]);
         ++handed;
@@ -355,6 +351,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (!ok) break;
           }
           first = false;
+          seen = cur.it;
           load_queries<C, kProducers>(p, cur.it, cur.head, sq, tid);
           cp_async_wait<0>();
           fence_async();
@@ -391,6 +388,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           cp_async_commit();
           if (kv == 0 && tid == 0) flags[slot] = flags_of<MT, NT>(p, cur, end);
+          if (kv) (n / 2 & 1 ? look_t0[1] : look_t0[0]) = t0;
           look = look << 1 | (kv && tile_masked(it, t0, NT, p.a.window, p.group_div) ? 1u : 0u);
           ++n;
           if (n - handed > (uint32_t)kLag) {

@@ -201,9 +201,9 @@ __device__ __forceinline__ uint32_t tile_at(int rows, int row, int chunk) {
 __device__ __forceinline__ bool try_bar(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
       : "=r"(ok)
-      : "r"(bar), "r"(parity)
+      : "r"(bar), "r"(parity), "r"(500u)  // ns
       : "memory");
   return ok != 0;
 }
@@ -228,6 +228,32 @@ __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.
 __device__ __forceinline__ bool tile_masked(const Item& it, int t0, int nt, int window, const FastDiv& group) {
   const int p0 = it.len - it.n, plo = p0 + (int)group.quot(it.f0), phi = it.hi - 1;
   return t0 + nt - 1 > plo || t0 < it.lo || (window > 0 && t0 <= phi - window);
+}
+
+// The elements of a 32-bit word that are not finite, replaced by zero.
+template <int DT>
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
+  if constexpr (DT == kF32) {
+    return (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
+  } else {
+    constexpr uint32_t e = DT == kBF16 ? 0x7f80u : 0x7c00u;
+    if ((w & e) == e) w &= 0xffff0000u;
+    if ((w >> 16 & e) == e) w &= 0x0000ffffu;
+    return w;
+  }
+}
+
+// Replaces the values of one 16-byte chunk of a V tile that are not finite by
+// zero; whether there were any in a token that some row sees (t: the chunk's
+// token). Slots outside that range may hold anything.
+template <int DT>
+__device__ __forceinline__ bool clean_chunk(uint32_t ad, int t, const Item& it) {
+  uint4 w;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(ad));
+  const uint4 f = make_uint4(finite_or_zero<DT>(w.x), finite_or_zero<DT>(w.y), finite_or_zero<DT>(w.z), finite_or_zero<DT>(w.w));
+  if (f.x == w.x && f.y == w.y && f.z == w.z && f.w == w.w) return false;
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(ad), "r"(f.x), "r"(f.y), "r"(f.z), "r"(f.w) : "memory");
+  return t >= it.lo && t < it.hi;
 }
 
 // Pages as TMA tensors (element, slot, head, page). A tile of NT tokens is
@@ -341,19 +367,6 @@ __device__ __forceinline__ float capped(float s, float scale, float cap) {
     return cap * (1.f - __fdividef(2.f, 1.f + exp2_fast(2.f * kLog2e * x)));
   }
 }
-// The elements of a 32-bit word that are not finite, replaced by zero.
-template <int DT>
-__device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
-  if constexpr (DT == kF32) {
-    return (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
-  } else {
-    constexpr uint32_t e = DT == kBF16 ? 0x7f80u : 0x7c00u;
-    if ((w & e) == e) w &= 0xffff0000u;
-    if ((w >> 16 & e) == e) w &= 0x0000ffffu;
-    return w;
-  }
-}
-
 // What a CTA of the main kernel leaves for the join: whether the cut at its
 // first tile is the first one through an item, and that item.
 struct Cut {
