@@ -22,7 +22,8 @@ namespace rai {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBufCap = 2 * kThreads * 8;  // most elements of a step, twice
+constexpr int kBufCap = 2048;  // candidates a slice holds between two sorts
+constexpr float kLog2e = 1.4426950408889634f;
 
 // A float's bits in the order of its value (-0 as +0).
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -37,8 +38,14 @@ __device__ __forceinline__ uint64_t key_of(float x, int token) {
 }
 
 // e^(x - m), where x = m also counts when both are infinite: a row with
-// infinite logits shares its mass among them, a row of -inf among all.
-__device__ __forceinline__ float weight(float x, float m) { return x == m ? 1.f : expf(x - m); }
+// infinite logits shares its mass among them, a row of -inf among all. (The
+// error of ex2.approx is the same function of x - m in every row: it all but
+// cancels between beams.)
+__device__ __forceinline__ float weight(float x, float m) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((x - m) * kLog2e));
+  return x == m ? 1.f : r;
+}
 
 template <int DT>
 __device__ __forceinline__ float to_f32(uint32_t w, int half) {
@@ -78,10 +85,10 @@ __device__ __forceinline__ void prune(uint64_t* buf, int n, int keep) {
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads) beam_slice_kernel(BeamArgs a, int slices, int len) {
+__global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(BeamArgs a, int slices, int len) {
   constexpr int V = DT == kF32 ? 4 : 8;  // elements of 16 bytes
-  constexpr int kU = 8 / V;              // vectors of a step
   constexpr int kE = DT == kF32 ? 4 : 2;
+  constexpr int N = 16, kVecs = N / V;   // elements and 16-byte loads of a thread in a step
   __shared__ uint64_t buf[kBufCap];
   __shared__ uint64_t tops[kThreads];
   __shared__ int count;
@@ -99,22 +106,31 @@ __global__ void __launch_bounds__(kThreads) beam_slice_kernel(BeamArgs a, int sl
   float m = -INFINITY;
   double sum = 0.0;
   uint64_t bar = 0;  // keys at or above it are kept
-  __syncthreads();
-  for (int at = base; at < end; at += kThreads * V * kU) {
-    float x[V * kU];
-    bool whole[kU];
+  auto first_of = [&](int at, int u) { return at + (u * kThreads + (int)threadIdx.x) * V; };
+  auto fetch = [&](int at, uint4 (&w)[kVecs]) {  // whole vectors only
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int e0 = at + (u * kThreads + threadIdx.x) * V;
-      whole[u] = e0 >= begin && e0 + V <= end;
-      if (whole[u]) {
-        const uint4 w = __ldcs(reinterpret_cast<const uint4*>(src + (long long)e0 * kE));
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    for (int u = 0; u < kVecs; ++u) {
+      const int e0 = first_of(at, u);
+      if (e0 >= begin && e0 + V <= end) w[u] = __ldcs(reinterpret_cast<const uint4*>(src + (long long)e0 * kE));
+    }
+  };
+  uint4 w[kVecs];
+  fetch(base, w);
+  __syncthreads();
+  for (int at = base; at < end; at += kThreads * N) {
+    float x[N];
+    uint32_t there = 0;  // bit per element
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const int e0 = first_of(at, u);
+      if (e0 >= begin && e0 + V <= end) {
+        const uint32_t ws[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           if constexpr (DT == kF32) x[u * V + i] = __uint_as_float(ws[i]);
           else x[u * V + i] = to_f32<DT>(ws[i / 2], i & 1);
         }
+        there |= ((1u << V) - 1u) << (u * V);
       } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -122,68 +138,89 @@ __global__ void __launch_bounds__(kThreads) beam_slice_kernel(BeamArgs a, int sl
           if (e0 + i >= begin && e0 + i < end) {
             if constexpr (DT == kF32) x[u * V + i] = reinterpret_cast<const float*>(src)[e0 + i];
             else x[u * V + i] = to_f32<DT>(reinterpret_cast<const uint16_t*>(src)[e0 + i], 0);
+            there |= 1u << (u * V + i);
           }
         }
       }
     }
+    if (at + kThreads * N < end) fetch(at + kThreads * N, w);  // in flight through this step
     float top = -INFINITY;
-    int there = 0;
-    uint64_t best = 0;
 #pragma unroll
-    for (int i = 0; i < V * kU; ++i) {
-      const int e = at + (i / V * kThreads + threadIdx.x) * V + i % V;
+    for (int i = 0; i < N; ++i) {
       if (!(x[i] == x[i])) x[i] = -INFINITY;  // a NaN is not chosen
-      if (e >= begin && e < end) {
-        top = fmaxf(top, x[i]);
-        ++there;
-      }
+      top = fmaxf(top, x[i]);                 // (elements that are not there are -inf)
     }
     if (there) {
       if (top > m) {
-        sum *= (double)expf(m - top);
+        sum *= (double)weight(m, top);
         m = top;
       }
-      float part = 0.f;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      if (there == (uint32_t)((1ull << N) - 1)) {
 #pragma unroll
-      for (int i = 0; i < V * kU; ++i) {
-        const int e = at + (i / V * kThreads + threadIdx.x) * V + i % V;
-        if (e >= begin && e < end) part += weight(x[i], m);
+        for (int i = 0; i < N; ++i) part[i & 3] += weight(x[i], m);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (there >> i & 1u) part[i & 3] += weight(x[i], m);
       }
-      sum += (double)part;
+      sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
     }
     if (at == base) {
       // The keep-th largest of the threads' best is no larger than the
       // keep-th largest element: a first bar.
+      uint64_t best = 0;
 #pragma unroll
-      for (int i = 0; i < V * kU; ++i) {
-        const int e = at + (i / V * kThreads + threadIdx.x) * V + i % V;
-        if (e >= begin && e < end) best = max(best, key_of(x[i], e));
-      }
+      for (int i = 0; i < N; ++i)
+        if ((there >> i & 1u) && x[i] == top) best = max(best, key_of(x[i], first_of(at, i / V) + i % V));
       tops[threadIdx.x] = best;
       bitonic(tops, kThreads);
       bar = tops[a.keep - 1];
     }
-    const float bar_x = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
-    if (there && top >= bar_x) {
+    // Elements at or above the bar go to the buffer; whenever it fills up it
+    // is cut to the keep best, which raises the bar.
+    uint32_t pending = 0;
+    {
+      const float bar_x = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
+      if (there && top >= bar_x) {
 #pragma unroll
-      for (int i = 0; i < V * kU; ++i) {
-        const int e = at + (i / V * kThreads + threadIdx.x) * V + i % V;
-        if (e >= begin && e < end && x[i] >= bar_x) {
-          const uint64_t k = key_of(x[i], e);
-          if (k >= bar) buf[atomicAdd(&count, 1)] = k;
-        }
+        for (int i = 0; i < N; ++i)
+          if ((there >> i & 1u) && x[i] >= bar_x) pending |= 1u << i;
       }
     }
-    __syncthreads();
-    const int n = count;
-    if (n > kBufCap - kThreads * V * kU || n > 4 * a.keep + 64) {
-      prune(buf, n, a.keep);
-      bar = buf[a.keep - 1];
-      if (threadIdx.x == 0) count = min(n, a.keep);
+    for (;;) {
+      const uint64_t lowest = bar;
+      if (pending) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (pending >> i & 1u) {
+            const uint64_t k = key_of(x[i], first_of(at, i / V) + i % V);
+            if (k < lowest) {
+              pending &= ~(1u << i);
+              continue;
+            }
+            const int slot = atomicAdd(&count, 1);
+            if (slot < kBufCap) {
+              buf[slot] = k;
+              pending &= ~(1u << i);
+            }
+          }
+      }
+      const int again = __syncthreads_or(pending != 0);
+      const int n = min(count, kBufCap);
+      __syncthreads();  // everyone has read the count
+      if (again || n > 4 * a.keep + 192) {
+        prune(buf, n, a.keep);
+        bar = buf[min(n, a.keep) - 1];
+        if (n < a.keep) bar = 0;
+        if (threadIdx.x == 0) count = min(n, a.keep);
+        __syncthreads();
+      }
+      if (!again) break;
     }
-    __syncthreads();
   }
-  const int n = count;
+  __syncthreads();
+  const int n = min(count, kBufCap);
   prune(buf, n, a.keep);
   // Join the threads' sums.
   float top = m;
@@ -192,7 +229,7 @@ __global__ void __launch_bounds__(kThreads) beam_slice_kernel(BeamArgs a, int sl
   if ((threadIdx.x & 31) == 0) wm[threadIdx.x >> 5] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) top = fmaxf(top, wm[w]);
+  for (int i = 0; i < kThreads / 32; ++i) top = fmaxf(top, wm[i]);
   double s = sum == 0.0 ? 0.0 : sum * (double)weight(m, top);
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
@@ -201,97 +238,114 @@ __global__ void __launch_bounds__(kThreads) beam_slice_kernel(BeamArgs a, int sl
   char* out = static_cast<char*>(a.ws) + ((long long)row * slices + slice) * slice_bytes(a.keep);
   if (threadIdx.x == 0) {
     Slice r = {top, 0, 0.0};
-    for (int w = 0; w < kThreads / 32; ++w) r.sum += wsum[w];
+    for (int i = 0; i < kThreads / 32; ++i) r.sum += wsum[i];
     *reinterpret_cast<Slice*>(out) = r;
   }
   for (int i = threadIdx.x; i < a.keep; i += kThreads)
     reinterpret_cast<uint64_t*>(out + sizeof(Slice))[i] = i < n ? buf[i] : 0;
 }
 
-struct Cand {
-  double score;
-  float logit;
-  int flat;  // beam * vocab + token, -1: none
-};
-__device__ __forceinline__ bool before(const Cand& a, const Cand& b) {
-  if (a.flat < 0 || b.flat < 0) return b.flat < 0 && a.flat >= 0;
-  if (a.score != b.score) return a.score > b.score;
-  if (a.logit != b.logit) return a.logit > b.logit;
-  return a.flat < b.flat;
-}
-__device__ __forceinline__ Cand shuffled(const Cand& c, int o) {
-  Cand r;
-  r.score = __shfl_xor_sync(~0u, c.score, o);
-  r.logit = __shfl_xor_sync(~0u, c.logit, o);
-  r.flat = __shfl_xor_sync(~0u, c.flat, o);
-  return r;
-}
-
 constexpr int kMaxSlices = 16;
 
+// A candidate's place in the order: its score's bits in order, then its
+// logit's, then its flat number (beam * vocab + token) the other way round.
+struct Cand {
+  uint64_t score = 0;  // 0: none
+  uint32_t logit = 0, flat = 0;
+};
+__device__ __forceinline__ uint64_t ordered(double x) {
+  const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
+  return b ^ ((b >> 63) ? ~0ull : 1ull << 63);
+}
+__device__ __forceinline__ double unordered(uint64_t o) {
+  return __longlong_as_double((long long)(o ^ ((o >> 63) ? 1ull << 63 : ~0ull)));
+}
+// The first of the warp's candidates, in every lane.
+__device__ __forceinline__ Cand first_of_warp(const Cand& c) {
+  Cand b;
+  const uint32_t hi = __reduce_max_sync(~0u, (uint32_t)(c.score >> 32));
+  bool in = (uint32_t)(c.score >> 32) == hi;
+  const uint32_t lo = __reduce_max_sync(~0u, in ? (uint32_t)c.score : 0u);
+  in = in && (uint32_t)c.score == lo;
+  b.score = (uint64_t)hi << 32 | lo;
+  b.logit = __reduce_max_sync(~0u, in ? c.logit : 0u);
+  in = in && c.logit == b.logit;
+  b.flat = __reduce_min_sync(~0u, in ? c.flat : 0xffffffffu);
+  return b;
+}
+
 // One CTA per request, one thread per (beam, slice) list; each round takes
-// the best of the lists' heads.
+// the best of the lists' heads. Bound by the rounds' latency.
 __global__ void __launch_bounds__(kMaxBeams * kMaxSlices) beam_merge_kernel(BeamArgs a, int slices) {
-  __shared__ double lse[kMaxBeams];  // log of the sum beside the maximum
-  __shared__ float tops[kMaxBeams];
-  __shared__ Cand warp_best[kMaxBeams * kMaxSlices / 32];
+  __shared__ double sums[kMaxBeams * kMaxSlices], lse[kMaxBeams];  // lse: log of the sum beside the maximum
+  __shared__ float tops[kMaxBeams * kMaxSlices];
+  __shared__ Cand warp_best[2][kMaxBeams * kMaxSlices / 32];
   __shared__ Cand chosen[kMaxKeep];
   __shared__ int next[kMaxBeams];
+  __shared__ uint64_t heads[4096];  // the lists, where they fit
   pdl_wait_prior();
   pdl_launch_dependents();
   const int req = blockIdx.x, lists = a.beams * slices, warps = blockDim.x >> 5;
   const size_t sb = slice_bytes(a.keep);
   const char* ws = static_cast<const char*>(a.ws) + (long long)req * lists * sb;
+  const bool real = (int)threadIdx.x < lists;
+  const int beam = threadIdx.x / slices;
+  const char* mine_at = ws + (long long)threadIdx.x * sb;
+  Slice s = {-INFINITY, 0, 0.0};
+  float score = 0.f;
+  if (real) {
+    s = *reinterpret_cast<const Slice*>(mine_at);
+    score = a.scores[req * a.beams + beam];
+    if (!(score == score)) score = -INFINITY;
+    tops[threadIdx.x] = s.max;
+  }
+  const bool fits = lists * a.keep <= 4096;
+  if (fits)
+    for (int i = threadIdx.x; i < lists * a.keep; i += blockDim.x)
+      heads[i] = reinterpret_cast<const uint64_t*>(ws + (long long)(i / a.keep) * sb + sizeof(Slice))[i % a.keep];
+  __syncthreads();
+  float top = -INFINITY;
+  if (real) {
+    for (int i = 0; i < slices; ++i) top = fmaxf(top, tops[beam * slices + i]);
+    sums[threadIdx.x] = s.sum * (s.max == top ? 1.0 : exp((double)s.max - (double)top));
+  }
+  __syncthreads();
   if (threadIdx.x < a.beams) {
-    const char* mine = ws + (long long)threadIdx.x * slices * sb;
-    float top = -INFINITY;
-    for (int i = 0; i < slices; ++i) top = fmaxf(top, reinterpret_cast<const Slice*>(mine + i * sb)->max);
     double sum = 0.0;
-    for (int i = 0; i < slices; ++i) {
-      const Slice s = *reinterpret_cast<const Slice*>(mine + i * sb);
-      sum += s.sum * (s.max == top ? 1.0 : exp((double)s.max - (double)top));
-    }
-    tops[threadIdx.x] = top;
+    for (int i = 0; i < slices; ++i) sum += sums[threadIdx.x * slices + i];
     lse[threadIdx.x] = log(sum);
   }
   __syncthreads();
-  const int beam = threadIdx.x / slices;
-  const bool real = (int)threadIdx.x < lists;
-  const uint64_t* list = reinterpret_cast<const uint64_t*>(ws + (long long)threadIdx.x * sb + sizeof(Slice));
-  float score = 0.f;
-  if (real) {
-    score = a.scores[req * a.beams + beam];
-    if (!(score == score)) score = -INFINITY;
-  }
+  const uint64_t* list = fits ? heads + threadIdx.x * a.keep : reinterpret_cast<const uint64_t*>(mine_at + sizeof(Slice));
   int at = 0;
   auto head = [&]() {
-    Cand c = {0.0, 0.f, -1};
+    Cand c;
+    c.flat = 0xffffffffu;
     if (!real || at >= a.keep) return c;
     const uint64_t k = list[at];
     if (!k) return c;
-    c.logit = unordered((uint32_t)(k >> 32));
-    c.flat = beam * a.vocab + (int)(0xffffffffu - (uint32_t)k);
-    const double d = c.logit == tops[beam] ? 0.0 : (double)c.logit - (double)tops[beam];
-    c.score = (double)score + (d - lse[beam]);
+    c.logit = (uint32_t)(k >> 32);
+    c.flat = (uint32_t)(beam * a.vocab) + (0xffffffffu - (uint32_t)k);
+    const float x = unordered(c.logit);
+    const double d = x == top ? 0.0 : (double)x - (double)top;
+    c.score = ordered((double)score + (d - lse[beam]));
     return c;
   };
   Cand mine = head();
   for (int r = 0; r < a.keep; ++r) {
-    Cand best = mine;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const Cand c = shuffled(best, o);
-      if (before(c, best)) best = c;
-    }
+    Cand best = first_of_warp(mine);
     if (warps > 1) {
-      if ((threadIdx.x & 31) == 0) warp_best[threadIdx.x >> 5] = best;
+      // Every warp reads all warps' best; two buffers, so one barrier a round.
+      const int lane = threadIdx.x & 31;
+      if (lane == 0) warp_best[r & 1][threadIdx.x >> 5] = best;
       __syncthreads();
-      for (int w = 0; w < warps; ++w)
-        if (before(warp_best[w], best)) best = warp_best[w];
-      __syncthreads();
+      Cand c;
+      c.flat = 0xffffffffu;
+      if (lane < warps) c = warp_best[r & 1][lane];
+      best = first_of_warp(c);
     }
     if (threadIdx.x == 0) chosen[r] = best;
-    if (best.flat >= 0 && best.flat == mine.flat) {
+    if (best.score && best.flat == mine.flat) {
       ++at;
       mine = head();
     }
@@ -300,26 +354,33 @@ __global__ void __launch_bounds__(kMaxBeams * kMaxSlices) beam_merge_kernel(Beam
   for (int r = threadIdx.x; r < a.keep; r += blockDim.x) {
     const Cand c = chosen[r];
     const long long o = (long long)req * a.keep + r;
-    const int b = c.flat < 0 ? -1 : c.flat / a.vocab;
-    a.cand_score[o] = c.flat < 0 ? -INFINITY : (float)c.score;
+    const int b = c.score ? (int)c.flat / a.vocab : -1;
+    a.cand_score[o] = c.score ? (float)unordered(c.score) : -INFINITY;
     a.cand_beam[o] = b;
-    a.cand_token[o] = c.flat < 0 ? -1 : c.flat - b * a.vocab;
+    a.cand_token[o] = c.score ? (int)c.flat - b * a.vocab : -1;
   }
-  if (threadIdx.x == 0) {
+  if (threadIdx.x < 32) {
+    // Candidates that do not end, in order.
     int n = 0;
-    for (int r = 0; r < a.keep && n < a.beams; ++r)
-      if (chosen[r].flat >= 0 && chosen[r].flat % a.vocab != a.eos) next[n++] = r;
-    for (; n < a.beams; ++n) next[n] = -1;
+    for (int r0 = 0; r0 < a.keep; r0 += 32) {
+      const int r = r0 + threadIdx.x;
+      const bool goes = r < a.keep && chosen[r].score && (int)chosen[r].flat % a.vocab != a.eos;
+      const uint32_t mask = __ballot_sync(~0u, goes);
+      const int place = n + __popc(mask & ((1u << threadIdx.x) - 1u));
+      if (goes && place < a.beams) next[place] = r;
+      n += __popc(mask);
+    }
+    for (int i = n + threadIdx.x; i < a.beams; i += 32) next[i] = -1;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < a.beams; i += blockDim.x) {
     const long long o = (long long)req * a.beams + i;
     const bool some = next[i] >= 0;
     const Cand c = some ? chosen[next[i]] : Cand{};
-    const int b = some ? c.flat / a.vocab : 0;
-    a.score[o] = some ? (float)c.score : -INFINITY;
+    const int b = some ? (int)c.flat / a.vocab : 0;
+    a.score[o] = some ? (float)unordered(c.score) : -INFINITY;
     a.parent[o] = some ? req * a.beams + b : -1;
-    a.token[o] = some ? c.flat - b * a.vocab : -1;
+    a.token[o] = some ? (int)c.flat - b * a.vocab : -1;
   }
   if (!a.history) return;
   for (int i = 0; i < a.beams; ++i) {
@@ -329,24 +390,25 @@ __global__ void __launch_bounds__(kMaxBeams * kMaxSlices) beam_merge_kernel(Beam
       continue;
     }
     const Cand c = chosen[next[i]];
-    const int b = c.flat / a.vocab;
+    const int b = (int)c.flat / a.vocab;
     const long long p = (long long)req * a.beams + b;
     int n = a.hist_len[p];
-    const bool fits = n >= 0 && n < a.hist_cap;
-    if (!fits) n = min(max(n, 0), a.hist_cap);
+    const bool ok = n >= 0 && n < a.hist_cap;
+    if (!ok) n = min(max(n, 0), a.hist_cap);
     for (int x = threadIdx.x; x < n; x += blockDim.x) a.out_history[o * a.out_stride + x] = a.history[p * a.hist_stride + x];
     if (threadIdx.x == 0) {
-      if (fits) a.out_history[o * a.out_stride + n] = c.flat - b * a.vocab;
+      if (ok) a.out_history[o * a.out_stride + n] = (int)c.flat - b * a.vocab;
       else atomicOr(a.err, kErrBadInput);
-      a.out_len[o] = fits ? n + 1 : n;
+      a.out_len[o] = ok ? n + 1 : n;
     }
   }
 }
 
 int slices_of(int batch, int beams, int vocab) {
-  // Enough CTAs for four on each SM, none with less than 2048 elements.
+  // As many CTAs as are resident at once (four on each SM), none with less
+  // than 2048 elements.
   const long long rows = (long long)batch * beams;
-  long long n = (4ll * device_sm_count() + rows - 1) / rows;
+  long long n = 4ll * device_sm_count() / rows;
   const long long most = (vocab + 2047) / 2048;
   n = n < most ? n : most;
   n = n < kMaxSlices ? n : kMaxSlices;

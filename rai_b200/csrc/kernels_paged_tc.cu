@@ -758,8 +758,8 @@ cudaError_t launch(const AttnArgs& a, const KvMaps& maps, int box, cudaStream_t 
   p.min_tiles = C::DUO ? 6 : 8;
   p.item_cost = C::DUO ? 2 : 3;
   p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
-  // Not launched ahead of its predecessor's end: its CTAs would share the SMs
-  // with the last call's join and run unevenly.
+  // Not launched ahead of its predecessor's end: a batch of prompts takes 344
+  // us so and 357 us with it (long verification: 165 either way).
   paged_attn_tc_kernel<C, CAP, TMA><<<p.grid, kTcThreads, C::kSmem, s>>>(p, maps, box);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
