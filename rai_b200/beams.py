@@ -64,11 +64,9 @@ def select(logits: torch.Tensor, scores: torch.Tensor, *, keep: Optional[int] = 
     dev = _device(("logits", logits), ("scores", scores))
     if b == 0 or n == 0 or v == 0:
         raise ValueError("logits: a size is zero")
-    # One allocation for the float outputs, one for the integer ones.
-    fl = scores.new_empty((b * (keep + n),))
-    it = scores.new_empty((2 * b * (keep + n),), dtype=torch.int32)
-    cs, sc = fl.split([b * keep, b * n])
-    cb, ct, pa, tk = it.split([b * keep, b * keep, b * n, b * n])
+    cs, sc = scores.new_empty((b, keep)), torch.empty_like(scores)
+    cb, ct = scores.new_empty((2, b, keep), dtype=torch.int32).unbind(0)
+    pa, tk = scores.new_empty((2, b, n), dtype=torch.int32).unbind(0)
     hist = [0, 0, 0, 0, 0, 0, 0]
     out_h = out_n = None
     if history is not None:
@@ -88,8 +86,7 @@ def select(logits: torch.Tensor, scores: torch.Tensor, *, keep: Optional[int] = 
                       pa.data_ptr(), tk.data_ptr(), *hist, b, n, v, keep, eos, dtype, workspace.data_ptr(),
                       workspace.numel() * workspace.element_size())
     _launch(dev, lib().rai_gpu_beam_select, args)
-    return BeamChoice(cs.view(b, keep), cb.view(b, keep), ct.view(b, keep), sc.view(b, n), pa.view(b, n), tk.view(b, n),
-                      out_h, out_n)
+    return BeamChoice(cs, cb, ct, sc, pa, tk, out_h, out_n)
 
 
 __all__ = ["BeamChoice", "select"]

@@ -41,11 +41,32 @@ __device__ __forceinline__ uint64_t key_of(float x, int token) {
 // infinite logits shares its mass among them, a row of -inf among all. (The
 // error of ex2.approx is the same function of x - m in every row: it all but
 // cancels between beams.)
-__device__ __forceinline__ float weight(float x, float m) {
+__device__ __forceinline__ float exp_of(float d) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((x - m) * kLog2e));
-  return x == m ? 1.f : r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * kLog2e));
+  return r;
 }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 exp2_of(float2 a) {
+  float2 d;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d.x) : "f"(a.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d.y) : "f"(a.y));
+  return d;
+}
+__device__ __forceinline__ float weight(float x, float m) { return x == m ? 1.f : exp_of(x - m); }
 
 template <int DT>
 __device__ __forceinline__ float to_f32(uint32_t w, int half) {
@@ -76,9 +97,24 @@ __device__ __forceinline__ void bitonic(uint64_t* a, int n) {
   __syncthreads();
 }
 
-// The `keep` largest of buf[0 .. n), sorted, in front; keys are unique.
+// The `keep` largest of buf[0 .. n), sorted, in front; keys are unique. Up to
+// a key per thread each counts the larger ones (n steps, two barriers; a sort
+// of 256 has 36 barriers and takes three times as long), more are sorted.
 __device__ __forceinline__ void prune(uint64_t* buf, int n, int keep) {
-  int size = 64;
+  if (n <= kThreads) {
+    uint64_t k = 0;
+    int rank = 0;
+    if ((int)threadIdx.x < n) {
+      k = buf[threadIdx.x];
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) rank += buf[i] > k;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < n && rank < keep) buf[rank] = k;
+    __syncthreads();
+    return;
+  }
+  int size = 512;
   while (size < n) size <<= 1;
   for (int i = n + threadIdx.x; i < size; i += kThreads) buf[i] = 0;
   bitonic(buf, size);
@@ -90,7 +126,8 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(BeamArgs a, int
   constexpr int kE = DT == kF32 ? 4 : 2;
   constexpr int N = 16, kVecs = N / V;   // elements and 16-byte loads of a thread in a step
   __shared__ uint64_t buf[kBufCap];
-  __shared__ uint64_t tops[kThreads];
+  __shared__ uint64_t tops[kMaxKeep + 1];
+  static_assert(kThreads / 4 == kMaxKeep, "groups");
   __shared__ int count;
   __shared__ float wm[kThreads / 32];
   __shared__ double wsum[kThreads / 32];
@@ -146,70 +183,72 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(BeamArgs a, int
     if (at + kThreads * N < end) fetch(at + kThreads * N, w);  // in flight through this step
     float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (!(x[i] == x[i])) x[i] = -INFINITY;  // a NaN is not chosen
-      top = fmaxf(top, x[i]);                 // (elements that are not there are -inf)
-    }
+    for (int i = 0; i < N; ++i) top = fmaxf(top, x[i]);  // (elements that are not there are -inf)
     if (there) {
       if (top > m) {
         sum *= (double)weight(m, top);
         m = top;
       }
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
-      if (there == (uint32_t)((1ull << N) - 1)) {
+      // Pairs: (x - m) log2(e), exponentials, sums.
+      float2 part[2] = {{0.f, 0.f}, {0.f, 0.f}};
+      const float2 mm = {-m, -m};
 #pragma unroll
-        for (int i = 0; i < N; ++i) part[i & 3] += weight(x[i], m);
-      } else {
+      for (int i = 0; i < N; i += 2) part[i / 2 & 1] = add2(part[i / 2 & 1], exp2_of(mul2(add2({x[i], x[i + 1]}, mm), {kLog2e, kLog2e})));
+      float all = (part[0].x + part[0].y) + (part[1].x + part[1].y);
+      if (!(fabsf(m) <= 3.4028235e38f) || !(all == all)) {
+        // An infinite maximum, or a NaN among them, which is not chosen.
+        all = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (there >> i & 1u) part[i & 3] += weight(x[i], m);
+        for (int i = 0; i < N; ++i) {
+          if (!(x[i] == x[i])) x[i] = -INFINITY;
+          if (there >> i & 1u) all += weight(x[i], m);
+        }
       }
-      sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
+      sum += (double)all;
     }
     if (at == base) {
-      // The keep-th largest of the threads' best is no larger than the
-      // keep-th largest element: a first bar.
+      // A first bar: the keep-th largest of the best of 64 groups of four
+      // threads is no larger than the keep-th largest element.
       uint64_t best = 0;
 #pragma unroll
       for (int i = 0; i < N; ++i)
         if ((there >> i & 1u) && x[i] == top) best = max(best, key_of(x[i], first_of(at, i / V) + i % V));
-      tops[threadIdx.x] = best;
-      bitonic(tops, kThreads);
-      bar = tops[a.keep - 1];
+      best = max(best, __shfl_xor_sync(~0u, best, 1));
+      best = max(best, __shfl_xor_sync(~0u, best, 2));
+      if ((threadIdx.x & 3) == 0) tops[threadIdx.x >> 2] = best;
+      __syncthreads();
+      if (threadIdx.x < kMaxKeep) {
+        const uint64_t k = tops[threadIdx.x];
+        int rank = 0;
+#pragma unroll 8
+        for (int i = 0; i < kMaxKeep; ++i) rank += tops[i] > k || (tops[i] == k && i < (int)threadIdx.x);
+        if (rank == a.keep - 1) tops[kMaxKeep] = k;
+      }
+      __syncthreads();
+      bar = tops[kMaxKeep];
     }
     // Elements at or above the bar go to the buffer; whenever it fills up it
     // is cut to the keep best, which raises the bar.
-    uint32_t pending = 0;
-    {
-      const float bar_x = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
-      if (there && top >= bar_x) {
+    uint32_t pending = 0;  // elements that found the buffer full
+    float bar_x = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
+    auto push = [&](uint32_t among) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          if ((there >> i & 1u) && x[i] >= bar_x) pending |= 1u << i;
-      }
-    }
-    for (;;) {
-      const uint64_t lowest = bar;
-      if (pending) {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (pending >> i & 1u) {
-            const uint64_t k = key_of(x[i], first_of(at, i / V) + i % V);
-            if (k < lowest) {
-              pending &= ~(1u << i);
-              continue;
-            }
+      for (int i = 0; i < N; ++i)
+        if (x[i] >= bar_x && (among >> i & 1u)) {
+          const uint64_t k = key_of(x[i], first_of(at, i / V) + i % V);
+          if (k >= bar) {
             const int slot = atomicAdd(&count, 1);
-            if (slot < kBufCap) {
-              buf[slot] = k;
-              pending &= ~(1u << i);
-            }
+            if (slot < kBufCap) buf[slot] = k;
+            else pending |= 1u << i;
           }
-      }
+        }
+    };
+    if (there && top >= bar_x) push(there);
+    for (;;) {
       const int again = __syncthreads_or(pending != 0);
       const int n = min(count, kBufCap);
       __syncthreads();  // everyone has read the count
-      if (again || n > 4 * a.keep + 192) {
+      if (again || n > a.keep + 80) {
         prune(buf, n, a.keep);
         bar = buf[min(n, a.keep) - 1];
         if (n < a.keep) bar = 0;
@@ -217,6 +256,10 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(BeamArgs a, int
         __syncthreads();
       }
       if (!again) break;
+      bar_x = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
+      const uint32_t rest = pending;
+      pending = 0;
+      if (rest) push(rest);
     }
   }
   __syncthreads();
