@@ -13,7 +13,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import native
-from .paged import _device, _dtype, _ints, _launch, lib
+from .paged import _cells, _device, _dtype, _ints, _launch, lib
 
 _ARGS = struct.Struct("2Qq6Q4Q2q5IiI4x2Q")
 
@@ -61,7 +61,7 @@ def select(logits: torch.Tensor, scores: torch.Tensor, *, keep: Optional[int] = 
         raise ValueError("scores: contiguous float32 [batch, beams]")
     if logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("logits: this operator has no gradient; call it under torch.no_grad()")
-    dev = _device(("logits", logits), ("scores", scores))
+    dev = _device(logits, scores)
     if b == 0 or n == 0 or v == 0:
         raise ValueError("logits: a size is zero")
     cs, sc = scores.new_empty((b, keep)), torch.empty_like(scores)
@@ -72,12 +72,11 @@ def select(logits: torch.Tensor, scores: torch.Tensor, *, keep: Optional[int] = 
     if history is not None:
         if hist_len is None:
             raise ValueError("hist_len: needed with history")
-        _device(("logits", logits), ("history", history), ("hist_len", hist_len))
+        _device(logits, history, hist_len)
         out_h = torch.empty_like(history, memory_format=torch.contiguous_format)
         out_n = torch.empty_like(hist_len)
-        stride = history.stride(0) if history.dim() == 2 and b * n > 1 else max(history.shape[-1], 1)
-        hist = [_ints("history", history, b * n, None), _ints("hist_len", hist_len, b * n), out_h.data_ptr(), out_n.data_ptr(),
-                stride, out_h.stride(0) if b * n > 1 else max(out_h.shape[-1], 1), history.shape[1]]
+        at, row_h, cap = _cells("history", history, b * n)
+        hist = [at, _ints("hist_len", hist_len, b * n), out_h.data_ptr(), out_n.data_ptr(), row_h, max(cap, 1), cap]
     if workspace is None:
         workspace = scores.new_empty((_workspace(dev, b, n, v, keep),), dtype=torch.uint8)
     elif workspace.get_device() != dev or not workspace.is_contiguous():

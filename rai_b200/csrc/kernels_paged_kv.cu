@@ -31,22 +31,32 @@ struct Elt<kBF16> {
   static __device__ __forceinline__ T put(float x) { return __float2bfloat16_rn(x); }
 };
 
-// N elements as 16-byte (or, for the narrower of two types, shorter) vectors.
+// N elements as 16-byte vectors (or one of 8 bytes), as they lie in memory
+// until they are needed.
 template <int DT, int N>
-__device__ __forceinline__ void load_n(const typename Elt<DT>::T* p, float (&x)[N]) {
+struct Raw {
   using T = typename Elt<DT>::T;
-  constexpr int kB = N * sizeof(T);
-  alignas(16) T v[N];
-  if constexpr (kB % 16 == 0) {
+  static constexpr int kB = N * sizeof(T);
+  static_assert(kB % 16 == 0 || kB == 8, "vector width");
+  uint32_t w[kB / 4];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kB % 16 == 0) {
 #pragma unroll
-    for (int i = 0; i < kB / 16; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
-  } else {
-    static_assert(kB == 8, "vector width");
-    reinterpret_cast<uint2*>(v)[0] = reinterpret_cast<const uint2*>(p)[0];
+      for (int i = 0; i < kB / 16; ++i) {
+        const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+      }
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x, w[1] = v.y;
+    }
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = Elt<DT>::get(v[i]);
-}
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (DT == kF32) return __uint_as_float(w[i]);
+    else if constexpr (DT == kBF16) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    else return __half2float(__ushort_as_half((uint16_t)(w[i / 2] >> (16 * (i & 1)))));
+  }
+};
 template <int DT, int N>
 __device__ __forceinline__ void store_n(typename Elt<DT>::T* p, const float (&x)[N]) {
   using T = typename Elt<DT>::T;
@@ -63,130 +73,175 @@ __device__ __forceinline__ void store_n(typename Elt<DT>::T* p, const float (&x)
   }
 }
 
-// cos and sin of pos * inv_freq. The product and its reduction by whole
-// turns are in 64 bits (a far position times a frequency has more than 24
-// significant bits above the point); what is left, within half a turn, has a
+// cos and sin of pos * inv_freq. The product and its reduction to a part of a
+// turn are in 64 bits (a far position times a frequency has more than 24
+// significant bits above the point); the part, within half a turn, has a
 // 32-bit sine and cosine.
 __device__ __forceinline__ void turn_of(int pos, float inv_freq, float mscale, float* c, float* s) {
-  const double a = (double)pos * (double)inv_freq;
-  const double n = rint(a * 0.15915494309189533577);
-  // 2 pi as a double and the rest of it.
-  const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.28318530717958647693, a));
+  const double t = (double)pos * (double)inv_freq * 0.15915494309189533577;
   float sv, cv;
-  sincosf((float)r, &sv, &cv);
+  sincospif((float)(2.0 * (t - rint(t))), &sv, &cv);
   *c = cv * mscale;
   *s = sv * mscale;
 }
 
 constexpr int kRopeThreads = 256;
 
-// One CTA per chunk row (looping): the row's angles go to shared memory, then
-// threads take vectors of kV elements of every q, k and v head; a half-split
-// pair's two vectors are one thread's work, so a rotation in place is safe.
-// Bound: HBM, each element read and written once.
+struct RopeUnits {
+  FastDiv rot, tail, whole;  // units of a head: rotated, behind the rotated part, all (v)
+  int parts;                 // warps that share a row
+};
+
+// The last s with q_start[s] <= row, by a warp: 32 probes a round.
+__device__ __forceinline__ int seq_of_row(const PagedChunk& c, int row, int lane) {
+  int lo = 0, span = c.n_seqs;
+  while (span > 1) {
+    const int step = (span + 31) / 32, at = lane * step;
+    const int n = __popc(__ballot_sync(~0u, at < span && c.q_start[lo + at] <= row));
+    if (n == 0) return 0;
+    lo += (n - 1) * step;
+    span = min(step, span - (n - 1) * step);
+  }
+  return lo;
+}
+
+// A warp takes a row, or with few rows a part of one: the row's angles go to
+// shared memory, then lanes take units of kV elements of every q, k and v
+// head (half-split: the two vectors of kV pairs, so a rotation in place is
+// safe), two units' loads before their stores. Bound: HBM, each element read
+// and written once; rows in flight hide the look-up of sequence and page.
 template <int IN, int OUT>
-__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const __grid_constant__ RopeArgs a,
+                                                                   const __grid_constant__ RopeUnits un) {
   using TI = typename Elt<IN>::T;
   using TO = typename Elt<OUT>::T;
   constexpr int kV = IN == kF32 && OUT == kF32 ? 4 : 8;
-  __shared__ float cs[128], sn[128];
+  constexpr int kU = IN == kF32 ? 1 : 2;
+  __shared__ float table[kRopeThreads / 32][2][128];
   const PagedChunk& ch = a.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float *cs = table[warp][0], *sn = table[warp][1];
+  const int half = a.rot / 2, stride = 32 * un.parts;
   pdl_wait_prior();
   pdl_launch_dependents();
-  const int half = a.rot / 2;
-  for (int row = blockIdx.x; row < ch.rows; row += gridDim.x) {
-    // The sequence of the row: the last with q_start <= row.
-    int lo = 0, hi = ch.n_seqs;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (ch.q_start[mid] <= row) lo = mid; else hi = mid;
-    }
-    const SeqRows r = seq_rows(ch, lo);
+  for (long long id = (long long)blockIdx.x * (kRopeThreads / 32) + warp; id < (long long)ch.rows * un.parts;
+       id += (long long)gridDim.x * (kRopeThreads / 32)) {
+    const int row = (int)(id / un.parts), part = (int)(id - (long long)row * un.parts);
+    const int seq = seq_of_row(ch, row, lane);
+    const SeqRows r = seq_rows(ch, seq);
     if (row < r.start || row >= r.start + r.n) continue;  // behind the last sequence (or before the first)
     const int pos = r.len - r.n + (row - r.start);
-    __syncthreads();
-    for (int i = threadIdx.x; i < half; i += kRopeThreads)
-      turn_of(pos, a.inv_freq[i], a.mscale, &cs[i], &sn[i]);
     int page = -1, slot = 0;
     if (pos >= 0) {
       const int pi = (int)ch.page.quot(pos);
-      page = page_of(ch, lo, pi);
+      page = page_of(ch, seq, pi);
       slot = pos - pi * (int)ch.page.d;
     }
-    __syncthreads();
+    __syncwarp();  // the last row's angles have been read
+    for (int i = lane; i < half; i += 32) turn_of(pos, a.inv_freq[i], a.mscale, &cs[i], &sn[i]);
+    __syncwarp();
     const TI* qr = static_cast<const TI*>(a.q) + (long long)row * a.q_row;
     const TI* kr = static_cast<const TI*>(a.k) + (long long)row * a.k_row;
     const TI* vr = static_cast<const TI*>(a.v) + (long long)row * a.v_row;
     TO* qo = static_cast<TO*>(a.q_out) + (long long)row * a.o_row;
     TO* ko = static_cast<TO*>(ch.k) + page * ch.k_page + slot * ch.k_slot;
     TO* vo = static_cast<TO*>(ch.v) + page * ch.v_page + slot * ch.v_slot;
+    const int turned = page >= 0 ? a.heads + ch.nkv : a.heads;  // heads of q, then of k
+    auto from = [&](int h) { return h < a.heads ? qr + (long long)h * a.q_head : kr + (long long)(h - a.heads) * a.k_head; };
+    auto into = [&](int h) { return h < a.heads ? qo + (long long)h * a.o_head : ko + (long long)(h - a.heads) * ch.k_head; };
     if (half % kV) {
       // Pairs do not fall on vectors: one pair, or one element behind the
       // rotated part, at a time.
       const int per = ch.hd - half;
-      for (int x = threadIdx.x; x < (a.heads + 2 * ch.nkv) * per; x += kRopeThreads) {
+      const int all = turned + (page >= 0 ? ch.nkv : 0);
+      for (int x = lane + 32 * part; x < all * per; x += stride) {
         const int head = x / per, e = x - head * per;
-        const bool is_q = head < a.heads, is_k = !is_q && head < a.heads + ch.nkv;
-        if (!is_q && page < 0) continue;
-        const int h = is_q ? head : is_k ? head - a.heads : head - a.heads - ch.nkv;
-        const TI* src = is_q ? qr + (long long)h * a.q_head : is_k ? kr + (long long)h * a.k_head : vr + (long long)h * a.v_head;
-        TO* dst = is_q ? qo + (long long)h * a.o_head : is_k ? ko + (long long)h * ch.k_head : vo + (long long)h * ch.v_head;
+        const bool turn = head < turned;
+        const TI* src = turn ? from(head) : vr + (long long)(head - turned) * a.v_head;
+        TO* dst = turn ? into(head) : vo + (long long)(head - turned) * ch.v_head;
         if (e >= half) {
           dst[half + e] = Elt<OUT>::put(Elt<IN>::get(src[half + e]));
           continue;
         }
         const int i = a.interleaved ? 2 * e : e, j = a.interleaved ? 2 * e + 1 : e + half;
         const float x0 = Elt<IN>::get(src[i]), x1 = Elt<IN>::get(src[j]);
-        const float c = is_q || is_k ? cs[e] : 1.f, s = is_q || is_k ? sn[e] : 0.f;
-        dst[i] = Elt<OUT>::put(is_q || is_k ? x0 * c - x1 * s : x0);
-        dst[j] = Elt<OUT>::put(is_q || is_k ? x1 * c + x0 * s : x1);
+        const float c = turn ? cs[e] : 1.f, s = turn ? sn[e] : 0.f;
+        dst[i] = Elt<OUT>::put(turn ? x0 * c - x1 * s : x0);
+        dst[j] = Elt<OUT>::put(turn ? x1 * c + x0 * s : x1);
       }
       continue;
     }
-    const int per = ch.hd / kV;  // vectors of a head
-    const int total = (a.heads + 2 * ch.nkv) * per;
-    for (int x = threadIdx.x; x < total; x += kRopeThreads) {
-      const int head = x / per, d = (x - head * per) * kV;
-      const TI* src;
-      TO* dst;
-      bool rotate = true;
-      if (head < a.heads) {
-        src = qr + (long long)head * a.q_head;
-        dst = qo + (long long)head * a.o_head;
-      } else if (head < a.heads + ch.nkv) {
-        if (page < 0) continue;
-        src = kr + (long long)(head - a.heads) * a.k_head;
-        dst = ko + (long long)(head - a.heads) * ch.k_head;
-      } else {
-        if (page < 0) continue;
-        src = vr + (long long)(head - a.heads - ch.nkv) * a.v_head;
-        dst = vo + (long long)(head - a.heads - ch.nkv) * ch.v_head;
-        rotate = false;
+    // Rotated units.
+    const int n_rot = turned * (int)un.rot.d;
+    for (int x0 = lane + 32 * part; x0 < n_rot; x0 += stride * kU) {
+      Raw<IN, kV> u[kU], w[kU];
+#pragma unroll
+      for (int k = 0; k < kU; ++k) {
+        const int x = x0 + k * stride;
+        if (x < n_rot) {
+          const int h = (int)un.rot.quot(x);
+          const TI* src = from(h) + (x - h * (int)un.rot.d) * kV;
+          u[k].load(src);
+          if (!a.interleaved) w[k].load(src + half);
+        }
       }
-      float u[kV], w[kV];
-      if (!rotate || d >= a.rot) {
-        load_n<IN, kV>(src + d, u);
-        store_n<OUT, kV>(dst + d, u);
-      } else if (a.interleaved) {
-        load_n<IN, kV>(src + d, u);
 #pragma unroll
-        for (int i = 0; i < kV; i += 2) {
-          const float c = cs[d / 2 + i / 2], s = sn[d / 2 + i / 2];
-          w[i] = u[i] * c - u[i + 1] * s;
-          w[i + 1] = u[i + 1] * c + u[i] * s;
-        }
-        store_n<OUT, kV>(dst + d, w);
-      } else if (d < half) {
-        load_n<IN, kV>(src + d, u);
-        load_n<IN, kV>(src + d + half, w);
+      for (int k = 0; k < kU; ++k) {
+        const int x = x0 + k * stride;
+        if (x < n_rot) {
+          const int h = (int)un.rot.quot(x), d = (x - h * (int)un.rot.d) * kV;
+          TO* dst = into(h) + d;
+          float y[kV];
+          if (a.interleaved) {
 #pragma unroll
-        for (int i = 0; i < kV; ++i) {
-          const float c = cs[d + i], s = sn[d + i], x0 = u[i], x1 = w[i];
-          u[i] = x0 * c - x1 * s;
-          w[i] = x1 * c + x0 * s;
+            for (int i = 0; i < kV; i += 2) {
+              const float c = cs[d / 2 + i / 2], s = sn[d / 2 + i / 2], y0 = u[k].get(i), y1 = u[k].get(i + 1);
+              y[i] = y0 * c - y1 * s;
+              y[i + 1] = y1 * c + y0 * s;
+            }
+          } else {
+            float z[kV];
+#pragma unroll
+            for (int i = 0; i < kV; ++i) {
+              const float c = cs[d + i], s = sn[d + i], y0 = u[k].get(i), y1 = w[k].get(i);
+              y[i] = y0 * c - y1 * s;
+              z[i] = y1 * c + y0 * s;
+            }
+            store_n<OUT, kV>(dst + half, z);
+          }
+          store_n<OUT, kV>(dst, y);
         }
-        store_n<OUT, kV>(dst + d, u);
-        store_n<OUT, kV>(dst + d + half, w);
+      }
+    }
+    // Copies: what lies behind the rotated part, then v.
+    const int n_tail = a.rot < ch.hd ? turned * (int)un.tail.d : 0, n_all = n_tail + (page >= 0 ? ch.nkv * (int)un.whole.d : 0);
+    for (int x0 = lane + 32 * part; x0 < n_all; x0 += stride * kU) {
+      Raw<IN, kV> u[kU];
+#pragma unroll
+      for (int k = 0; k < kU; ++k) {
+        const int x = x0 + k * stride;
+        if (x < n_tail) {
+          const int h = (int)un.tail.quot(x);
+          u[k].load(from(h) + a.rot + (x - h * (int)un.tail.d) * kV);
+        } else if (x < n_all) {
+          const int h = (int)un.whole.quot(x - n_tail);
+          u[k].load(vr + (long long)h * a.v_head + (x - n_tail - h * (int)un.whole.d) * kV);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kU; ++k) {
+        const int x = x0 + k * stride;
+        if (x >= n_all) continue;
+        float y[kV];
+#pragma unroll
+        for (int i = 0; i < kV; ++i) y[i] = u[k].get(i);
+        if (x < n_tail) {
+          const int h = (int)un.tail.quot(x);
+          store_n<OUT, kV>(into(h) + a.rot + (x - h * (int)un.tail.d) * kV, y);
+        } else {
+          const int h = (int)un.whole.quot(x - n_tail);
+          store_n<OUT, kV>(vo + (long long)h * ch.v_head + (x - n_tail - h * (int)un.whole.d) * kV, y);
+        }
       }
     }
   }
@@ -271,6 +326,56 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int* total) {  // excl
   return incl - v + (warp ? sh[warp - 1] : 0);
 }
 
+// A warp's run of the pages: 32 * n consecutive ones.
+struct Run {
+  int first, groups;
+};
+__device__ __forceinline__ Run run_of(int n_pages) {
+  const int groups = (n_pages + 31) / 32, warps = kMetaThreads / 32, per = (groups + warps - 1) / warps;
+  const int g0 = min(groups, (int)(threadIdx.x >> 5) * per);
+  return {g0 * 32, min(per, groups - g0)};
+}
+// f(page, whether the lane has one, its count) for each group of 32 pages of
+// the run, eight groups' counts fetched at a time; with STOP until f is false.
+template <bool STOP, typename F>
+__device__ __forceinline__ void scan_run_of(const int* refs, int n_pages, const Run& run, F f) {
+  const int lane = threadIdx.x & 31;
+  for (int g0 = 0; g0 < run.groups; g0 += 8) {
+    int v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int p = run.first + (g0 + i) * 32 + lane;
+      v[i] = g0 + i < run.groups && p < n_pages ? __ldcg(refs + p) : 1;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (g0 + i >= run.groups) return;
+      const int p = run.first + (g0 + i) * 32 + lane;
+      if constexpr (STOP) {
+        if (!f(p, p < n_pages, v[i])) return;
+      } else {
+        f(p, p < n_pages, v[i]);
+      }
+    }
+  }
+}
+// Exclusive sum over the block's warps of a value that each warp agrees on.
+__device__ __forceinline__ int warp_scan(int v, int* sh, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __syncthreads();
+  if (lane == 0) sh[warp] = v;
+  __syncthreads();
+  const int mine = sh[lane];  // kMetaThreads / 32 = 32 warps
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(~0u, incl, o);
+    if (lane >= o) incl += u;
+  }
+  *total = __shfl_sync(~0u, incl, 31);
+  return __shfl_sync(~0u, incl - mine, warp);
+}
+
 // One CTA. Releases what shrinks, then gives the sequences that grow the
 // lowest free pages in sequence order: first the copy of a shared last page
 // that is partly filled (all holders but the last copy it), then new pages.
@@ -341,13 +446,13 @@ __global__ void __launch_bounds__(kMetaThreads) kv_resize_kernel(TableArgs t, co
     place[s] = at;
     at += c;
   }
-  // Free pages, in order: each thread looks at a run of the counts.
-  const int run = (t.n_pages + kMetaThreads - 1) / kMetaThreads;
-  const int p0 = min((long long)t.n_pages, (long long)threadIdx.x * run), p1 = min(t.n_pages, p0 + run);
+  // Free pages, in order: each warp looks at a run of the counts, 32 at a
+  // time.
+  const Run run = run_of(t.n_pages);
   int mine = 0;
-  for (int p = p0; p < p1; ++p) mine += *(volatile int*)(t.refs + p) == 0;
+  scan_run_of<false>(t.refs, t.n_pages, run, [&](int p, bool in, int refs) { mine += __popc(__ballot_sync(~0u, in && refs == 0)); });
   int free_total;
-  int rank = block_scan(mine, sh, &free_total);
+  int rank = warp_scan(mine, sh, &free_total);
   const bool fits = total <= free_total;
   __shared__ int count;
   if (threadIdx.x == 0) {
@@ -356,29 +461,34 @@ __global__ void __launch_bounds__(kMetaThreads) kv_resize_kernel(TableArgs t, co
   }
   __syncthreads();
   if (fits && total > 0) {
-    for (int p = p0; p < p1 && rank < total; ++p) {
-      if (*(volatile int*)(t.refs + p) != 0) continue;
-      // The sequence that takes the rank-th page.
-      int lo = 0, hi = n;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (place[mid] <= rank) lo = mid; else hi = mid;
-      }
-      const int s = lo, len = table_len(t, t.lens, s);
-      int in = rank - place[s], cell = cells_of(len, ps) + in;
-      if (tail[s] >= 0) {
-        --cell;
-        if (in == 0) {
-          const int c = atomicAdd(&count, 1);
-          ws[1 + c] = tail[s];
-          ws[1 + n + c] = p;
-          atomicSub(t.refs + tail[s], 1);
+    scan_run_of<true>(t.refs, t.n_pages, run, [&](int p, bool in, int refs) {
+      const bool free = in && refs == 0;
+      const uint32_t mask = __ballot_sync(~0u, free);
+      const int mine_at = rank + __popc(mask & ((1u << (threadIdx.x & 31)) - 1u));
+      rank += __popc(mask);
+      if (free && mine_at < total) {
+        // The sequence that takes the page of this rank.
+        int lo = 0, hi = n;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (place[mid] <= mine_at) lo = mid; else hi = mid;
         }
+        const int s = lo, len = table_len(t, t.lens, s);
+        int nth = mine_at - place[s], cell = cells_of(len, ps) + nth;
+        if (tail[s] >= 0) {
+          --cell;
+          if (nth == 0) {
+            const int c = atomicAdd(&count, 1);
+            ws[1 + c] = tail[s];
+            ws[1 + n + c] = p;
+            atomicSub(t.refs + tail[s], 1);
+          }
+        }
+        t.table[(long long)s * t.stride + cell] = p;
+        t.refs[p] = 1;
       }
-      t.table[(long long)s * t.stride + cell] = p;
-      t.refs[p] = 1;
-      ++rank;
-    }
+      return rank < total;
+    });
   }
   __syncthreads();
   if (threadIdx.x == 0) ws[0] = count;
@@ -396,28 +506,30 @@ __global__ void __launch_bounds__(kMetaThreads) kv_resize_kernel(TableArgs t, co
 __global__ void __launch_bounds__(kMetaThreads) kv_compact_kernel(TableArgs t, int* used_out, int* ws, int* moved) {
   __shared__ int sh[32];
   pdl_wait_prior();
-  const int run = (t.n_pages + kMetaThreads - 1) / kMetaThreads;
-  const int p0 = min((long long)t.n_pages, (long long)threadIdx.x * run), p1 = min(t.n_pages, p0 + run);
+  const Run run = run_of(t.n_pages);
+  const uint32_t below = (1u << (threadIdx.x & 31)) - 1u;
   int mine = 0;
-  for (int p = p0; p < p1; ++p) mine += t.refs[p] > 0;
+  scan_run_of<false>(t.refs, t.n_pages, run, [&](int p, bool in, int refs) { mine += __popc(__ballot_sync(~0u, in && refs > 0)); });
   int used;
-  block_scan(mine, sh, &used);
+  warp_scan(mine, sh, &used);
   int holes = 0, highs = 0;
-  for (int p = p0; p < p1; ++p) {
-    const bool held = t.refs[p] > 0;
-    holes += !held && p < used;
-    highs += held && p >= used;
-  }
+  scan_run_of<false>(t.refs, t.n_pages, run, [&](int p, bool in, int refs) {
+    holes += __popc(__ballot_sync(~0u, in && refs <= 0 && p < used));
+    highs += __popc(__ballot_sync(~0u, in && refs > 0 && p >= used));
+  });
   int n_holes, n_highs;
-  int hole = block_scan(holes, sh, &n_holes);
-  int high = block_scan(highs, sh, &n_highs);  // n_highs == n_holes
+  int hole = warp_scan(holes, sh, &n_holes);
+  int high = warp_scan(highs, sh, &n_highs);  // n_highs == n_holes
   int *src = ws + 1, *dst = ws + 1 + t.n_pages / 2;
-  for (int p = p0; p < p1; ++p) {
-    const bool held = t.refs[p] > 0;
-    if (!held && p < used) dst[hole++] = p;
-    if (held && p >= used) src[high++] = p;
-    moved[p] = p;
-  }
+  scan_run_of<false>(t.refs, t.n_pages, run, [&](int p, bool in, int refs) {
+    const bool is_hole = in && refs <= 0 && p < used, is_high = in && refs > 0 && p >= used;
+    const uint32_t mh = __ballot_sync(~0u, is_hole), mg = __ballot_sync(~0u, is_high);
+    if (is_hole) dst[hole + __popc(mh & below)] = p;
+    if (is_high) src[high + __popc(mg & below)] = p;
+    hole += __popc(mh);
+    high += __popc(mg);
+    if (in) moved[p] = p;
+  });
   __syncthreads();
   for (int i = threadIdx.x; i < n_highs; i += kMetaThreads) {
     const int a = src[i], b = dst[i];
@@ -485,10 +597,21 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(PagePool pool, co
 }  // namespace
 
 cudaError_t rope_append(const RopeArgs& a, cudaStream_t s) {
-  const int grid = grid_cap(a.c.rows, 8);
+  const int kv = a.in_dtype == kF32 && a.cache_dtype == kF32 ? 4 : 8, half = a.rot / 2;
+  RopeUnits un;
+  un.parts = 1;
+  if (half % kv == 0) {
+    un.rot = FastDiv((a.interleaved ? a.rot : half) / kv);
+    un.tail = FastDiv(a.rot < a.c.hd ? (a.c.hd - a.rot) / kv : 1);
+    un.whole = FastDiv(a.c.hd / kv);
+  }
+  // Few rows: up to eight warps a row, until every SM has two CTAs' worth.
+  while (un.parts < 8 && (long long)a.c.rows * un.parts * 2 <= 16ll * device_sm_count()) un.parts *= 2;
+  const long long ctas = ((long long)a.c.rows * un.parts + kRopeThreads / 32 - 1) / (kRopeThreads / 32);
+  const int grid = grid_cap(ctas < INT_MAX ? (int)ctas : INT_MAX, 8);
 #define RAI_ROPE(I, O)                                                                                   \
   if (a.in_dtype == I && a.cache_dtype == O)                                                             \
-    return launch_pdl(rope_append_kernel<I, O>, dim3(grid), dim3(kRopeThreads), 0, s, a);
+    return launch_pdl(rope_append_kernel<I, O>, dim3(grid), dim3(kRopeThreads), 0, s, a, un);
   RAI_ROPE(kF32, kF32) RAI_ROPE(kF32, kF16) RAI_ROPE(kF32, kBF16)
   RAI_ROPE(kF16, kF32) RAI_ROPE(kF16, kF16) RAI_ROPE(kF16, kBF16)
   RAI_ROPE(kBF16, kF32) RAI_ROPE(kBF16, kF16) RAI_ROPE(kBF16, kBF16)

@@ -46,12 +46,14 @@ def _dtype(t: torch.Tensor, name: str) -> int:
     return d
 
 
-def _device(*tensors: Tuple[str, torch.Tensor]) -> int:
+def _device(first: torch.Tensor, *rest: torch.Tensor) -> int:
     """The CUDA device that all tensors are on."""
-    dev = tensors[0][1].get_device()
-    for name, t in tensors:
-        if t.get_device() != dev or dev < 0:
-            raise ValueError(f"{name}: every tensor has to be on one CUDA device")
+    dev = first.get_device()
+    for t in rest:
+        if t.get_device() != dev:
+            dev = -1
+    if dev < 0:
+        raise ValueError("every tensor has to be on one CUDA device")
     return dev
 
 
@@ -81,22 +83,29 @@ def _launch(dev: int, fn, *args) -> None:
         check(rc)
 
 
-def _ints(name: str, t: torch.Tensor, *shape: Optional[int]) -> int:
-    """Address of an int32 tensor of this shape, its last dimension dense."""
-    got = t.shape
-    if t.dtype is not torch.int32 or len(got) != len(shape):
-        raise ValueError(f"{name}: an int32 tensor of {len(shape)} dimension(s)")
-    for a, b in zip(got, shape):
-        if b is not None and a != b:
-            raise ValueError(f"{name}: shape {tuple(got)} does not fit the other arguments")
-    if not t.is_contiguous() and got[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name}: the last dimension has to be contiguous")
+_INT = torch.int32
+
+
+def _ints(name: str, t: torch.Tensor, n: int) -> int:
+    """Address of an int32 vector of n elements."""
+    if t.dtype is not _INT or t.shape != (n,):
+        raise ValueError(f"{name}: an int32 vector that fits the other arguments ({n}), not {t.dtype} {tuple(t.shape)}")
+    if n > 1 and not t.is_contiguous():
+        raise ValueError(f"{name}: has to be contiguous")
     return t.data_ptr()
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    """Row stride of a table; a one-row table may have any."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _cells(name: str, t: torch.Tensor, n: int):
+    """Address, row stride and columns of an int32 table of n rows."""
+    shape = t.shape
+    if t.dtype is not _INT or len(shape) != 2 or shape[0] != n:
+        raise ValueError(f"{name}: an int32 table of {n} rows, not {t.dtype} {tuple(shape)}")
+    if t.is_contiguous():
+        return t.data_ptr(), shape[1], shape[1]
+    if shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: the last dimension has to be contiguous")
+    # A one-row table may have any row stride.
+    return t.data_ptr(), t.stride(0) if n > 1 else max(t.stride(0), shape[1]), shape[1]
 
 
 def _rows3(name: str, t: torch.Tensor, heads: Optional[int], dim: int):
@@ -120,10 +129,10 @@ def _chunk(k_pages, v_pages, table, kv_len, q_start, rows: int, max_rows: int, d
     if hd > 1 and (ks[3] != 1 or vs[3] != 1):
         raise ValueError("k_pages, v_pages: head_dim has to be contiguous")
     n = kv_len.shape[0]
-    at = _ints("page_table", table, n, None)
+    at, row, width = _cells("page_table", table, n)
     return (k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
             at, _ints("kv_len", kv_len, n), _ints("q_start", q_start, n + 1),
-            _row_stride(table), n, table.shape[1], n_pages, page, nkv, hd, rows, max_rows, dtype)
+            row, n, width, n_pages, page, nkv, hd, rows, max_rows, dtype)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -167,8 +176,7 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
         os = _rows3("out", out, heads, hd)
         if out.shape[0] != rows or out.dtype is not q.dtype:
             raise ValueError("out: shape and type of q")
-    dev = _device(("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("kv_len", kv_len),
-                  ("q_start", q_start), ("out", out))
+    dev = _device(q, k_pages, v_pages, page_table, kv_len, q_start, out)
     if rows == 0 or kv_len.shape[0] == 0 or max_rows == 0:
         return out
     if max_rows > rows:
@@ -219,8 +227,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torc
         os = _rows3("q_out", q_out, heads, hd)
         if q_out.shape[0] != rows or q_out.dtype is not k_pages.dtype:
             raise ValueError("q_out: q's shape in the pages' type")
-    dev = _device(("q", q), ("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table),
-                  ("kv_len", kv_len), ("q_start", q_start), ("inv_freq", inv_freq), ("q_out", q_out))
+    dev = _device(q, k, v, k_pages, v_pages, page_table, kv_len, q_start, inv_freq, q_out)
     if rows == 0 or kv_len.shape[0] == 0:
         return q_out
     args = _ROPE.pack(*_chunk(k_pages, v_pages, page_table, kv_len, q_start, rows, rows, dtype), q.data_ptr(), k.data_ptr(),
@@ -245,39 +252,36 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, kind: str = "plain", 
 
 
 def _table(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, page_size: int) -> bytes:
-    n = table.shape[0]
-    return _TABLE.pack(_ints("page_table", table, None, None), _ints("lens", lens, n), _ints("refs", refs, None),
-                       _row_stride(table), n, table.shape[1], refs.shape[0], page_size)
+    n, pages = lens.shape[0], refs.shape[0]
+    at, row, width = _cells("page_table", table, n)
+    return _TABLE.pack(at, _ints("lens", lens, n), _ints("refs", refs, pages), row, n, width, pages, page_size)
 
 
 def _pool(k: torch.Tensor, v: torch.Tensor):
     """(bytes of rai_page_pool, page size) of the K and V pages of every
     layer: [layers, pages, kv_heads, page_size, head_dim], or one layer's four
     dimensions, a page being one dense block."""
-    if k.dim() == 4:
-        k = k.unsqueeze(0)
-    if v.dim() == 4:
-        v = v.unsqueeze(0)
-    shape = k.shape
-    _dtype(k, "k")
-    if len(shape) != 5 or shape != v.shape or k.dtype is not v.dtype:
+    shape, kst, vst = k.shape, k.stride(), v.stride()
+    if shape != v.shape or k.dtype is not v.dtype or len(shape) not in (4, 5):
         raise ValueError("k, v: two tensors [layers, pages, kv_heads, page_size, head_dim] of one shape and type")
+    _dtype(k, "k")
+    if len(shape) == 4:
+        shape, kst, vst = (1, *shape), (0, *kst), (0, *vst)
     e = k.element_size()
     layers, pages, heads, slots, dim = shape
     n = heads * slots * dim
-    strides = []
-    for name, t in (("k", k), ("v", v)):
-        st = t.stride()
-        if st[2:] != (slots * dim, dim, 1):
+    if (kst[2], kst[3], kst[4]) != (slots * dim, dim, 1) or vst != kst:
+        for st in (kst, vst):
             # A page's block may order its heads and slots either way.
             want = 1
             for s, m in sorted((s, m) for s, m in zip(st[2:], shape[2:]) if m > 1):
                 if s != want:
-                    raise ValueError(f"{name}: every page has to be one contiguous block")
+                    raise ValueError("k, v: every page has to be one contiguous block")
                 want *= m
-        # The stride of a single page or layer means nothing.
-        strides += [st[0] * e if layers > 1 else 0, st[1] * e if pages > 1 else n * e]
-    return _POOL.pack(k.data_ptr(), v.data_ptr(), *strides, n * e, layers, pages), slots
+    # The stride of a single page or layer means nothing.
+    kl, vl = (kst[0] * e, vst[0] * e) if layers > 1 else (0, 0)
+    kp, vp = (kst[1] * e, vst[1] * e) if pages > 1 else (n * e, n * e)
+    return _POOL.pack(k.data_ptr(), v.data_ptr(), kl, kp, vl, vp, n * e, layers, pages), slots
 
 
 def fork(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor, page_size: int, *,
@@ -293,10 +297,7 @@ def fork(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, paren
         out_table = page_table.new_empty((n, page_table.shape[1]))
     if out_lens is None:
         out_lens = lens.new_empty((n,))
-    dev = _device(("page_table", page_table), ("lens", lens), ("refs", refs), ("parents", parents), ("out_table", out_table),
-                  ("out_lens", out_lens))
-    if out_table.dim() != 2 or out_table.shape[0] != n:
-        raise ValueError("out_table: one row per parent")
+    dev = _device(page_table, lens, refs, parents, out_table, out_lens)
     _launch(dev, lib().rai_gpu_kv_fork, _table(page_table, lens, refs, page_size),
             _table(out_table, out_lens, refs, page_size), _ints("parents", parents, n))
     return out_table, out_lens
@@ -311,9 +312,8 @@ def resize(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, k: 
     that is partly filled. k, v: the pages of every layer. Returns an int32
     [1] on the device: 0, or the number of pages missing, when nothing grew."""
     pool, page = _pool(k, v)
-    dev = _device(("page_table", page_table), ("lens", lens), ("refs", refs), ("k", k), ("v", v),
-                  *((("new_lens", new_lens),) if new_lens is not None else ()))
-    n = page_table.shape[0]
+    dev = _device(page_table, lens, refs, k, v, lens if new_lens is None else new_lens)
+    n = lens.shape[0]
     status = lens.new_empty((1,))
     if workspace is None:
         workspace = lens.new_empty((lib().rai_gpu_kv_resize_workspace_bytes(n),), dtype=torch.uint8)
@@ -332,7 +332,7 @@ def compact(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, k:
     pool has to be in page_table. Returns the number of pages in use, int32
     [1] on the device."""
     pool, page = _pool(k, v)
-    dev = _device(("page_table", page_table), ("lens", lens), ("refs", refs), ("k", k), ("v", v))
+    dev = _device(page_table, lens, refs, k, v)
     used = refs.new_empty((1,))
     if workspace is None:
         workspace = refs.new_empty((lib().rai_gpu_kv_compact_workspace_bytes(refs.shape[0]),), dtype=torch.uint8)
@@ -347,7 +347,7 @@ def copy_pages(k: torch.Tensor, v: torch.Tensor, src: torch.Tensor, dst: torch.T
     """Copy page src[i] to page dst[i] in every layer (rai_gpu_kv_copy_pages).
     No destination may occur twice or be a source."""
     pool, _ = _pool(k, v)
-    dev = _device(("k", k), ("v", v), ("src", src), ("dst", dst))
+    dev = _device(k, v, src, dst)
     n = src.shape[0]
     _launch(dev, lib().rai_gpu_kv_copy_pages, pool, _ints("src", src, n), _ints("dst", dst, n), n)
 
