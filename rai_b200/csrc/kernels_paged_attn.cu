@@ -98,7 +98,7 @@ struct Cfg {
   static constexpr int kRowB = HD * kElt;
   static constexpr int NT = DT == kF32 ? (HD >= 128 ? 32 : 64) : HD == 64 ? 128 : 64;
   static constexpr int kTileB = NT * kRowB;
-  static constexpr int kStages = HD == 256 ? 2 : 3;
+  static constexpr int kStages = HD == 256 || (DT == kF32 && HD == 64) ? 2 : 3;
   static constexpr int WM = MT / 16, WN = 4 / WM, NTW = NT / WN;
   static constexpr bool kQReg = DT != kF32 && HD <= 128;  // query fragments stay in registers
   static constexpr int kQB = kQReg ? 0 : MT * kRowB;
@@ -170,13 +170,11 @@ __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo with both in tf32, hi rounded to nearest (lo is exact before
-// its own rounding). A value that is not finite stays whole in hi.
+// x = hi + lo with both in tf32: hi the upper 19 bits, lo the rest (exact),
+// rounded by the half step added below the bits that the tensor core reads.
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-  const float rest = x - __uint_as_float(hi);
-  const float r = fabsf(rest) <= 3.4e38f ? rest : 0.f;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(r));
+  hi = __float_as_uint(x) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi)) + 0x1000u;
 }
 // d += a b of f32 operands: the small products first.
 __device__ __forceinline__ void mma8x3(float (&d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], float b0, float b1) {
@@ -228,16 +226,25 @@ __global__ void __launch_bounds__(kThreads)
   }
   pdl_wait_prior();
   pdl_launch_dependents();
-  const Range rg = plan<MT, NT, kThreads>(p, blockIdx.x, sh);  // (with barriers of the CTA)
+  Range rg;
+  Cursor<MT, NT> ld;
+  if (p.direct) {
+    ld.unit = blockIdx.x / ch.nkv, ld.head = blockIdx.x - ld.unit * ch.nkv;
+    ld.it = item_of<MT, NT>(p, ld.unit);
+    ld.tile = 0, ld.pos = 0;
+    rg.begin = 0, rg.end = ld.it.tiles;
+    if (TMA) __syncthreads();
+  } else {
+    rg = plan<MT, NT, kThreads>(p, blockIdx.x, sh);  // (with barriers of the CTA)
+  }
   const long long begin = rg.begin, end = rg.end;
   if (begin >= end) {
     if (threadIdx.x == 0 && !p.whole) reinterpret_cast<Cut*>(p.a.part)[blockIdx.x] = Cut{};
     return;
   }
 
-  Cursor<MT, NT> ld, cur;
-  ld.seek(p, rg);
-  cur = ld;
+  if (!p.direct) ld.seek(p, rg);
+  Cursor<MT, NT> cur = ld;
   if (threadIdx.x == 0 && !p.whole) leave_cut<MT, NT>(p, rg, cur, blockIdx.x);
   uint32_t loaded = 0, done = 0;  // tiles
   TilePages<NT> pages;
@@ -679,6 +686,9 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
   p.min_tiles = p.whole ? 1 : kMinTiles;
   p.item_cost = kItemCost;
   p.grid = device_sm_count() * resident_ctas<C>();
+  const long long items = (long long)a.c.n_seqs * p.row_tiles * a.c.nkv;
+  p.direct = p.whole && items <= 2ll * p.grid;  // no need to share them out
+  if (p.direct) p.grid = (int)items;
   p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
   KvMaps maps;
   const int box = tma_box((int)a.c.page.d, C::NT);

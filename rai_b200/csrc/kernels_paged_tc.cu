@@ -70,9 +70,12 @@ struct Tc {
 };
 
 constexpr float kLazy = 8.f;  // log2 units
-// Few rows and heads wider than 64: from how many tokens a sequence can have
-// this kernel is the faster one.
-constexpr long long kTcFewRowsTokens = 1536;
+// Few rows and heads wider than 64: from how many tokens a sequence, and a
+// call's sequences and KV heads together, can have this kernel is the faster
+// one. (8 KV heads of 128: 256 x 1,000 tokens 328 us here and 404 us on
+// mma.sync, 16 x 2,000 73 / 83, 1 x 16,000 56 / 61; 64 x 1,000 134 / 136,
+// 256 x 300 167 / 162, 1 x 1,500 52 / 42. Heads of 64, 64 x 8,000: 233 / 120.)
+constexpr long long kTcFewRowsTokens = 768, kTcFewRowsTotal = 131072;
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -131,7 +134,7 @@ __device__ __forceinline__ bool look_through(uint32_t base, int t0, const Item& 
   constexpr int kChunks = C::HD / 8, kRowsPer = kProducers / kChunks;
   const int chunk = tid % kChunks, r0 = tid / kChunks;
   bool bad = false;
-#pragma unroll 4
+#pragma unroll 8
   for (int i = 0; i < C::NT / kRowsPer; ++i) {
     const int row = r0 + i * kRowsPer;
     bad |= clean_chunk<C::DT>(base + tile_at(C::NT, row, chunk), t0 + row, it);
@@ -414,7 +417,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (i >= (uint32_t)C::kSlots) i -= C::kSlots, phase ^= 1;
           }
         } ks = {0, 0}, vs = {1, 0};
-        bool ok = true;
+        // (A range may hold nothing but the beginning of an item's cost.)
+        Cursor<MT, NT> start;
+        start.seek(p, rg);
+        bool ok = start.pos < end;
         int items = 0;
         uint32_t k = 0;
         auto qk = [&](int half) {
@@ -437,7 +443,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if constexpr (!DUO) {
           bool first = true;  // tile k is its item's first here
           uint32_t now = 0, next = 0;
-          ok = wait_bar(&q_full[0], 0, err) && wait_bar(&kv_full[0], 0, err);
+          ok = ok && wait_bar(&q_full[0], 0, err) && wait_bar(&kv_full[0], 0, err);
           if (ok) {
             fence_after();
             next = flags[0];
@@ -590,16 +596,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               }
             }
             const float mc = (m == -INFINITY ? 0.f : m * p.c) - C::kPShift;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+            const float2 cc = {p.c, p.c}, nm = {-mc, -mc};
 #pragma unroll
             for (int x = 0; x < 64; ++x) {
-              const float a = exp2_fast(fmaf(__uint_as_float(v[2 * x]), p.c, -mc));
-              const float b = exp2_fast(fmaf(__uint_as_float(v[2 * x + 1]), p.c, -mc));
-              sum[x & 1] += a;
-              sum[2 + (x & 1)] += b;
-              v[x] = pack<DT>(a, b);
+              const float2 y = fma2({__uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1])}, cc, nm);
+              const float2 e = {exp2_fast(y.x), exp2_fast(y.y)};
+              sum[x & 1] = add2(sum[x & 1], e);
+              v[x] = pack<DT>(e.x, e.y);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             tm_st32(ts, v);
             tm_st32(ts + 32, v + 32);
             tm_wait_st();
@@ -754,9 +760,12 @@ cudaError_t launch(const AttnArgs& a, const KvMaps& maps, int box, cudaStream_t 
   p.row_tiles_div = FastDiv(p.row_tiles);
   p.group_div = FastDiv(a.group);
   p.grid = device_sm_count();
-  p.whole = false;
-  p.min_tiles = C::DUO ? 6 : 8;
-  p.item_cost = C::DUO ? 2 : 3;
+  p.whole = p.direct = false;
+  p.min_tiles = 10;
+  // An item costs about 11 us beside its tiles of 1.85 us (64 KB of K and V):
+  // prompts of 8,192 tokens take 700 / 624 / 621 / 638 us at 3 / 5 / 7 / 10.
+  // (Capped scores make the tiles twice as dear.)
+  p.item_cost = CAP ? 3 : 6;
   p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
   // Not launched ahead of its predecessor's end: a batch of prompts takes 344
   // us so and 357 us with it (long verification: 165 either way).
@@ -782,7 +791,9 @@ cudaError_t choose(const AttnArgs& a, cudaStream_t s) {
 bool paged_attention_tc_takes(const AttnArgs& a) {
   if (a.dtype == kF32 || a.c.hd > 128) return false;
   if ((long long)a.c.max_rows * a.group > 64) return true;
-  return a.c.hd > 64 && tma_box((int)a.c.page.d, 128) && (long long)a.c.max_pages * a.c.page.d >= kTcFewRowsTokens;
+  const long long tokens = (long long)a.c.max_pages * a.c.page.d;
+  return a.c.hd > 64 && tma_box((int)a.c.page.d, 128) && tokens >= kTcFewRowsTokens &&
+         tokens * a.c.n_seqs * a.c.nkv >= kTcFewRowsTotal;
 }
 
 size_t paged_attention_tc_workspace(const AttnArgs& a) {

@@ -134,6 +134,7 @@ size_t rai_gpu_paged_attention_workspace_bytes(const rai_paged_attention* a) {
   rai::AttnArgs o;
   o.c.hd = (int)a->chunk.head_dim, o.c.max_rows = (int)a->chunk.max_rows;
   o.c.max_pages = (int)a->chunk.max_pages, o.c.page.d = a->chunk.page_size;
+  o.c.n_seqs = (int)a->chunk.n_seqs, o.c.nkv = (int)a->chunk.n_kv_heads;
   o.group = (int)(a->n_heads / a->chunk.n_kv_heads);
   o.dtype = (int)a->chunk.dtype;
   return rai::paged_attention_workspace(o);

@@ -21,7 +21,8 @@ constexpr int kPlanWords = 22;
 struct Params {
   AttnArgs a;
   int row_tiles, min_tiles, item_cost, grid;
-  bool whole;  // items are short: none is cut
+  bool whole;   // items are short: none is cut
+  bool direct;  // one CTA per item, in order
   float c;  // log2(e) * scale, or log2(e) when the scores are capped
   FastDiv row_tiles_div, group_div;
 };
@@ -140,7 +141,7 @@ struct Cursor {
   }
   __device__ __forceinline__ void next(const Params& p) {
     ++pos;
-    if (++tile < it.tiles) return;
+    if (++tile < it.tiles || p.direct) return;
     tile = 0;
     pos += p.item_cost;
     if (++head < p.a.c.nkv) return;
@@ -201,9 +202,9 @@ __device__ __forceinline__ uint32_t tile_at(int rows, int row, int chunk) {
 __device__ __forceinline__ bool try_bar(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
       : "=r"(ok)
-      : "r"(bar), "r"(parity), "r"(500u)  // ns
+      : "r"(bar), "r"(parity)
       : "memory");
   return ok != 0;
 }
@@ -243,6 +244,13 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
   }
 }
 
+// Whether a word holds an element that is not finite: its magnitude's bits plus
+// the exponent's unit reach the sign bit. (The bits of interest, not a flag.)
+template <int DT>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  if constexpr (DT == kF32) return ((w & 0x7fffffffu) + 0x00800000u) & 0x80000000u;
+  else return ((w & 0x7fff7fffu) + (DT == kBF16 ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+}
 // Replaces the values of one 16-byte chunk of a V tile that are not finite by
 // zero; whether there were any in a token that some row sees (t: the chunk's
 // token). Slots outside that range may hold anything.
@@ -250,8 +258,8 @@ template <int DT>
 __device__ __forceinline__ bool clean_chunk(uint32_t ad, int t, const Item& it) {
   uint4 w;
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(ad));
+  if (!(not_finite<DT>(w.x) | not_finite<DT>(w.y) | not_finite<DT>(w.z) | not_finite<DT>(w.w))) return false;
   const uint4 f = make_uint4(finite_or_zero<DT>(w.x), finite_or_zero<DT>(w.y), finite_or_zero<DT>(w.z), finite_or_zero<DT>(w.w));
-  if (f.x == w.x && f.y == w.y && f.z == w.z && f.w == w.w) return false;
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(ad), "r"(f.x), "r"(f.y), "r"(f.z), "r"(f.w) : "memory");
   return t >= it.lo && t < it.hi;
 }
@@ -355,6 +363,22 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 template <int DT>
 __device__ __forceinline__ float capped(float s, float scale, float cap) {

@@ -136,10 +136,11 @@ def _chunk(k_pages, v_pages, table, kv_len, q_start, rows: int, max_rows: int, d
 
 
 @functools.lru_cache(maxsize=1024)
-def _attn_workspace(dev: int, dtype: int, hd: int, nkv: int, heads: int, max_rows: int, max_pages: int, page: int) -> int:
+def _attn_workspace(dev: int, dtype: int, hd: int, nkv: int, heads: int, max_rows: int, max_pages: int, page: int,
+                    seqs: int) -> int:
     a = native.PagedAttention()
     a.chunk.dtype, a.chunk.head_dim, a.chunk.n_kv_heads, a.chunk.max_rows = dtype, hd, nkv, max_rows
-    a.chunk.max_pages, a.chunk.page_size = max_pages, page
+    a.chunk.max_pages, a.chunk.page_size, a.chunk.n_seqs = max_pages, page, seqs
     a.n_heads = heads
     with torch.cuda.device(dev):
         return native.lib().rai_gpu_paged_attention_workspace_bytes(C.byref(a))
@@ -148,7 +149,7 @@ def _attn_workspace(dev: int, dtype: int, hd: int, nkv: int, heads: int, max_row
 def attention_workspace_bytes(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor, max_rows: int) -> int:
     """Bytes of the workspace that `attention` takes for these arguments."""
     return _attn_workspace(q.get_device(), _dtype(k_pages, "k_pages"), k_pages.shape[3], k_pages.shape[1], q.shape[1],
-                           min(max_rows, q.shape[0]), page_table.shape[1], k_pages.shape[2])
+                           min(max_rows, q.shape[0]), page_table.shape[1], k_pages.shape[2], page_table.shape[0])
 
 
 def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -189,7 +190,7 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
         lse_at = lse.data_ptr()
     ws_at = ws_bytes = 0
     if workspace is None:
-        need = _attn_workspace(dev, dtype, hd, chunk[16], heads, max_rows, chunk[13], chunk[15])
+        need = _attn_workspace(dev, dtype, hd, chunk[16], heads, max_rows, chunk[13], chunk[15], chunk[12])
         if need:
             workspace = q.new_empty((need,), dtype=torch.uint8)
             ws_at, ws_bytes = workspace.data_ptr(), need

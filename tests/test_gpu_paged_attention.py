@@ -56,7 +56,7 @@ def make_q(T, H, D, dtype, dev, seed=1, scale=1.0):
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("heads,nkv,hd", [(14, 2, 64), (32, 8, 128), (4, 4, 32), (6, 2, 96), (15, 5, 80), (4, 2, 256),
                                           (8, 1, 16), (5, 1, 136)])
-@pytest.mark.parametrize("wide", [0, 150])
+@pytest.mark.parametrize("wide", [0, 2000])
 def test_shapes_and_lengths(dtype, heads, nkv, hd, wide):
     """A table for longer sequences than there are (wide) may choose another
     kernel."""
@@ -76,8 +76,9 @@ def test_shapes_and_lengths(dtype, heads, nkv, hd, wide):
 def test_pages_caps_and_windows(dtype, page, softcap, window, rows):
     dev = torch.device("cuda", 0)
     lens = [3, 300, 130, 140]
-    c = ref.Cache(lens, 2, 64, page, dtype, dev, seed=page, wide=1 + 2000 // page)
-    q = make_q(sum(rows), 6, 64, dtype, dev, scale=2.0)
+    hd = 64 if sum(rows) > 50 else 128
+    c = ref.Cache(lens, 2, hd, page, dtype, dev, seed=page, wide=1 + 40000 // page)
+    q = make_q(sum(rows), 6, hd, dtype, dev, scale=2.0)
     got, lse = run(c, q, rows, softcap=softcap, window=window)
     agree(c, q, rows, got, lse, softcap=softcap, window=window)
 
@@ -112,7 +113,7 @@ def test_few_long_sequences_are_cut(dtype, rows, lens):
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("rows", [[5, 3, 150, 200], [5, 3, 40, 7]], ids=["many", "few"])
-@pytest.mark.parametrize("wide", [0, 150])
+@pytest.mark.parametrize("wide", [0, 2000])
 def test_rows_that_see_nothing(dtype, hd, rows, wide):
     """kv_len below the row count: the first rows stand before the sequence."""
     dev = torch.device("cuda", 0)
@@ -127,7 +128,7 @@ def test_rows_that_see_nothing(dtype, hd, rows, wide):
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("rows,window", [(6, 0), (6, 40), (160, 0), (300, 90)])
-@pytest.mark.parametrize("wide", [0, 100])
+@pytest.mark.parametrize("wide", [0, 10000])
 def test_what_is_masked_does_not_matter(dtype, hd, rows, window, wide):
     """NaN and infinities in later tokens, in tokens behind the window, in
     unused slots: only rows that see them change."""
