@@ -553,29 +553,6 @@ __global__ void __launch_bounds__(kThreads)
       }
       if (wn == 0) {
         const long long item_at = cur.pos - cur.tile;  // of its first tile
-        if (poison) {
-          // Rows that see a V value which is not finite get it after all.
-          const int ta = it.first * NT + (int)max(0ll, begin - item_at) * NT, tb = (it.first + cur.tile + 1) * NT;
-          for (int t = max(ta, it.lo); t < min(tb, it.hi); ++t) {
-            const int tt = t / NT * NT;
-            if (!(tt + NT - 1 > plo || tt < it.lo || (p.a.window > 0 && tt <= phi - p.a.window))) continue;
-            const int pi = (int)ch.page.quot(t), page = page_of(ch, it.seq, pi);
-            if (page < 0) continue;
-            const long long vo = page * ch.v_page + (long long)cur.head * ch.v_head + (t - pi * (int)ch.page.d) * ch.v_slot;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (t > pos[h] || (p.a.window > 0 && t <= pos[h] - p.a.window)) continue;
-#pragma unroll
-              for (int x = 0; x < HD / 8; ++x)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int col = x * 8 + 2 * t4 + e;
-                  const float v = col < ch.hd ? value<DT>(ch.v, vo + col) : 0.f;
-                  if (!(fabsf(v) <= 3.4028235e38f)) acc[x][2 * h + e] += v;
-                }
-            }
-          }
-        }
         const bool whole = item_at >= begin && cur.last_of_item();
         if (whole) {
 #pragma unroll
@@ -610,6 +587,27 @@ __global__ void __launch_bounds__(kThreads)
             if (t4 == 0) {
               part[MT * HD + r] = m[h] == -INFINITY ? -INFINITY : m[h] * p.c;
               part[MT * HD + MT + r] = l[h];
+            }
+          }
+        }
+        if (poison) {
+          // Rows that see a V value which is not finite get it after all.
+          const int ta = it.first * NT + (int)max(0ll, begin - item_at) * NT, tb = (it.first + cur.tile + 1) * NT;
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            const int r = wm * 16 + g + 8 * h, f = it.f0 + r, i = (int)p.group_div.quot(f), at = h ? pos[1] : pos[0];
+            if (r >= it.nf) continue;
+            const int from = max(max(ta, it.lo), p.a.window > 0 ? at - p.a.window + 1 : 0), till = min(min(tb, it.hi), at + 1);
+            const long long o = (long long)(it.start + i) * p.a.o_row + (long long)(cur.head * p.a.group + f - i * p.a.group) * p.a.o_head;
+#pragma unroll 1
+            for (int x = 0; x < HD / 4; ++x) {
+              const int col = (x >> 1) * 8 + 2 * t4 + (x & 1);
+              if (col >= ch.hd) continue;
+              const float v = lost_values<DT, NT>(p, it, cur.head, col, from, till);
+              if (v != 0.f) {
+                if (whole) put<DT>(p.a.out, o + col, v);
+                else part_of(p, C::kPartFloats, blockIdx.x, first_slot)[r * HD + col] = v;
+              }
             }
           }
         }

@@ -678,28 +678,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     o[y] = __float_as_uint(w);
                   }
                 }
-                if (poisoned && real) {
-                  // A row that sees a V value which is not finite gets it after all.
-                  const int ta = it.first * NT + (int)max(0ll, begin - item_at) * NT, tb = (it.first + cur.tile + 1) * NT;
-                  const int from = max(max(ta, it.lo), p.a.window > 0 ? pos - p.a.window + 1 : 0), till = min(min(tb, it.hi), pos + 1);
-                  for (int t = from; t < till; ++t) {
-                    if (!tile_masked(it, t / NT * NT, NT, p.a.window, p.group_div)) continue;
-                    const int pi = (int)ch.page.quot(t), page = page_of(ch, it.seq, pi);
-                    if (page < 0) continue;
-                    const long long vo = page * ch.v_page + (long long)cur.head * ch.v_head + (t - pi * (int)ch.page.d) * ch.v_slot;
-#pragma unroll
-                    for (int y = 0; y < 32; ++y) {
-                      const float w = x + y < ch.hd ? value<DT>(ch.v, vo + x + y) : 0.f;
-                      if (!(fabsf(w) <= 3.4028235e38f)) o[y] = __float_as_uint(__uint_as_float(o[y]) + w);
-                    }
-                  }
-                }
-                if (!real) continue;
-                if (!whole) {
+                if (real && !whole) {
 #pragma unroll
                   for (int y = 0; y < 32; y += 4)
                     *reinterpret_cast<uint4*>(part + r * HD + x + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
-                } else {
+                } else if (real) {
 #pragma unroll
                   for (int y = 0; y < 32; y += 8) {
                     uint32_t w[4];
@@ -707,6 +690,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int z = 0; z < 4; ++z)
                       w[z] = pack<DT>(__uint_as_float(o[y + 2 * z]) * inv, __uint_as_float(o[y + 2 * z + 1]) * inv);
                     if (x + y < ch.hd) *reinterpret_cast<uint4*>(out + x + y) = make_uint4(w[0], w[1], w[2], w[3]);
+                  }
+                }
+              }
+              if (poisoned && real) {
+                // A row that sees a V value which is not finite gets it after all.
+                const int ta = it.first * NT + (int)max(0ll, begin - item_at) * NT, tb = (it.first + cur.tile + 1) * NT;
+                const int from = max(max(ta, it.lo), p.a.window > 0 ? pos - p.a.window + 1 : 0), till = min(min(tb, it.hi), pos + 1);
+#pragma unroll 1
+                for (int col = 0; col < ch.hd; ++col) {
+                  const float v = lost_values<DT, NT>(p, it, cur.head, col, from, till);
+                  if (v != 0.f) {
+                    if (whole) put<DT>(out, col, v);
+                    else part[r * HD + col] = v;
                   }
                 }
               }

@@ -391,6 +391,30 @@ __device__ __forceinline__ float capped(float s, float scale, float cap) {
     return cap * (1.f - __fdividef(2.f, 1.f + exp2_fast(2.f * kLog2e * x)));
   }
 }
+// The V values of column `col` that are not finite among the tokens [from,
+// till) of the item's masked tiles, added up; 0: there are none. (The tiles'
+// copies of them were zeroed, so that they do not reach rows that may not see
+// them; the rows that do get them here.)
+template <int DT, int NT>
+__device__ __noinline__ float lost_values(const Params& p, const Item it, int kv_head, int col, int from, int till) {
+  const PagedChunk& c = p.a.c;
+  float sum = 0.f;
+  for (int t = from; t < till; ++t) {
+    if (!tile_masked(it, t / NT * NT, NT, p.a.window, p.group_div)) continue;
+    const int pi = (int)c.page.quot(t), page = page_of(c, it.seq, pi);
+    if (page < 0) continue;
+    const float v = value<DT>(c.v, page * c.v_page + (long long)kv_head * c.v_head + (t - pi * (int)c.page.d) * c.v_slot + col);
+    if (!(fabsf(v) <= 3.4028235e38f)) sum += v;
+  }
+  return sum;
+}
+template <int DT>
+__device__ __forceinline__ void put(void* base, long long i, float v) {
+  if constexpr (DT == kF32) static_cast<float*>(base)[i] = v;
+  else if constexpr (DT == kF16) static_cast<__half*>(base)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(v);
+}
+
 // What a CTA of the main kernel leaves for the join: whether the cut at its
 // first tile is the first one through an item, and that item.
 struct Cut {
