@@ -301,22 +301,24 @@ __global__ void __launch_bounds__(256) kv_fork_kernel(TableArgs in, TableArgs ou
   }
 }
 
-__device__ __forceinline__ int block_scan(int v, int* sh, int* total) {  // exclusive, kMetaThreads threads
+// Exclusive sum over kMetaThreads threads; in 64 bits, since many sequences can
+// ask for more pages than 32 bits count.
+__device__ __forceinline__ long long block_scan(long long v, long long* sh, long long* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int incl = v;
+  long long incl = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(~0u, incl, o);
+    const long long u = __shfl_up_sync(~0u, incl, o);
     if (lane >= o) incl += u;
   }
   __syncthreads();
   if (lane == 31) sh[warp] = incl;
   __syncthreads();
   if (warp == 0) {
-    int w = sh[lane];
+    long long w = sh[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(~0u, w, o);
+      const long long u = __shfl_up_sync(~0u, w, o);
       if (lane >= o) w += u;
     }
     sh[lane] = w;
@@ -386,6 +388,7 @@ __global__ void __launch_bounds__(kMetaThreads) kv_resize_kernel(TableArgs t, co
   __shared__ int tail[kMaxTableSeqs];   // page to copy on write, or -1
   __shared__ int place[kMaxTableSeqs];  // exclusive sum of the pages that sequences take
   __shared__ int sh[32];
+  __shared__ long long wide[32];
   pdl_wait_prior();
   const int n = t.n_seqs, ps = t.page_size;
   const int cap = (int)min((long long)t.max_pages * ps, (long long)(INT_MAX - 1024));
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(kMetaThreads) kv_resize_kernel(TableArgs t, co
     if (s < n) place[s] = copies;
   }
   __syncthreads();
-  int sum = 0;
+  long long sum = 0;
   const int per = (n + kMetaThreads - 1) / kMetaThreads;
   const int s0 = min(n, (int)threadIdx.x * per), s1 = min(n, s0 + per);
   for (int s = s0; s < s1; ++s) {
@@ -439,11 +442,12 @@ __global__ void __launch_bounds__(kMetaThreads) kv_resize_kernel(TableArgs t, co
     else place[s] = 0;
     sum += place[s];
   }
-  int total;
-  int at = block_scan(sum, sh, &total);
+  long long total;
+  long long at = block_scan(sum, wide, &total);
+  // (Where the sum passes 32 bits nothing is given, and place is not read.)
   for (int s = s0; s < s1; ++s) {
     const int c = place[s];
-    place[s] = at;
+    place[s] = (int)at;
     at += c;
   }
   // Free pages, in order: each warp looks at a run of the counts, 32 at a
@@ -457,7 +461,7 @@ __global__ void __launch_bounds__(kMetaThreads) kv_resize_kernel(TableArgs t, co
   __shared__ int count;
   if (threadIdx.x == 0) {
     count = 0;
-    *status = fits ? 0 : total - free_total;
+    *status = fits ? 0 : (int)min(total - free_total, (long long)INT_MAX);
   }
   __syncthreads();
   if (fits && total > 0) {

@@ -73,6 +73,12 @@ int check_heads(uint32_t heads, const rai::PagedChunk& c) {
   return RAI_OK;
 }
 
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + nb && y < x + na;
+}
+size_t table_bytes(const rai_page_table& t) { return ((size_t)(t.n_seqs - 1) * t.table_stride + t.max_pages) * 4; }
+
 int attention_args(const rai_paged_attention* a, rai::AttnArgs* out) {
   if (!a || !a->q || !a->out) return bad("null argument");
   rai::AttnArgs o;
@@ -82,6 +88,8 @@ int attention_args(const rai_paged_attention* a, rai::AttnArgs* out) {
   if (!vec_stride(a->q_row, elt) || !vec_stride(a->q_head, elt) || !vec_stride(a->out_row, elt) ||
       !vec_stride(a->out_head, elt) || !aligned(a->q, 16) || !aligned(a->out, 16))
     return bad("q, out: every vector has to start on a 16-byte boundary");
+  if ((uint64_t)a->chunk.n_seqs * (((uint64_t)a->chunk.max_rows * (a->n_heads / a->chunk.n_kv_heads) + 15) / 16) > (1u << 30))
+    return bad("n_seqs * max_rows is out of range");
   if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return bad("scale has to be positive");
   if (!(a->softcap >= 0.f) || !std::isfinite(a->softcap)) return bad("softcap");
   if (a->window > (1u << 30)) return bad("window");
@@ -225,7 +233,9 @@ int rai_gpu_kv_fork(const rai_page_table* in, const rai_page_table* out, const i
     if (a.refs != b.refs || a.n_pages != b.n_pages || a.page_size != b.page_size)
       return bad("fork: both tables have to be of one pool");
     if (b.max_pages < a.max_pages) return bad("fork: the new table is narrower than the old one");
-    if (a.table == b.table || a.lens == b.lens) return bad("fork: the new table and lengths need their own memory");
+    if (overlap(in->table, table_bytes(*in), out->table, table_bytes(*out)) ||
+        overlap(in->lens, in->n_seqs * 4ull, out->lens, out->n_seqs * 4ull))
+      return bad("fork: the new table and lengths need their own memory");
     if (int rc = rai::kernel_status_word(&a.err)) return rc;
     b.err = a.err;
     return done(rai::kv_fork(a, b, parents, static_cast<cudaStream_t>(stream)));
@@ -306,7 +316,11 @@ int rai_gpu_beam_select(const rai_beam_select* a, void* stream) {
     if (a->history) {
       if (!a->hist_len || !a->out_history || !a->out_len) return bad("null argument");
       if (!a->hist_cap || a->hist_stride < a->hist_cap || a->out_hist_stride < a->hist_cap) return bad("history strides");
-      if (a->out_history == a->history || a->out_len == a->hist_len) return bad("the new histories need their own memory");
+      const uint64_t rows = (uint64_t)a->batch * a->beams;
+      if (overlap(a->history, ((rows - 1) * a->hist_stride + a->hist_cap) * 4, a->out_history,
+                  ((rows - 1) * a->out_hist_stride + a->hist_cap) * 4) ||
+          overlap(a->hist_len, rows * 4, a->out_len, rows * 4))
+        return bad("the new histories need their own memory");
       o.history = a->history, o.hist_len = a->hist_len, o.out_history = a->out_history, o.out_len = a->out_len;
       o.hist_stride = a->hist_stride, o.out_stride = a->out_hist_stride, o.hist_cap = (int)a->hist_cap;
       if (a->hist_cap > (1u << 30)) return bad("history strides");
