@@ -139,28 +139,30 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(BeamArgs a, int
   // Vector slots from the 16-byte boundary at or before the slice's start.
   const int off = (int)((reinterpret_cast<uintptr_t>(src + (long long)begin * kE) & 15) / kE);
   const int base = begin - off;
+  constexpr int kStep = kThreads * N;
   if (threadIdx.x == 0) count = 0;
   float m = -INFINITY;
   double sum = 0.0;
   uint64_t bar = 0;  // keys at or above it are kept
+  float bar_x = -INFINITY;
   auto first_of = [&](int at, int u) { return at + (u * kThreads + (int)threadIdx.x) * V; };
+  auto inside = [&](int at) { return at >= begin && at + kStep <= end; };  // the step is whole
   auto fetch = [&](int at, uint4 (&w)[kVecs]) {  // whole vectors only
+    const bool all = inside(at);
 #pragma unroll
     for (int u = 0; u < kVecs; ++u) {
       const int e0 = first_of(at, u);
-      if (e0 >= begin && e0 + V <= end) w[u] = __ldcs(reinterpret_cast<const uint4*>(src + (long long)e0 * kE));
+      if (all || (e0 >= begin && e0 + V <= end)) w[u] = __ldcs(reinterpret_cast<const uint4*>(src + (long long)e0 * kE));
     }
   };
-  uint4 w[kVecs];
-  fetch(base, w);
-  __syncthreads();
-  for (int at = base; at < end; at += kThreads * N) {
-    float x[N];
-    uint32_t there = 0;  // bit per element
+  // The step's elements; bit per element that is there.
+  auto take = [&](int at, const uint4 (&w)[kVecs], float (&x)[N]) -> uint32_t {
+    const bool all = inside(at);
+    uint32_t there = 0;
 #pragma unroll
     for (int u = 0; u < kVecs; ++u) {
       const int e0 = first_of(at, u);
-      if (e0 >= begin && e0 + V <= end) {
+      if (all || (e0 >= begin && e0 + V <= end)) {
         const uint32_t ws[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -180,90 +182,129 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(BeamArgs a, int
         }
       }
     }
-    if (at + kThreads * N < end) fetch(at + kThreads * N, w);  // in flight through this step
-    float top = -INFINITY;
+    return there;
+  };
+  // Elements of `among` at or above the bar go to the buffer; the ones that
+  // find it full come back.
+  auto push = [&](int at, const float (&x)[N], uint32_t among) -> uint32_t {
+    uint32_t full = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) top = fmaxf(top, x[i]);  // (elements that are not there are -inf)
-    if (there) {
-      if (top > m) {
-        sum *= (double)weight(m, top);
-        m = top;
-      }
-      // Pairs: (x - m) log2(e), exponentials, sums.
-      float2 part[2] = {{0.f, 0.f}, {0.f, 0.f}};
-      const float2 mm = {-m, -m};
-#pragma unroll
-      for (int i = 0; i < N; i += 2) part[i / 2 & 1] = add2(part[i / 2 & 1], exp2_of(mul2(add2({x[i], x[i + 1]}, mm), {kLog2e, kLog2e})));
-      float all = (part[0].x + part[0].y) + (part[1].x + part[1].y);
-      if (!(fabsf(m) <= 3.4028235e38f) || !(all == all)) {
-        // An infinite maximum, or a NaN among them, which is not chosen.
-        all = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          if (!(x[i] == x[i])) x[i] = -INFINITY;
-          if (there >> i & 1u) all += weight(x[i], m);
+    for (int i = 0; i < N; ++i)
+      if (x[i] >= bar_x && (among >> i & 1u)) {
+        const uint64_t k = key_of(x[i], first_of(at, i / V) + i % V);
+        if (k >= bar) {
+          const int slot = atomicAdd(&count, 1);
+          if (slot < kBufCap) buf[slot] = k;
+          else full |= 1u << i;
         }
       }
-      sum += (double)all;
-    }
-    if (at == base) {
-      // A first bar: the keep-th largest of the best of 64 groups of four
-      // threads is no larger than the keep-th largest element.
-      uint64_t best = 0;
+    return full;
+  };
+  // Cut the buffer's first n to the keep best, which raises the bar.
+  auto cut = [&](int n) {
+    prune(buf, n, a.keep);
+    bar = n >= a.keep ? buf[a.keep - 1] : 0;
+    bar_x = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
+    if (threadIdx.x == 0) count = min(n, a.keep);
+    __syncthreads();
+  };
+  uint4 w[kVecs];
+  fetch(base, w);
+  __syncthreads();
+  // Rounds of kRound steps without a barrier: a buffer that overflows within
+  // one (rising logits, many equal ones) is put back to where it was and the
+  // round's elements are pushed again with a barrier each step.
+  constexpr int kRound = 4;
+  int held = 0;  // in the buffer at the round's start
+  for (int r0 = base; r0 < end; r0 += kRound * kStep) {
+    const int stop = min(end, r0 + kRound * kStep);
+    for (int at = r0; at < stop; at += kStep) {
+      float x[N];
+      const uint32_t there = take(at, w, x);
+      if (at + kStep < end) fetch(at + kStep, w);  // in flight through this step
+      float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if ((there >> i & 1u) && x[i] == top) best = max(best, key_of(x[i], first_of(at, i / V) + i % V));
-      best = max(best, __shfl_xor_sync(~0u, best, 1));
-      best = max(best, __shfl_xor_sync(~0u, best, 2));
-      if ((threadIdx.x & 3) == 0) tops[threadIdx.x >> 2] = best;
-      __syncthreads();
-      if (threadIdx.x < kMaxKeep) {
-        const uint64_t k = tops[threadIdx.x];
-        int rank = 0;
-#pragma unroll 8
-        for (int i = 0; i < kMaxKeep; ++i) rank += tops[i] > k || (tops[i] == k && i < (int)threadIdx.x);
-        if (rank == a.keep - 1) tops[kMaxKeep] = k;
-      }
-      __syncthreads();
-      bar = tops[kMaxKeep];
-    }
-    // Elements at or above the bar go to the buffer; whenever it fills up it
-    // is cut to the keep best, which raises the bar.
-    uint32_t pending = 0;  // elements that found the buffer full
-    float bar_x = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
-    auto push = [&](uint32_t among) {
+      for (int i = 0; i < N; ++i) top = fmaxf(top, x[i]);  // (elements that are not there are -inf)
+      if (there) {
+        if (top > m) {
+          sum *= (double)weight(m, top);
+          m = top;
+        }
+        // Pairs: (x - m) log2(e), exponentials, sums.
+        float2 part[2] = {{0.f, 0.f}, {0.f, 0.f}};
+        const float2 mm = {-m, -m};
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (x[i] >= bar_x && (among >> i & 1u)) {
-          const uint64_t k = key_of(x[i], first_of(at, i / V) + i % V);
-          if (k >= bar) {
-            const int slot = atomicAdd(&count, 1);
-            if (slot < kBufCap) buf[slot] = k;
-            else pending |= 1u << i;
+        for (int i = 0; i < N; i += 2) part[i / 2 & 1] = add2(part[i / 2 & 1], exp2_of(mul2(add2({x[i], x[i + 1]}, mm), {kLog2e, kLog2e})));
+        float all = (part[0].x + part[0].y) + (part[1].x + part[1].y);
+        if (!(fabsf(m) <= 3.4028235e38f) || !(all == all)) {
+          // An infinite maximum, or a NaN among them, which is not chosen.
+          all = 0.f;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            if (!(x[i] == x[i])) x[i] = -INFINITY;
+            if (there >> i & 1u) all += weight(x[i], m);
           }
         }
-    };
-    if (there && top >= bar_x) push(there);
-    for (;;) {
-      const int again = __syncthreads_or(pending != 0);
-      const int n = min(count, kBufCap);
-      __syncthreads();  // everyone has read the count
-      if (again || n > a.keep + 80) {
-        prune(buf, n, a.keep);
-        bar = buf[min(n, a.keep) - 1];
-        if (n < a.keep) bar = 0;
-        if (threadIdx.x == 0) count = min(n, a.keep);
-        __syncthreads();
+        sum += (double)all;
       }
-      if (!again) break;
-      bar_x = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
-      const uint32_t rest = pending;
-      pending = 0;
-      if (rest) push(rest);
+      if (at == base) {
+        // A first bar: the keep-th largest of the best of 64 groups of four
+        // threads is no larger than the keep-th largest element.
+        uint64_t best = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if ((there >> i & 1u) && x[i] == top) best = max(best, key_of(x[i], first_of(at, i / V) + i % V));
+        best = max(best, __shfl_xor_sync(~0u, best, 1));
+        best = max(best, __shfl_xor_sync(~0u, best, 2));
+        if ((threadIdx.x & 3) == 0) tops[threadIdx.x >> 2] = best;
+        __syncthreads();
+        if (threadIdx.x < kMaxKeep) {
+          const uint64_t k = tops[threadIdx.x];
+          int rank = 0;
+#pragma unroll 8
+          for (int i = 0; i < kMaxKeep; ++i) rank += tops[i] > k || (tops[i] == k && i < (int)threadIdx.x);
+          if (rank == a.keep - 1) tops[kMaxKeep] = k;
+        }
+        __syncthreads();
+        bar = tops[kMaxKeep];
+        bar_x = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
+      }
+      if (there && top >= bar_x) push(at, x, there);
+    }
+    __syncthreads();
+    const int n = count;
+    __syncthreads();  // everyone has read the count
+    if (n > kBufCap) {
+      if (threadIdx.x == 0) count = held;
+      __syncthreads();
+      for (int at = r0; at < stop; at += kStep) {
+        uint4 v[kVecs];
+        float x[N];
+        fetch(at, v);
+        uint32_t rest = take(at, v, x);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (!(x[i] == x[i])) x[i] = -INFINITY;
+        for (int again = 1; again;) {
+          rest = push(at, x, rest);
+          again = __syncthreads_or(rest != 0);
+          const int now = min(count, kBufCap);
+          __syncthreads();
+          held = now;
+          if (again || now > kBufCap / 2) {
+            cut(now);
+            held = min(now, a.keep);
+          }
+        }
+      }
+    } else if (n > a.keep + 80 || (r0 == base && n > a.keep)) {
+      cut(n);
+      held = min(n, a.keep);
+    } else {
+      held = n;
     }
   }
-  __syncthreads();
-  const int n = min(count, kBufCap);
+  const int n = held;
   prune(buf, n, a.keep);
   // Join the threads' sums.
   float top = m;

@@ -150,3 +150,38 @@ def test_in_a_graph_and_twice_the_same():
     for a, b in zip(got[:6], second[:6]):
         assert torch.equal(a, b)
     assert not torch.equal(want.cand_scores, got.cand_scores)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_more_equal_logits_than_a_buffer_holds(dtype):
+    """Long runs of the best value, and steps that each beat the last."""
+    x = torch.zeros((2, 3, 70001), dtype=dtype)
+    x[0, 0, 9000:60000] = 3.0
+    x[0, 1] = torch.arange(70001).div(8192, rounding_mode="floor").to(dtype)
+    x[0, 2, ::2] = 1.0
+    x[1, 0, 65000:] = 2.0
+    x[1, 1] = -math.inf
+    x[1, 1, 69990:] = 1.0
+    s = torch.tensor([[0.0, -1.0, -0.5], [0.0, 0.0, 0.0]])
+    check(x.cuda(), s.cuda(), eos=9001)
+    check(x.cuda(), s.cuda(), keep=64, eos=3)
+
+
+def test_on_two_streams_at_once():
+    from rai_b200 import beams
+    xs = [torch.randn((8, 4, 50000), device="cuda") for _ in range(2)]
+    s = torch.zeros((8, 4), device="cuda")
+    want = [beams.select(x, s) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(beams.select(xs[i], s))
+    torch.cuda.synchronize()
+    for w, rs in zip(want, got):
+        for r in rs:
+            for a, b in zip(w[:6], r[:6]):
+                assert torch.equal(a, b)
