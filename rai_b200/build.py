@@ -13,6 +13,7 @@ import hashlib
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -83,6 +84,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and os.path.exists(LIB) and os.path.exists(stamp):
         with open(stamp) as fh:
             if fh.read().strip() == digest:
+                build_torch_ops(force, verbose)
                 return LIB
     bdir = os.path.join(HERE, "_build")
     os.makedirs(bdir, exist_ok=True)
@@ -103,7 +105,45 @@ def build(force: bool = False, verbose: bool = False) -> str:
     os.replace(tmp, LIB)
     with open(stamp, "w") as fh:
         fh.write(digest)
+    build_torch_ops(force, verbose)
     return LIB
+
+
+TORCH_OPS = os.path.join(HERE, "_torch_ops.so")
+
+
+def build_torch_ops(force: bool = False, verbose: bool = False) -> str | None:
+    """The extension behind rai_b200.paged and rai_b200.beams (csrc/
+    torch_ops.cpp), against the installed torch; None without torch."""
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError:
+        return None
+    src = os.path.join(CSRC, "torch_ops.cpp")
+    lib_dir = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{p}" for p in cpp_extension.include_paths("cuda")), "-I" + sysconfig.get_paths()["include"], src,
+           "-L" + HERE, "-l:librai_gpu.so", "-Wl,-rpath,$ORIGIN", "-L" + lib_dir, "-Wl,-rpath," + lib_dir,
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-ltorch"]
+    h = hashlib.sha256((torch.__version__ + " ".join(cmd)).encode())
+    for f in (src, os.path.join(ROOT, "include", "rai_gpu.h")):
+        with open(f, "rb") as fh:
+            h.update(fh.read())
+    stamp = TORCH_OPS + ".sha256"
+    if not force and os.path.exists(TORCH_OPS) and os.path.exists(stamp):
+        with open(stamp) as fh:
+            if fh.read().strip() == h.hexdigest():
+                return TORCH_OPS
+    tmp = TORCH_OPS + ".tmp"
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run([*cmd, "-o", tmp], check=True)
+    os.replace(tmp, TORCH_OPS)
+    with open(stamp, "w") as fh:
+        fh.write(h.hexdigest())
+    return TORCH_OPS
 
 
 if __name__ == "__main__":

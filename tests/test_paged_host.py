@@ -4,11 +4,12 @@ import ctypes as C
 import json
 import math
 import os
+import subprocess
 
 import numpy as np
 import pytest
 
-from conftest import GOLDEN
+from conftest import GOLDEN, ROOT
 from rai_b200 import native
 
 I = native.RAI_ERR_INVALID
@@ -158,29 +159,24 @@ def test_beams_refuse():
         assert select(**kw) == U, kw
 
 
-def test_packed_arguments_have_the_structures_layout():
-    torch = pytest.importorskip("torch")
-    from rai_b200 import beams, paged
-    for packed, struct in ((paged._ATTN, native.PagedAttention), (paged._ROPE, native.RopeAppend), (paged._TABLE, native.PageTable),
-                           (paged._POOL, native.PagePool), (beams._ARGS, native.BeamSelect)):
-        assert packed.size == C.sizeof(struct)
-        # Field by field: a number in each place comes out in its field.
-        names = []
-
-        def walk(s, prefix=""):
-            for n, t in s._fields_:
-                if issubclass(t, C.Structure):
-                    walk(t, prefix + n + ".")
-                else:
-                    names.append((prefix + n, t))
-        walk(struct)
-        values = [i + 1 for i in range(len(names))]
-        s = struct.from_buffer_copy(packed.pack(*values))
-        for (n, t), v in zip(names, values):
-            o = s
-            for part in n.split("."):
-                o = getattr(o, part)
-            assert o == v, n
+def test_structures_have_the_headers_layout(tmp_path):
+    """Size and field offsets of the ctypes structures against a C compiler's
+    reading of include/rai_gpu.h."""
+    pairs = [(native.PagedChunk, "rai_paged_chunk"), (native.PagedAttention, "rai_paged_attention"), (native.RopeAppend, "rai_rope_append"),
+             (native.PageTable, "rai_page_table"), (native.PagePool, "rai_page_pool"), (native.BeamSelect, "rai_beam_select")]
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{ROOT}/include/rai_gpu.h"', "int main(void) {"]
+    want = []
+    for py, c in pairs:
+        lines.append(f'printf("%zu\\n", sizeof({c}));')
+        want.append(C.sizeof(py))
+        for name, _ in py._fields_:
+            lines.append(f'printf("%zu\\n", offsetof({c}, {name}));')
+            want.append(getattr(py, name).offset)
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["return 0; }"]))
+    subprocess.run(["gcc", str(src), "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == want
 
 
 def test_host_tensors_are_refused():
