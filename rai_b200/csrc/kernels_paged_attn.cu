@@ -45,10 +45,10 @@ cudaError_t paged_attention_tc(const AttnArgs& a, cudaStream_t s);
 
 namespace paged_attn {
 
-bool make_maps(const PagedChunk& c, int dtype, int box, KvMaps* maps) {
-  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static Encode encoder() {
   static const Encode encode = [] {
     void* f = nullptr;
     cudaDriverEntryPointQueryResult r;
@@ -59,6 +59,25 @@ bool make_maps(const PagedChunk& c, int dtype, int box, KvMaps* maps) {
     }
     return reinterpret_cast<Encode>(f);
   }();
+  return encode;
+}
+
+bool make_q_map(const AttnArgs& a, int rows, CUtensorMap* map) {
+  const Encode encode = encoder();
+  if (!encode || a.group > 256 || rows > 256) return false;
+  const int heads = a.group * a.c.nkv;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.c.hd, (cuuint64_t)heads, (cuuint64_t)a.c.rows};
+  // The stride of a dimension of one means nothing, but has to be valid.
+  const cuuint64_t strides[2] = {(cuuint64_t)(heads == 1 ? 8 : a.q_head) * 2, (cuuint64_t)(a.c.rows == 1 ? 8 : a.q_row) * 2};
+  if (!strides[0] || !strides[1] || strides[0] >= (1ull << 40) || strides[1] >= (1ull << 40)) return false;
+  const cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)rows}, ones[3] = {1, 1, 1};
+  return encode(map, a.dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                const_cast<void*>(a.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool make_maps(const PagedChunk& c, int dtype, int box, KvMaps* maps) {
+  const Encode encode = encoder();
   if (!encode) return false;
   const int elt = dtype == kF32 ? 4 : 2;
   const CUtensorMapDataType type = dtype == kF32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32

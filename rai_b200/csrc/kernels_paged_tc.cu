@@ -180,9 +180,13 @@ __device__ __forceinline__ uint32_t flags_of(const Params& p, const Cursor<MT, N
   return f;
 }
 
+// The lowest n bits, n cut to 0 .. 32.
+__device__ __forceinline__ uint32_t bits_to(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+
 template <typename C, bool CAP, bool TMA>
 __global__ void __launch_bounds__(kTcThreads, 1)
-    paged_attn_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ KvMaps maps, int box) {
+    paged_attn_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ KvMaps maps, int box,
+                         const __grid_constant__ CUtensorMap q_map, bool q_tma) {
   constexpr int DT = C::DT, HD = C::HD, MT = C::MT, NT = C::NT;
   constexpr bool DUO = C::DUO;
   constexpr int kQThreads = DUO ? 32 : kProducers;
@@ -208,7 +212,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_init(&b_ready, 4);
     mbar_init(&b_read, 4);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], kQThreads);
+      mbar_init(&q_full[i], q_tma ? 1 : kQThreads);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
@@ -294,10 +298,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const Item& it = cur.it;
         if (!DUO && fresh) {
           if (k > 0 && !__all_sync(~0u, wait_bar(&q_empty[0], (items - 1) & 1, err))) break;
-          load_queries<C, kProducers>(p, it, cur.head, sq, tid);
-          cp_async_wait<0>();
-          fence_async();
-          mbar_arrive(&q_full[0]);
+          if (q_tma) {
+            // group heads x (256 / group) rows, as the flattened rows lie
+            if (tid == 0) {
+              mbar_arrive_expect_tx(&q_full[0], MT * HD * 2);
+              const int qi = it.start + (int)p.group_div.quot(it.f0);
+#pragma unroll
+              for (int x = 0; x < HD / 64; ++x) tma_load3(sq + x * MT * 128, &q_map, x * 64, cur.head * p.a.group, qi, &q_full[0]);
+            }
+          } else {
+            load_queries<C, kProducers>(p, it, cur.head, sq, tid);
+            cp_async_wait<0>();
+            fence_async();
+            mbar_arrive(&q_full[0]);
+          }
           fresh = false;
         }
         if (!__all_sync(~0u, wait_bar(&landed[k % kLanded], k / kLanded & 1, err))) break;
@@ -564,10 +578,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               for (int x = 0; x < 128; ++x) v[x] = __float_as_uint(capped<DT>(__uint_as_float(v[x]), p.a.scale, p.a.softcap));
             }
             if (tile_masked(it, t0, NT, p.a.window, p.group_div)) {
+              // Columns from .. till as bits: two instructions an element (a
+              // comparison with both ends was a branch each, 4 us a tile).
               const int from = max(it.lo, p.a.window > 0 ? pos - p.a.window + 1 : 0) - t0, till = pos - t0;
 #pragma unroll
-              for (int x = 0; x < 128; ++x)
-                if (x > till || x < from) v[x] = 0xff800000u;
+              for (int w = 0; w < 4; ++w) {
+                const uint32_t bits = bits_to(till + 1 - 32 * w) & ~bits_to(from - 32 * w);
+#pragma unroll
+                for (int x = 0; x < 32; ++x) v[32 * w + x] = bits >> x & 1u ? v[32 * w + x] : 0xff800000u;
+              }
             }
             float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -739,6 +758,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
 template <typename C, bool CAP, bool TMA>
 cudaError_t launch(const AttnArgs& a, const KvMaps& maps, int box, cudaStream_t s) {
+  CUtensorMap q_map;
+  const bool q_tma = TMA && !C::DUO && 256 % a.group == 0 && make_q_map(a, 256 / a.group, &q_map);
   static std::once_flag once[64];
   static cudaError_t ready[64];
   int dev = 0;
@@ -765,7 +786,7 @@ cudaError_t launch(const AttnArgs& a, const KvMaps& maps, int box, cudaStream_t 
   p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
   // Not launched ahead of its predecessor's end: a batch of prompts takes 344
   // us so and 357 us with it (long verification: 165 either way).
-  paged_attn_tc_kernel<C, CAP, TMA><<<p.grid, kTcThreads, C::kSmem, s>>>(p, maps, box);
+  paged_attn_tc_kernel<C, CAP, TMA><<<p.grid, kTcThreads, C::kSmem, s>>>(p, maps, box, q_map, q_tma);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return launch_pdl(paged_combine_kernel<C>, dim3(p.grid - 1, combine_grid_y(C::MT)), dim3(kCombineThreads), 0, s, p);

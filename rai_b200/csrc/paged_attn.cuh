@@ -277,6 +277,9 @@ inline int tma_box(int page, int nt) {
 }
 // Whether the maps could be made (kernels_paged_attn.cu).
 bool make_maps(const PagedChunk& c, int dtype, int box, KvMaps* maps);
+// The queries of 16-bit types as a tensor (element, head, row), `rows` rows of
+// one KV head's heads a box.
+bool make_q_map(const AttnArgs& a, int rows, CUtensorMap* map);
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page,
                                          uint64_t* bar) {
@@ -284,6 +287,13 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
       "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
           dst),
       "l"(map), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
 }
 
