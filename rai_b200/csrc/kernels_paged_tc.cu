@@ -72,7 +72,7 @@ struct Tc {
 constexpr float kLazy = 8.f;  // log2 units
 // Few rows and heads wider than 64: from how many tokens a sequence, and a
 // call's sequences and KV heads together, can have this kernel is the faster
-// one. (8 KV heads of 128: 256 x 1,000 tokens 328 us here and 404 us on
+// one. (8 KV heads of 128: 256 x 1,000 tokens 305 us here and 404 us on
 // mma.sync, 16 x 2,000 73 / 83, 1 x 16,000 56 / 61; 64 x 1,000 134 / 136,
 // 256 x 300 167 / 162, 1 x 1,500 52 / 42. Heads of 64, 64 x 8,000: 233 / 120.)
 constexpr long long kTcFewRowsTokens = 768, kTcFewRowsTotal = 131072;
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __shared__ uint64_t kv_full[C::kSlots], kv_empty[C::kSlots], q_full[2], q_empty[2], s_full[2], p_full[2], o_done[2], drained;
   __shared__ uint64_t b_ready, b_read;  // DUO: half B's sums are there, were read
   __shared__ float2 b_sums[DUO ? 128 : 1];  // half B's (m, l)
-  __shared__ uint64_t landed[kLanded];
+  __shared__ uint64_t landed[kLanded], looked;
   __shared__ uint32_t flags[C::kSlots];  // of the tile whose K is in the slot
   __shared__ uint32_t tmem_slot;
   __shared__ int poison[4];  // ordinal + 1 of an item with masked V values that are not finite
@@ -219,6 +219,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&o_done[i], 1);
     }
     mbar_init(&drained, 1);
+    mbar_init(&looked, 2);
     for (int i = 0; i < kLanded; ++i) mbar_init(&landed[i], 1);
     for (int i = 0; i < 4; ++i) poison[i] = 0;
     fence_barrier_init();
@@ -294,12 +295,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (tid == 0) leave_cut<MT, NT>(p, rg, cur, blockIdx.x);
       int items = 0;
       bool fresh = true;
+      uint32_t asked = 0, looks = 0;  // query tiles requested by TMA, V tiles looked through
       for (uint32_t k = 0; cur.pos < end; ++k) {
         const Item& it = cur.it;
         if (!DUO && fresh) {
           if (k > 0 && !__all_sync(~0u, wait_bar(&q_empty[0], (items - 1) & 1, err))) break;
           if (q_tma) {
             // group heads x (256 / group) rows, as the flattened rows lie
+            ++asked;
             if (tid == 0) {
               mbar_arrive_expect_tx(&q_full[0], MT * HD * 2);
               const int qi = it.start + (int)p.group_div.quot(it.f0);
@@ -320,7 +323,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (tile_masked(it, t0, NT, p.a.window, p.group_div)) {
           if (look_through<C>(skv + slot * C::kTileB, t0, it, tid)) *(volatile int*)&poison[items & 3] = items + 1;
           fence_async();
-          asm volatile("bar.sync 1, 64;" ::: "memory");
+          // Both warps' shares are done. (Waits are bounded, so this is no
+          // bar.sync, which a warp that gave up would leave the other in.)
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&looked);
+          if (warp == 10 && !__all_sync(~0u, wait_bar(&looked, looks & 1, err))) break;
+          ++looks;
         }
         if (tid == 0) mbar_arrive(&kv_full[slot]);
         if (cur.last_of_item()) {
@@ -329,6 +337,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         cur.next(p);
       }
+      // What was requested lands before the CTA ends.
+      if (asked && tid == 0) wait_bar(&q_full[0], (asked - 1) & 1, nullptr);
     } else if (begin < end && !TMA && warp >= 10) {
       // ---------------- K, V and queries by 16-byte copies ----------------
       const int tid = threadIdx.x - 10 * 32;
@@ -779,12 +789,11 @@ cudaError_t launch(const AttnArgs& a, const KvMaps& maps, int box, cudaStream_t 
   p.grid = device_sm_count();
   p.whole = p.direct = false;
   p.min_tiles = 10;
-  // An item costs about 11 us beside its tiles of 1.85 us (64 KB of K and V):
-  // prompts of 8,192 tokens take 700 / 624 / 621 / 638 us at 3 / 5 / 7 / 10.
-  // (Capped scores make the tiles twice as dear.)
-  p.item_cost = CAP ? 3 : 6;
+  // An item costs about 5 us beside its tiles of 1.8 us: three prompts of
+  // 3,000 tokens take 325 / 324 / 329 / 342 us at 2 / 3 / 4 / 6.
+  p.item_cost = 3;
   p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
-  // Not launched ahead of its predecessor's end: a batch of prompts takes 344
+  // Not launched ahead of its predecessor's end: a batch of prompts took 344
   // us so and 357 us with it (long verification: 165 either way).
   paged_attn_tc_kernel<C, CAP, TMA><<<p.grid, kTcThreads, C::kSmem, s>>>(p, maps, box, q_map, q_tma);
   e = cudaGetLastError();
