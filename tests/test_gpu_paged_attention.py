@@ -271,3 +271,40 @@ def test_offsets_past_32_bits():
     got = paged.attention(q, k, v, table, c.kv_len, ref.starts_of([1], dev), 1)
     want = paged.attention(q, c.k, c.v, c.table, c.kv_len, ref.starts_of([1], dev), 1)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("heads,nkv", [(2, 2), (8, 1), (7, 1), (32, 2)])
+@pytest.mark.parametrize("hd", [64, 80, 128])
+def test_chunks_shorter_than_a_query_tile(heads, nkv, hd):
+    """Row tensors with fewer rows than a tile of queries has, groups that do
+    and do not divide it."""
+    dev = torch.device("cuda", 0)
+    for rows, lens in (([70], [70]), ([129, 66], [400, 66]), ([300], [1000])):
+        c = ref.Cache(lens, nkv, hd, 16, torch.bfloat16, dev, seed=hd)
+        q = make_q(sum(rows), heads, hd, torch.bfloat16, dev)
+        got, lse = run(c, q, rows)
+        agree(c, q, rows, got, lse)
+
+
+def test_two_streams_at_once():
+    """Calls of both kernels that may overlap, each with its own workspace."""
+    from rai_b200 import paged
+    dev = torch.device("cuda", 0)
+    jobs = []
+    for hd, rows, lens in ((64, [1] * 8, [700] * 8), (128, [200, 90], [2000, 90]), (128, [1, 3], [9000, 9000])):
+        c = ref.Cache(lens, 2, hd, 16, torch.bfloat16, dev, seed=hd, wide=4000)
+        q = make_q(sum(rows), 8, hd, torch.bfloat16, dev)
+        jobs.append((q, c.k, c.v, c.table, c.kv_len, ref.starts_of(rows, dev), max(rows)))
+    want = [paged.attention(*j) for j in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[] for _ in jobs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(6):
+        for s, j, g in zip(streams, jobs, got):
+            with torch.cuda.stream(s):
+                g.append(paged.attention(*j))
+    torch.cuda.synchronize()
+    paged.status()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, x) for x in g)
