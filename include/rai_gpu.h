@@ -452,8 +452,8 @@ typedef struct {
   uint32_t n_layers, n_pages;
 } rai_page_pool;
 
-/* Fork: out sequence i takes the pages of `in` sequence parents[i] (device;
- * -1: empty). No data moves: refs (shared, in place) of a page become the
+/* Fork: out sequence i takes the pages of `in` sequence parents[i] (device,
+ * [out->n_seqs]; -1: empty). No data moves: refs (shared, in place) of a page become the
  * number of out cells that name it, so a sequence without children is freed
  * and one with several is shared, its last page too (rai_gpu_kv_resize then
  * copies it on write). `out` has its own table and lengths and in's refs;

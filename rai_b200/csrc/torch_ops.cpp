@@ -247,6 +247,9 @@ std::pair<rai_page_pool, int64_t> pool_of(const Tensor& k, const Tensor& v) {
 std::tuple<Tensor, Tensor> kv_fork(const Tensor& table, const Tensor& lens, const Tensor& refs, const Tensor& parents, int64_t page_size,
                                 const OptTensor& table_in, const OptTensor& lens_in) {
   need(parents.dim() == 1 && parents.size(0) > 0 && lens.numel() > 0 && table.dim() == 2, "fork: no sequences");
+  // The number of children is the outputs': one for each parent named.
+  need(!lens_in || (lens_in->dim() == 1 && lens_in->size(0) == parents.size(0)), "out_lens: as many as parents");
+  need(!table_in || (table_in->dim() == 2 && table_in->size(0) == parents.size(0)), "out_table: as many rows as parents");
   const c10::DeviceIndex dev = device_of(table, lens, refs, parents);
   on_device(table_in, dev);
   on_device(lens_in, dev);

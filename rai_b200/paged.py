@@ -87,8 +87,8 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, kind: str = "plain", 
 def fork(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor, page_size: int, *,
          out_table: Optional[torch.Tensor] = None, out_lens: Optional[torch.Tensor] = None):
     """Sequence i of the result takes the pages of sequence parents[i] (-1:
-    none); returns (table, lens), in new memory or in out_table, out_lens
-    (rai_gpu_kv_fork). refs is updated in place: sequences without children
+    none); returns (table, lens), in new memory or in out_table, out_lens (as
+    many rows as parents) (rai_gpu_kv_fork). refs is updated in place: sequences without children
     are freed, children of one parent share its pages. No page moves."""
     return _ops.fork(page_table, lens, refs, parents, page_size, out_table, out_lens)
 

@@ -378,3 +378,24 @@ def test_resize_gives_nothing_when_pages_are_short():
     table = torch.full((n, 600), -1, dtype=torch.int32, device=dev)
     assert paged.resize(table, lens, refs, k, k.clone(), delta=600).item() == n * 600 - 3
     assert lens.sum().item() == 0 and refs.sum().item() == 0 and (table == -1).all()
+
+
+@pytest.mark.parametrize("children", [1, 2, 5])
+def test_fork_into_given_outputs(children):
+    """out_table (a part of a wider one) and out_lens, more or fewer children
+    than parents."""
+    from rai_b200 import paged
+    dev = torch.device("cuda", 0)
+    lens = [20, 33, 7]
+    c = ref.Cache(lens, 1, 16, 16, torch.bfloat16, dev, junk=0.0)
+    want = ref.Pages(c.rows, lens, lists(c.refs), 16)
+    parents = [1, 0, 1, -1, 2][:children]
+    width = c.table.shape[1]
+    want.fork(parents, width)
+    wide = torch.full((children, width + 3), 77, dtype=torch.int32, device=dev)
+    out, n = wide[:, :width], torch.full((children,), 77, dtype=torch.int32, device=dev)
+    got = paged.fork(c.table, c.kv_len, c.refs, torch.tensor(parents, dtype=torch.int32, device=dev), 16, out_table=out, out_lens=n)
+    paged.status()
+    assert got[0].data_ptr() == out.data_ptr() and got[1].data_ptr() == n.data_ptr()
+    check_pages(want, out, n, c.refs)
+    assert (wide[:, width:] == 77).all()

@@ -220,3 +220,17 @@ def test_rope_frequencies():
             paged.rope_frequencies(**{"rot_dim": 64, **bad})
     with pytest.raises(ValueError):
         paged.rope_frequencies(64, kind="cubic")
+
+
+@pytest.mark.parametrize("rows", [1, 3, 9])
+def test_fork_refuses_outputs_of_another_number_of_rows(rows):
+    """The kernel takes the number of children from the outputs and reads as
+    many parents."""
+    torch = pytest.importorskip("torch")
+    from rai_b200 import paged
+    i32 = dict(dtype=torch.int32)
+    table, lens, refs, parents = torch.zeros(2, 4, **i32), torch.ones(2, **i32), torch.ones(8, **i32), torch.zeros(2, **i32)
+    with pytest.raises(ValueError, match="out_lens"):
+        paged.fork(table, lens, refs, parents, 16, out_table=torch.zeros(2, 4, **i32), out_lens=torch.zeros(rows, **i32))
+    with pytest.raises(ValueError, match="out_table"):
+        paged.fork(table, lens, refs, parents, 16, out_table=torch.zeros(rows, 4, **i32), out_lens=torch.zeros(2, **i32))
