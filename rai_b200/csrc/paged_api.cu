@@ -138,7 +138,9 @@ int check_pool(const rai_page_pool* p, uint32_t n_pages, rai::PagePool* out) {
 extern "C" {
 
 size_t rai_gpu_paged_attention_workspace_bytes(const rai_paged_attention* a) {
-  if (!a || !a->chunk.n_kv_heads || !a->n_heads) return 0;
+  // (Sizes that the call refuses need no workspace; the rules below divide by
+  // some of them.)
+  if (!a || !a->chunk.n_kv_heads || !a->n_heads || !a->chunk.page_size || !a->chunk.max_rows) return 0;
   rai::AttnArgs o;
   o.c.hd = (int)a->chunk.head_dim, o.c.max_rows = (int)a->chunk.max_rows;
   o.c.max_pages = (int)a->chunk.max_pages, o.c.page.d = a->chunk.page_size;

@@ -5,6 +5,7 @@ import json
 import math
 import os
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -234,3 +235,20 @@ def test_fork_refuses_outputs_of_another_number_of_rows(rows):
         paged.fork(table, lens, refs, parents, 16, out_table=torch.zeros(2, 4, **i32), out_lens=torch.zeros(rows, **i32))
     with pytest.raises(ValueError, match="out_table"):
         paged.fork(table, lens, refs, parents, 16, out_table=torch.zeros(rows, 4, **i32), out_lens=torch.zeros(2, **i32))
+
+
+def test_attention_workspace_of_empty_pages():
+    """Pages of no tokens: refused by the call, no division by zero in the
+    query before it. (In a child, which the division would end.)"""
+    code = """
+import ctypes as C
+from rai_b200 import native
+for hd in (64, 128, 256):
+    for dtype in range(3):
+        for page, rows in ((0, 1), (0, 500), (16, 0)):
+            a = native.PagedAttention(chunk=native.PagedChunk(n_seqs=1, max_pages=400, n_pages=4, page_size=page, n_kv_heads=2, head_dim=hd,
+                                                              rows=rows, max_rows=rows, dtype=dtype), n_heads=4)
+            assert native.lib().rai_gpu_paged_attention_workspace_bytes(C.byref(a)) == 0
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT)
+    assert attn(dict(page_size=0)) == I
