@@ -295,11 +295,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (tid == 0) leave_cut<MT, NT>(p, rg, cur, blockIdx.x);
       int items = 0;
       bool fresh = true;
-      uint32_t asked = 0, looks = 0;  // query tiles requested by TMA, V tiles looked through
+      uint32_t asked = 0;  // query tiles requested by TMA
       for (uint32_t k = 0; cur.pos < end; ++k) {
         const Item& it = cur.it;
         if (!DUO && fresh) {
-          if (k > 0 && !__all_sync(~0u, wait_bar(&q_empty[0], (items - 1) & 1, err))) break;
+          // (By TMA warp 10 alone asks. Warp 11 has no part in it, so nothing
+          // would keep the next phase from completing before it looked.)
+          if (k > 0 && (!q_tma || warp == 10) && !__all_sync(~0u, wait_bar(&q_empty[0], (items - 1) & 1, err))) break;
           if (q_tma) {
             // group heads x (256 / group) rows, as the flattened rows lie
             ++asked;
@@ -320,17 +322,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!__all_sync(~0u, wait_bar(&landed[k % kLanded], k / kLanded & 1, err))) break;
         const uint32_t slot = (2 * k + 1) % C::kSlots;
         const int t0 = (it.first + cur.tile) * NT;
-        if (tile_masked(it, t0, NT, p.a.window, p.group_div)) {
+        // The warps meet at every tile, so that neither is ever a phase of a
+        // barrier (looked, landed) ahead of the other: a wait by parity takes
+        // two phases ahead for none. (Waits are bounded, so this is no
+        // bar.sync, which a warp that gave up would leave the other in.) A
+        // tile that nobody looks through is handed over before.
+        const bool masked = tile_masked(it, t0, NT, p.a.window, p.group_div);
+        if (masked) {
           if (look_through<C>(skv + slot * C::kTileB, t0, it, tid)) *(volatile int*)&poison[items & 3] = items + 1;
           fence_async();
-          // Both warps' shares are done. (Waits are bounded, so this is no
-          // bar.sync, which a warp that gave up would leave the other in.)
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&looked);
-          if (warp == 10 && !__all_sync(~0u, wait_bar(&looked, looks & 1, err))) break;
-          ++looks;
+        } else if (tid == 0) {
+          mbar_arrive(&kv_full[slot]);
         }
-        if (tid == 0) mbar_arrive(&kv_full[slot]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&looked);
+        if (!__all_sync(~0u, wait_bar(&looked, k & 1, err))) break;
+        if (masked && tid == 0) mbar_arrive(&kv_full[slot]);
         if (cur.last_of_item()) {
           fresh = true;
           ++items;

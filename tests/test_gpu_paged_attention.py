@@ -308,3 +308,21 @@ def test_two_streams_at_once():
     paged.status()
     for w, g in zip(want, got):
         assert all(torch.equal(w, x) for x in g)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=str)
+@pytest.mark.parametrize("heads,nkv,hd", [(16, 16, 64), (16, 16, 128), (12, 4, 64), (16, 4, 64)])
+@pytest.mark.parametrize("window", [40, 256])
+def test_many_masked_tiles_in_a_row(dtype, heads, nkv, hd, window):
+    """Long chunks behind a window of a few tiles: nearly every tile of V is
+    looked through by two warps that have to stay together, in items of a few
+    tiles each, whose queries come by TMA or by copies."""
+    dev = torch.device("cuda", 0)
+    rows, lens = [3000, 300, 2500, 2999, 1], [3000, 800, 2600, 4000, 900]
+    c = ref.Cache(lens, nkv, hd, 16, dtype, dev, seed=window)
+    q = make_q(sum(rows), heads, hd, dtype, dev)
+    first, lse = run(c, q, rows, window=window)
+    for _ in range(20):
+        got, _ = run(c, q, rows, window=window)
+        assert torch.equal(got, first)
+    agree(c, q, rows, first, lse, window=window)
