@@ -409,12 +409,19 @@ template <int DT, int NT>
 __device__ __noinline__ float lost_values(const Params& p, const Item it, int kv_head, int col, int from, int till) {
   const PagedChunk& c = p.a.c;
   float sum = 0.f;
-  for (int t = from; t < till; ++t) {
-    if (!tile_masked(it, t / NT * NT, NT, p.a.window, p.group_div)) continue;
-    const int pi = (int)c.page.quot(t), page = page_of(c, it.seq, pi);
-    if (page < 0) continue;
-    const float v = value<DT>(c.v, page * c.v_page + (long long)kv_head * c.v_head + (t - pi * (int)c.page.d) * c.v_slot + col);
-    if (!(fabsf(v) <= 3.4028235e38f)) sum += v;
+  // By tiles: what lies between the masked ones may be a long context, and the
+  // other warps' waits are bounded.
+  for (int t = from; t < till;) {
+    const int next = min(till, (t / NT + 1) * NT);
+    if (tile_masked(it, t / NT * NT, NT, p.a.window, p.group_div)) {
+      for (; t < next; ++t) {
+        const int pi = (int)c.page.quot(t), page = page_of(c, it.seq, pi);
+        if (page < 0) continue;
+        const float v = value<DT>(c.v, page * c.v_page + (long long)kv_head * c.v_head + (t - pi * (int)c.page.d) * c.v_slot + col);
+        if (!(fabsf(v) <= 3.4028235e38f)) sum += v;
+      }
+    }
+    t = next;
   }
   return sum;
 }

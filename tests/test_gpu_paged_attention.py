@@ -326,3 +326,36 @@ def test_many_masked_tiles_in_a_row(dtype, heads, nkv, hd, window):
         got, _ = run(c, q, rows, window=window)
         assert torch.equal(got, first)
     agree(c, q, rows, first, lse, window=window)
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)], ids=str)
+def test_an_infinite_value_at_the_end_of_a_million_tokens(dtype, hd):
+    """Sequences that share one long context, a whole item or a third of one to
+    a CTA: giving the value back to the rows that see it walks the masked tiles
+    alone, so that no other warp's wait runs out meanwhile."""
+    from rai_b200 import paged
+    dev = torch.device("cuda", 0)
+    n, seqs, page = 1_000_003, 150, 128
+    g = torch.Generator(device=dev).manual_seed(hd)
+    pages = -(-n // page)
+    k, v = (torch.randn((pages, 1, page, hd), device=dev, generator=g).to(dtype) for _ in range(2))
+    t = n - 2
+    v[t // page, 0, t % page, 1] = math.inf
+    v[t // page, 0, t % page, hd - 1] = math.nan
+    table = torch.arange(pages, dtype=torch.int32, device=dev).expand(seqs, pages).contiguous()
+    q = torch.randn((1, 2, hd), device=dev, generator=g).to(dtype).expand(seqs, 2, hd).contiguous()
+    lens = torch.full((seqs,), n, dtype=torch.int32, device=dev)
+    got = paged.attention(q, k, v, table, lens, torch.arange(seqs + 1, dtype=torch.int32, device=dev), 1)
+    paged.status()
+    kk, vv = (x.view(-1, hd)[:n].double() for x in (k, v))
+    p = torch.softmax(hd ** -0.5 * (q[0].double() @ kk.T), 1)
+    seen = torch.isfinite(vv)
+    want = p @ torch.where(seen, vv, 0.0)
+    size = p @ torch.where(seen, vv, 0.0).abs()
+    assert (got[:, :, 1] == math.inf).all() and torch.isnan(got[:, :, hd - 1]).all()
+    cols = [c for c in range(hd) if c not in (1, hd - 1)]
+    # Roundings of the output and the probabilities, sums of n terms in f32
+    # (random: their square root), scores off by hd + 4 roundings.
+    u = ref.EPS[dtype]
+    bound = u * want.abs() + size * (1.01 * u + 2 * (hd + 4) * 2.0 ** -24 * 10 + n ** 0.5 * 2.0 ** -22) + 2.0 ** -24 * (dtype == torch.float16)
+    assert ((got[:, :, cols].double() - want[:, cols]).abs() <= bound[:, cols]).all()
