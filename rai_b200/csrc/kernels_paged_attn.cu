@@ -432,7 +432,11 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int x = 0; x < NTW / 8; ++x)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) s[x][y] = capped<DT>(s[x][y], p.a.scale, p.a.softcap);
+        for (int y = 0; y < 4; y += 2) {
+          const float2 z = capped<DT>({s[x][y], s[x][y + 1]}, p.a.scale, p.a.softcap, p.inv_cap);
+          s[x][y] = z.x;
+          s[x][y + 1] = z.y;
+        }
     }
     if (masked) {
 #pragma unroll
@@ -711,6 +715,7 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
   p.direct = p.whole && items <= 2ll * p.grid;  // no need to share them out
   if (p.direct) p.grid = (int)items;
   p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
+  p.inv_cap = a.softcap > 0.f ? 1.f / a.softcap : 0.f;
   KvMaps maps;
   const int box = tma_box((int)a.c.page.d, C::NT);
   const bool tma = box && make_maps(a.c, a.dtype, box, &maps);

@@ -592,7 +592,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tm_wait_ld();
             if constexpr (CAP) {
 #pragma unroll
-              for (int x = 0; x < 128; ++x) v[x] = __float_as_uint(capped<DT>(__uint_as_float(v[x]), p.a.scale, p.a.softcap));
+              for (int x = 0; x < 128; x += 2) {
+                const float2 y = capped<DT>({__uint_as_float(v[x]), __uint_as_float(v[x + 1])}, p.a.scale, p.a.softcap, p.inv_cap);
+                v[x] = __float_as_uint(y.x);
+                v[x + 1] = __float_as_uint(y.y);
+              }
             }
             if (tile_masked(it, t0, NT, p.a.window, p.group_div)) {
               // Columns from .. till as bits: two instructions an element (a
@@ -800,6 +804,7 @@ cudaError_t launch(const AttnArgs& a, const KvMaps& maps, int box, cudaStream_t 
   // 3,000 tokens take 325 / 324 / 329 / 342 us at 2 / 3 / 4 / 6.
   p.item_cost = 3;
   p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
+  p.inv_cap = a.softcap > 0.f ? 1.f / a.softcap : 0.f;
   // Not launched ahead of its predecessor's end: a batch of prompts took 344
   // us so and 357 us with it (long verification: 165 either way).
   paged_attn_tc_kernel<C, CAP, TMA><<<p.grid, kTcThreads, C::kSmem, s>>>(p, maps, box, q_map, q_tma);

@@ -91,7 +91,7 @@ int attention_args(const rai_paged_attention* a, rai::AttnArgs* out) {
   if ((uint64_t)a->chunk.n_seqs * (((uint64_t)a->chunk.max_rows * (a->n_heads / a->chunk.n_kv_heads) + 15) / 16) > (1u << 30))
     return bad("n_seqs * max_rows is out of range");
   if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return bad("scale has to be positive");
-  if (!(a->softcap >= 0.f) || !std::isfinite(a->softcap)) return bad("softcap");
+  if (!(a->softcap == 0.f || std::isnormal(a->softcap)) || a->softcap < 0.f) return bad("softcap: 0, or a positive normal number");
   if (a->window > (1u << 30)) return bad("window");
   o.q = a->q, o.out = a->out, o.lse = a->lse;
   o.q_row = a->q_row, o.q_head = a->q_head, o.o_row = a->out_row, o.o_head = a->out_head;

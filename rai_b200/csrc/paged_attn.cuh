@@ -24,6 +24,7 @@ struct Params {
   bool whole;   // items are short: none is cut
   bool direct;  // one CTA per item, in order
   float c;  // log2(e) * scale, or log2(e) when the scores are capped
+  float inv_cap;  // 1 / softcap
   FastDiv row_tiles_div, group_div;
 };
 
@@ -390,15 +391,42 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// cap tanh(z / cap), z = scale s, of two scores, right relative to the score
+// for any cap.
+//
+// 16-bit types: tanh x = 1 - 2 / (1 + e^2x) is right to 2^-21.6 of 1, which
+// for small x is nothing of x; there z (1 - x^2 / 3 + 2 x^4 / 15), whose next
+// term is 17/315 x^6 < 2^-22 below x = 1/8. At that border the first form is
+// right to 2^-18.6 of the score. (y = 2 log2(e) x serves both.)
 template <int DT>
-__device__ __forceinline__ float capped(float s, float scale, float cap) {
-  const float x = __fdividef(s * scale, cap);
+__device__ __forceinline__ float2 capped(float2 s, float scale, float cap, float inv_cap) {
+  const float2 z = mul2(s, {scale, scale});
   if constexpr (DT == kF32) {
-    return cap * tanhf(x);
+    const float2 x = mul2(z, {inv_cap, inv_cap});
+    // Below 2^-12 tanh x is x; z has not been through a quotient that may
+    // lie below the normal numbers.
+    return {fabsf(x.x) < 0x1p-12f ? z.x : cap * tanhf(x.x), fabsf(x.y) < 0x1p-12f ? z.y : cap * tanhf(x.y)};
   } else {
-    // tanh x = 1 - 2 / (1 + e^2x): a few 2^-23 of the cap, far below the
-    // 2^-9 that a probability is rounded to.
-    return cap * (1.f - __fdividef(2.f, 1.f + exp2_fast(2.f * kLog2e * x)));
+    const float k = 2.f * kLog2e * inv_cap;
+    const float2 y = mul2(z, {k, k});
+    const float2 e = add2({exp2_fast(y.x), exp2_fast(y.y)}, {1.f, 1.f});
+    const float2 far = mul2(fma2({rcp_fast(e.x), rcp_fast(e.y)}, {-2.f, -2.f}, {1.f, 1.f}), {cap, cap});
+    constexpr float k2 = 4.f * kLog2e * kLog2e, c1 = -1.f / (3.f * k2), c2 = 2.f / (15.f * k2 * k2);
+    const float2 w = mul2(y, y);
+    const float2 near = fma2(mul2(z, w), fma2(w, {c2, c2}, {c1, c1}), z);
+    return {fabsf(y.x) < 0.36f ? near.x : far.x, fabsf(y.y) < 0.36f ? near.y : far.y};
   }
 }
 // The V values of column `col` that are not finite among the tokens [from,

@@ -359,3 +359,25 @@ def test_an_infinite_value_at_the_end_of_a_million_tokens(dtype, hd):
     u = ref.EPS[dtype]
     bound = u * want.abs() + size * (1.01 * u + 2 * (hd + 4) * 2.0 ** -24 * 10 + n ** 0.5 * 2.0 ** -22) + 2.0 ** -24 * (dtype == torch.float16)
     assert ((got[:, :, cols].double() - want[:, cols]).abs() <= bound[:, cols]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("hd,rows", [(64, [1, 3]), (128, [1, 3]), (128, [70, 3])], ids=str)
+@pytest.mark.parametrize("cap", [2.0, 100.0, 1e4, 1e6, 1e12, 3e38])
+def test_caps_far_above_the_scores(dtype, hd, rows, cap):
+    """A cap may be off by a part of the score, not of the cap."""
+    dev = torch.device("cuda", 0)
+    lens = [200, 90]
+    c = ref.Cache(lens, 2, hd, 16, dtype, dev, seed=hd)
+    q = make_q(sum(rows), 4, hd, dtype, dev, scale=2.0)
+    got, lse = run(c, q, rows, softcap=cap)
+    want, _, wlse = ref.attention(q, c, rows, hd ** -0.5, cap)
+    # What the roundings around the cap may make of the same scores uncapped;
+    # the cap moves each score by 2^-17 of itself at most.
+    _, bound, _ = ref.attention(q, c, rows, hd ** -0.5)
+    top = max(q.double().norm(dim=-1).max() * k.norm(dim=-1).max() for k, _ in (c.tokens(s) for s in range(2))) * hd ** -0.5
+    size = max(v.abs().max() for _, v in (c.tokens(s) for s in range(2)))
+    # (bound holds the probabilities' and the output's roundings relative to
+    # the uncapped ones: 2 u of the largest value covers the capped ones.)
+    assert ((got.double() - want).abs() <= torch.clamp(bound, min=2.1 * ref.EPS[dtype] * size) + 2.0 ** -16 * top * size).all()
+    assert ((lse.double() - wlse).abs() <= 2.0 ** -18 * (1 + wlse.abs()) + 2.0 ** -17 * top).all()

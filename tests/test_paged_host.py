@@ -252,3 +252,8 @@ for hd in (64, 128, 256):
 """
     subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT)
     assert attn(dict(page_size=0)) == I
+
+
+@pytest.mark.parametrize("cap", [1e-40, -1e-40, -0.5, math.nan])
+def test_attention_refuses_caps_without_a_reciprocal(cap):
+    assert attn(softcap=cap) == I
