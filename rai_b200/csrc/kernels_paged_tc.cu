@@ -27,8 +27,8 @@
 // Warps: 0-3 and 4-7 softmax of halves A and B, 8 TMEM and MMA issue (one
 // thread; the MMAs of one thread run in issue order, so the next Q K^T may be
 // issued over a P that P V still reads), 9 K and V by TMA, a piece of a page
-// per lane (DUO: and the queries, two buffers), 10-11 the hand-over of V tiles
-// (in masked tiles they are looked through first) and the queries. Pages that
+// per lane (DUO: and the queries, two buffers), 10-11 the masked V tiles, which
+// are looked through before the MMA gets them, and the queries. Pages that
 // TMA cannot fetch (sizes that are not 8 x 2^i or whole tiles) come by 16-byte
 // copies of warps 10-11. Tiles lie in the 128-byte swizzle the MMA reads,
 // K-major for Q K^T and N-major for P V. Every wait is bounded; on a timeout
@@ -168,6 +168,11 @@ __device__ __forceinline__ void load_queries(const Params& p, const Item& it, in
 }
 
 constexpr int kLanded = 8;  // V tiles between their landing and their hand-over
+// V tile k goes through the hands of warps 10 and 11. (Besides the masked ones
+// one in 1024, since their waits for the next are bounded.)
+__device__ __forceinline__ bool by_hand(const Params& p, const Item& it, uint32_t k, int t0, int nt) {
+  return (k & 1023u) == 1023u || tile_masked(it, t0, nt, p.a.window, p.group_div);
+}
 
 // What the issuing thread has to know of a tile: it is the last of its item;
 // the last of its item here; the last of the CTA.
@@ -249,12 +254,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       cur.seek(p, rg);
       TilePieces<NT, HD / 64, 2> pieces;
       pieces.fetch(ch, cur.it, (cur.it.first + cur.tile) * NT, box, lane);
-      uint32_t issued = 0;
+      uint32_t issued = 0, by_hands = 0;
+      uint32_t handed = 0;  // bit i: fetch issued - 1 - i is a V tile that goes by hand
       int items = 0;
       bool ok = true, fresh = true;
       for (uint32_t k = 0; cur.pos < end && ok; ++k) {
         const Item& it = cur.it;
         const int t0 = (it.first + cur.tile) * NT;
+        const bool hand = by_hand(p, it, k, t0, NT);
         const bool queries = DUO && fresh;
         if (queries) {
           if (items >= 2) ok = __all_sync(~0u, wait_bar(&q_empty[items & 1], (items / 2 - 1) & 1, err));
@@ -268,8 +275,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (ok) {
             if (kv == 0 && lane == 0) flags[slot] = flags_of<MT, NT>(p, cur, end);
             pieces.load(ch, it, t0, box, lane, kv ? &maps.v : &maps.k, cur.head, skv + slot * C::kTileB,
-                        kv ? &landed[k % kLanded] : &kv_full[slot]);
+                        kv && hand ? &landed[by_hands % kLanded] : &kv_full[slot]);
             ++issued;
+            handed = handed << 1 | (kv && hand ? 1u : 0u);
+            if (kv && hand) ++by_hands;
           }
         }
         if (queries) {
@@ -283,19 +292,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (cur.pos < end) pieces.fetch(ch, cur.it, (cur.it.first + cur.tile) * NT, box, lane);
       }
       // What was requested lands before the CTA ends.
-      for (uint32_t n = issued > C::kSlots ? issued - C::kSlots : 0; n < issued; ++n) {
-        if (n & 1) wait_bar(&landed[n / 2 % kLanded], n / 2 / kLanded & 1, nullptr);
-        else wait_bar(&kv_full[n % C::kSlots], n / C::kSlots & 1, nullptr);
+      for (uint32_t i = 0; i < C::kSlots && i < issued; ++i, handed >>= 1) {
+        const uint32_t n = issued - 1 - i;
+        if (handed & 1u) {
+          --by_hands;
+          wait_bar(&landed[by_hands % kLanded], by_hands / kLanded & 1, nullptr);
+        } else {
+          wait_bar(&kv_full[n % C::kSlots], n / C::kSlots & 1, nullptr);
+        }
       }
     } else if (begin < end && TMA && warp >= 10) {
-      // ---------------- queries; V tiles handed over ----------------
+      // ---------------- queries; masked V tiles ----------------
       const int tid = threadIdx.x - 10 * 32;
       Cursor<MT, NT> cur;
       cur.seek(p, rg);
       if (tid == 0) leave_cut<MT, NT>(p, rg, cur, blockIdx.x);
       int items = 0;
       bool fresh = true;
-      uint32_t asked = 0;  // query tiles requested by TMA
+      uint32_t asked = 0, seen = 0;  // query tiles requested by TMA, V tiles that went by hand
       for (uint32_t k = 0; cur.pos < end; ++k) {
         const Item& it = cur.it;
         if (!DUO && fresh) {
@@ -319,25 +333,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           fresh = false;
         }
-        if (!__all_sync(~0u, wait_bar(&landed[k % kLanded], k / kLanded & 1, err))) break;
-        const uint32_t slot = (2 * k + 1) % C::kSlots;
         const int t0 = (it.first + cur.tile) * NT;
-        // The warps meet at every tile, so that neither is ever a phase of a
-        // barrier (looked, landed) ahead of the other: a wait by parity takes
-        // two phases ahead for none. (Waits are bounded, so this is no
-        // bar.sync, which a warp that gave up would leave the other in.) A
-        // tile that nobody looks through is handed over before.
-        const bool masked = tile_masked(it, t0, NT, p.a.window, p.group_div);
-        if (masked) {
-          if (look_through<C>(skv + slot * C::kTileB, t0, it, tid)) *(volatile int*)&poison[items & 3] = items + 1;
+        if (by_hand(p, it, k, t0, NT)) {
+          if (!__all_sync(~0u, wait_bar(&landed[seen % kLanded], seen / kLanded & 1, err))) break;
+          const uint32_t slot = (2 * k + 1) % C::kSlots;
+          if (tile_masked(it, t0, NT, p.a.window, p.group_div) && look_through<C>(skv + slot * C::kTileB, t0, it, tid))
+            *(volatile int*)&poison[items & 3] = items + 1;
           fence_async();
-        } else if (tid == 0) {
-          mbar_arrive(&kv_full[slot]);
+          __syncwarp();
+          // Both wait for both shares, so that neither is ever two phases of
+          // a barrier ahead of the other: a wait by parity takes two for none.
+          // (Waits are bounded, so this is no bar.sync, which a warp that gave
+          // up would leave the other in.)
+          if (lane == 0) mbar_arrive(&looked);
+          if (!__all_sync(~0u, wait_bar(&looked, seen & 1, err))) break;
+          if (tid == 0) mbar_arrive(&kv_full[slot]);
+          ++seen;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&looked);
-        if (!__all_sync(~0u, wait_bar(&looked, k & 1, err))) break;
-        if (masked && tid == 0) mbar_arrive(&kv_full[slot]);
         if (cur.last_of_item()) {
           fresh = true;
           ++items;
