@@ -198,6 +198,15 @@ __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
   hi = __float_as_uint(x) & 0xffffe000u;
   lo = __float_as_uint(x - __uint_as_float(hi)) + 0x1000u;
 }
+// The same for the operand that meets K and V (q, probabilities): a lower half
+// of zero would make NaN of an infinite one, so it gets 2^-40 of the upper
+// half, which is nothing beside the product that is left out. (An infinite x
+// has -0 for its lower half: the NaN of inf - inf and the half step.)
+__device__ __forceinline__ void split_first(float x, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xffffe000u;
+  const float h = __uint_as_float(hi);
+  lo = __float_as_uint(fmaf(h, 0x1p-40f, x - h)) + 0x1000u;
+}
 // d += a b of f32 operands: the small products first.
 __device__ __forceinline__ void mma8x3(float (&d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], float b0, float b1) {
   uint32_t h0, l0, h1, l1;
@@ -417,7 +426,7 @@ __global__ void __launch_bounds__(kThreads)
         uint32_t ah[4], al[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          split(lds_f32(sq + tile_at(MT, wm * 16 + g + 8 * (e & 1), kk * 2 + (e >> 1)) + 4 * t4), ah[e], al[e]);
+          split_first(lds_f32(sq + tile_at(MT, wm * 16 + g + 8 * (e & 1), kk * 2 + (e >> 1)) + 4 * t4), ah[e], al[e]);
 #pragma unroll
         for (int x = 0; x < NTW / 8; ++x) {
           const int tk = w0 + x * 8 + g;
@@ -493,10 +502,10 @@ __global__ void __launch_bounds__(kThreads)
       uint32_t ah[NTW / 8][4], al[NTW / 8][4];
 #pragma unroll
       for (int kk = 0; kk < NTW / 8; ++kk) {
-        split(s[kk][0], ah[kk][0], al[kk][0]);
-        split(s[kk][2], ah[kk][1], al[kk][1]);
-        split(s[kk][1], ah[kk][2], al[kk][2]);
-        split(s[kk][3], ah[kk][3], al[kk][3]);
+        split_first(s[kk][0], ah[kk][0], al[kk][0]);
+        split_first(s[kk][2], ah[kk][1], al[kk][1]);
+        split_first(s[kk][1], ah[kk][2], al[kk][2]);
+        split_first(s[kk][3], ah[kk][3], al[kk][3]);
       }
 #pragma unroll
       for (int x = 0; x < HD / 8; ++x) {

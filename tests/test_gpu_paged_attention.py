@@ -381,3 +381,41 @@ def test_caps_far_above_the_scores(dtype, hd, rows, cap):
     # the uncapped ones: 2 u of the largest value covers the capped ones.)
     assert ((got.double() - want).abs() <= torch.clamp(bound, min=2.1 * ref.EPS[dtype] * size) + 2.0 ** -16 * top * size).all()
     assert ((lse.double() - wlse).abs() <= 2.0 ** -18 * (1 + wlse.abs()) + 2.0 ** -17 * top).all()
+
+
+class Without:
+    """A cache of one sequence without its token t."""
+
+    def __init__(self, cache, t):
+        self.lens, self.c, self.t = [cache.lens[0] - 1], cache, t
+
+    def tokens(self, s):
+        k, v = self.c.tokens(0)
+        keep = torch.arange(k.shape[1], device=k.device) != self.t
+        return k[:, keep], v[:, keep]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 8, 40, 90])
+def test_infinite_keys_and_values_that_rows_see(dtype, hd, rows):
+    """A key of -inf has weight 0 and an infinite value is its rows' output,
+    also where the factor beside it is a power of two (a probability of 1, a
+    query of small integers), in tiles that no mask touches."""
+    dev = torch.device("cuda", 0)
+    n = 700
+    c = ref.Cache([n], 2, hd, 16, dtype, dev, seed=hd + rows)
+    q = torch.randint(1, 4, (rows, 4, hd), generator=torch.Generator().manual_seed(rows)).to(dtype).to(dev)
+
+    def token(t):
+        return c.rows[0][t // 16], t % 16
+    p, s = token(37)
+    c.k[p, :, s] = -math.inf
+    p, s = token(90)
+    c.k[p, :, s] = 40.0  # its probability is 1
+    c.v[p, :, s, 3] = math.inf
+    c.v[p, 0, s, 5] = -math.inf
+    c.v[p, 1, s, 7] = math.nan
+    got, lse = run(c, q, [rows])
+    agree(Without(c, 37), q, [rows], got, lse)
+    assert (got[:, :, 3] == math.inf).all() and (got[:, :2, 5] == -math.inf).all() and torch.isnan(got[:, 2:, 7]).all()
