@@ -493,7 +493,8 @@ RAI_API int rai_gpu_kv_copy_pages(const rai_page_pool* pool, const int32_t* src,
  * elements apart, any alignment), scores [batch][beams] f32 the beams' log
  * probabilities. Candidates (beam, token) are ordered by
  * scores[beam] + log softmax(logits[beam])[token] in 64 bits, equal ones by
- * logit, then by beam and token, lowest first. cand_* [batch][keep] the first
+ * logit, then by beam and token, lowest first (the scores that are
+ * written are f32 and, for vocabularies to 200,000, within 2^-16 of that). cand_* [batch][keep] the first
  * `keep`; score / parent / token [batch][beams] the first `beams` of those
  * whose token is not eos (-1: none is), parent as the sequence number
  * request * beams + beam, for rai_gpu_kv_fork. Places that nothing fills hold

@@ -10,9 +10,11 @@
 //
 // Order: by score in 64 bits, equal scores by logit, then by beam and token
 // (lowest first). Within a row the score grows with the logit, so a slice
-// only needs the logit and the token. Exponentials are 32-bit and their sums
-// 64-bit: the scores of different beams are then right to about 1e-8, which
-// keeps near ties in order.
+// only needs the logit and the token. Exponentials are 32-bit, so a row's
+// log-sum is right to lse_error() (some 1e-6) at first; where candidates of
+// different beams are nearer than that, the second kernel sums the rows of
+// these beams again in 64 bits (60 us for two rows of 151,936; few calls
+// have such candidates, but ones whose beams are equal do).
 #include <cuda_runtime.h>
 
 #include "paged.h"
@@ -22,6 +24,7 @@ namespace rai {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kStepElements = kThreads * 16;
 constexpr int kBufCap = 2048;  // candidates a slice holds between two sorts
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -38,9 +41,7 @@ __device__ __forceinline__ uint64_t key_of(float x, int token) {
 }
 
 // e^(x - m), where x = m also counts when both are infinite: a row with
-// infinite logits shares its mass among them, a row of -inf among all. (The
-// error of ex2.approx is the same function of x - m in every row: it all but
-// cancels between beams.)
+// infinite logits shares its mass among them, a row of -inf among all.
 __device__ __forceinline__ float exp_of(float d) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * kLog2e));
@@ -124,7 +125,7 @@ template <int DT>
 __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(BeamArgs a, int slices, int len) {
   constexpr int V = DT == kF32 ? 4 : 8;  // elements of 16 bytes
   constexpr int kE = DT == kF32 ? 4 : 2;
-  constexpr int N = 16, kVecs = N / V;   // elements and 16-byte loads of a thread in a step
+  constexpr int N = kStepElements / kThreads, kVecs = N / V;  // elements and 16-byte loads of a thread in a step
   __shared__ uint64_t buf[kBufCap];
   __shared__ uint64_t tops[kMaxKeep + 1];
   static_assert(kThreads / 4 == kMaxKeep, "groups");
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(BeamArgs a, int
   // Vector slots from the 16-byte boundary at or before the slice's start.
   const int off = (int)((reinterpret_cast<uintptr_t>(src + (long long)begin * kE) & 15) / kE);
   const int base = begin - off;
-  constexpr int kStep = kThreads * N;
+  constexpr int kStep = kStepElements;
   if (threadIdx.x == 0) count = 0;
   float m = -INFINITY;
   double sum = 0.0;
@@ -358,18 +359,54 @@ __device__ __forceinline__ Cand first_of_warp(const Cand& c) {
   return b;
 }
 
+// How far a row's log-sum may be off, by the steps of a thread of the pass. A
+// weight is the product of at most steps + 2 exponentials (its own, one for
+// each time its thread's maximum moved, one for the join), each off by 2^-22 of
+// itself and by 2.25 x 2^-24 of its argument (difference, product, constant).
+// The arguments of one weight add up to its distance from the maximum, whose
+// mean over the mass is at most ln(vocab). Five more roundings add 16 weights.
+__host__ __device__ inline double lse_error(int steps, int vocab) {
+  return ((steps + 2) * 4.0 + 2.25 * log((double)vocab) + 5.0) * 0x1p-24;
+}
+template <int DT>
+__device__ __forceinline__ float logit_at(const void* row, int i) {
+  if constexpr (DT == kF32) return static_cast<const float*>(row)[i];
+  else return to_f32<DT>(static_cast<const uint16_t*>(row)[i], 0);
+}
+// The sum of e^(x - top) over a row in 64 bits, by the CTA; the same for the
+// same logits wherever they lie. `top` is finite.
+__device__ __noinline__ double exact_sum(const void* row, int dtype, int vocab, float top, double* warps) {
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < vocab; i += blockDim.x) {
+    const float x = dtype == kF32 ? logit_at<kF32>(row, i) : dtype == kF16 ? logit_at<kF16>(row, i) : logit_at<kBF16>(row, i);
+    if (x == x) sum += exp((double)x - (double)top);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  double all = 0.0;
+  for (int w = 0; w < (int)blockDim.x >> 5; ++w) all += warps[w];
+  return all;
+}
+
+constexpr int kMergeThreads = 256;  // at least: the work but the lists' is shared among all
+
 // One CTA per request, one thread per (beam, slice) list; each round takes
 // the best of the lists' heads. Bound by the rounds' latency.
-__global__ void __launch_bounds__(kMaxBeams * kMaxSlices) beam_merge_kernel(BeamArgs a, int slices) {
+__global__ void __launch_bounds__(kMaxBeams * kMaxSlices) beam_merge_kernel(BeamArgs a, int slices, double error) {
   __shared__ double sums[kMaxBeams * kMaxSlices], lse[kMaxBeams];  // lse: log of the sum beside the maximum
   __shared__ float tops[kMaxBeams * kMaxSlices];
   __shared__ Cand warp_best[2][kMaxBeams * kMaxSlices / 32];
   __shared__ Cand chosen[kMaxKeep];
   __shared__ int next[kMaxBeams];
+  __shared__ uint32_t again;  // beams whose sums are needed in 64 bits
+  __shared__ double warp_sums[kMaxBeams * kMaxSlices / 32];
   __shared__ uint64_t heads[4096];  // the lists, where they fit
   pdl_wait_prior();
   pdl_launch_dependents();
-  const int req = blockIdx.x, lists = a.beams * slices, warps = blockDim.x >> 5;
+  const int req = blockIdx.x, lists = a.beams * slices, warps = (lists + 31) / 32;  // that hold lists
   const size_t sb = slice_bytes(a.keep);
   const char* ws = static_cast<const char*>(a.ws) + (long long)req * lists * sb;
   const bool real = (int)threadIdx.x < lists;
@@ -383,6 +420,7 @@ __global__ void __launch_bounds__(kMaxBeams * kMaxSlices) beam_merge_kernel(Beam
     if (!(score == score)) score = -INFINITY;
     tops[threadIdx.x] = s.max;
   }
+  if (threadIdx.x == 0) again = 0;
   const bool fits = lists * a.keep <= 4096;
   if (fits)
     for (int i = threadIdx.x; i < lists * a.keep; i += blockDim.x)
@@ -415,24 +453,58 @@ __global__ void __launch_bounds__(kMaxBeams * kMaxSlices) beam_merge_kernel(Beam
     c.score = ordered((double)score + (d - lse[beam]));
     return c;
   };
-  Cand mine = head();
-  for (int r = 0; r < a.keep; ++r) {
-    Cand best = first_of_warp(mine);
-    if (warps > 1) {
-      // Every warp reads all warps' best; two buffers, so one barrier a round.
-      const int lane = threadIdx.x & 31;
-      if (lane == 0) warp_best[r & 1][threadIdx.x >> 5] = best;
-      __syncthreads();
-      Cand c;
-      c.flat = 0xffffffffu;
-      if (lane < warps) c = warp_best[r & 1][lane];
-      best = first_of_warp(c);
+  Cand mine;
+  auto choose = [&]() {
+    at = 0;
+    mine = head();
+    for (int r = 0; r < a.keep; ++r) {
+      Cand best = first_of_warp(mine);
+      if (warps > 1) {
+        // Every warp reads all warps' best; two buffers, so one barrier a round.
+        const int lane = threadIdx.x & 31;
+        if (lane == 0) warp_best[r & 1][threadIdx.x >> 5] = best;
+        asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
+        Cand c;
+        c.flat = 0xffffffffu;
+        if (lane < warps) c = warp_best[r & 1][lane];
+        best = first_of_warp(c);
+      }
+      if (threadIdx.x == 0) chosen[r] = best;
+      if (best.score && best.flat == mine.flat) {
+        ++at;
+        mine = head();
+      }
     }
-    if (threadIdx.x == 0) chosen[r] = best;
-    if (best.score && best.flat == mine.flat) {
-      ++at;
-      mine = head();
+  };
+  if ((int)threadIdx.x < warps * 32) choose();
+  __syncthreads();
+  // Candidates of different beams that the sums' error may have put in the
+  // wrong order: neighbours among the chosen ones, and a list's first one left
+  // against the last one chosen of another beam. (Equal scores of -inf are
+  // equal whatever the sums; their difference is NaN.)
+  auto near = [&](const Cand& x, const Cand& y) { return y.score && unordered(x.score) - unordered(y.score) <= 2.0 * error; };
+  auto beam_of = [&](const Cand& c) { return (int)c.flat / a.vocab; };
+  if ((int)threadIdx.x + 1 < a.keep) {
+    const Cand x = chosen[threadIdx.x], y = chosen[threadIdx.x + 1];
+    if (near(x, y) && beam_of(x) != beam_of(y)) atomicOr(&again, 1u << beam_of(x) | 1u << beam_of(y));
+  }
+  if (real && mine.score && near(chosen[a.keep - 1], mine)) {
+    for (int r = a.keep - 1; r >= 0 && near(chosen[r], mine); --r)
+      if (beam_of(chosen[r]) != beam) atomicOr(&again, 1u << beam_of(chosen[r]) | 1u << beam);
+  }
+  __syncthreads();
+  if (again) {
+    for (int b = 0; b < a.beams; ++b) {
+      if (!(again >> b & 1u)) continue;
+      float m = -INFINITY;
+      for (int i = 0; i < slices; ++i) m = fmaxf(m, tops[b * slices + i]);
+      if (!(fabsf(m) <= 3.4028235e38f)) continue;  // a number of equal ones: exact
+      const char* row = static_cast<const char*>(a.logits) + (long long)(req * a.beams + b) * a.row * (a.dtype == kF32 ? 4 : 2);
+      const double sum = exact_sum(row, a.dtype, a.vocab, m, warp_sums);
+      if (threadIdx.x == 0) lse[b] = log(sum);
     }
+    __syncthreads();
+    if ((int)threadIdx.x < warps * 32) choose();
   }
   __syncthreads();
   for (int r = threadIdx.x; r < a.keep; r += blockDim.x) {
@@ -515,7 +587,8 @@ cudaError_t beam_select(const BeamArgs& a, cudaStream_t s) {
                                     : launch_pdl(beam_slice_kernel<kBF16>, grid, dim3(kThreads), 0, s, a, slices, len);
   if (e != cudaSuccess) return e;
   const int lists = a.beams * slices;
-  return launch_pdl(beam_merge_kernel, dim3(a.batch), dim3((lists + 31) / 32 * 32), 0, s, a, slices);
+  const int threads = lists > kMergeThreads ? (lists + 31) / 32 * 32 : kMergeThreads;
+  return launch_pdl(beam_merge_kernel, dim3(a.batch), dim3(threads), 0, s, a, slices, lse_error((len + kStepElements - 1) / kStepElements + 1, a.vocab));
 }
 
 }  // namespace rai

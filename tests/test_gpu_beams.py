@@ -185,3 +185,23 @@ def test_on_two_streams_at_once():
         for r in rs:
             for a, b in zip(w[:6], r[:6]):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("N,V", [(4, 3001), (8, 500), (2, 152001), (32, 4097)])
+@pytest.mark.parametrize("peak", [0.0, 12.0])
+def test_beams_nearer_than_32_bits(dtype, N, V, peak):
+    """Beam scores set so that the best candidates of different beams are at
+    the same sum but for the scores' own rounding (1e-7 and less), on flat
+    rows and on rows where a few tokens hold the mass."""
+    g = torch.Generator().manual_seed(V)
+    B = 24 if V < 10000 else 6
+    x = 2 * torch.randn((B, N, V), generator=g)
+    for i in range(3):
+        at = torch.randint(0, V, (B, N, 1), generator=g)
+        x.scatter_(2, at, peak + torch.rand((B, N, 1), generator=g))
+    x = x.to(dtype)
+    y = x.double()
+    s = (-4.0 - (y.amax(2) - torch.logsumexp(y, 2))).float()
+    check(x.cuda(), s.cuda(), eos=V // 2)
+    check(x.cuda(), s.cuda(), keep=N)
