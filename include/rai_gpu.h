@@ -498,7 +498,8 @@ RAI_API int rai_gpu_kv_copy_pages(const rai_page_pool* pool, const int32_t* src,
  * `keep`; score / parent / token [batch][beams] the first `beams` of those
  * whose token is not eos (-1: none is), parent as the sequence number
  * request * beams + beam, for rai_gpu_kv_fork. Places that nothing fills hold
- * -infinity and -1. NaN logits and scores count as -infinity; in a row with
+ * -infinity and -1. NaN logits and scores count as -infinity, and so does
+ * what has no weight in a beam of score +infinity; in a row with
  * +infinity those share the mass, a row of -infinity is uniform (the
  * degenerate rows of softmax_probabilities, rai-infer/src/speculative.rs).
  * history (may be NULL): int32 [batch * beams][.] with hist_len tokens a

@@ -460,7 +460,8 @@ __global__ void __launch_bounds__(kMaxBeams * kMaxSlices) beam_merge_kernel(Beam
     c.flat = (uint32_t)(beam * a.vocab) + (0xffffffffu - (uint32_t)k);
     const float x = unordered(c.logit);
     const double d = x == top ? 0.0 : (double)x - (double)top;
-    c.score = ordered((double)score + (d - lse[beam]));
+    const double total = (double)score + (d - lse[beam]);
+    c.score = ordered(total == total ? total : -INFINITY);  // (a beam of +infinity, a token of weight 0)
     return c;
   };
   Cand mine;

@@ -205,3 +205,25 @@ def test_beams_nearer_than_32_bits(dtype, N, V, peak):
     s = (-4.0 - (y.amax(2) - torch.logsumexp(y, 2))).float()
     check(x.cuda(), s.cuda(), eos=V // 2)
     check(x.cuda(), s.cuda(), keep=N)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_beams_of_infinite_score(dtype):
+    """What a grammar took out of a beam of +infinity is not chosen before what
+    it left."""
+    from rai_b200 import beams
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn((1, 2, 500), generator=g).to(dtype)
+    x[:, :, 7:] = -math.inf
+    s = torch.tensor([[-1.0, math.inf]])
+    r = beams.select(x.cuda(), s.cuda(), keep=16)
+    left = sorted(range(7), key=lambda t: (-x[0, 1, t].item(), t))
+    assert r.cand_beams[0, :7].tolist() == [1] * 7 and r.cand_tokens[0, :7].tolist() == left
+    assert (r.cand_scores[0, :7] == math.inf).all()
+    other = sorted(range(7), key=lambda t: (-x[0, 0, t].item(), t))
+    assert r.cand_beams[0, 7:14].tolist() == [0] * 7 and r.cand_tokens[0, 7:14].tolist() == other
+    assert (r.cand_scores[0, 14:] == -math.inf).all() and not torch.isnan(r.scores).any()
+    assert r.parents[0].tolist() == [1, 1] and r.tokens[0].tolist() == left[:2]
+    one = beams.select(x[:, 1:].cuda(), s[:, 1:].cuda(), keep=16)
+    assert one.cand_tokens[0].tolist() == left + list(range(7, 16))
+    assert (one.cand_scores[0, :7] == math.inf).all() and (one.cand_scores[0, 7:] == -math.inf).all()
