@@ -78,6 +78,11 @@ void no_gradient(const Tensor& t, const char* name) {
   if (t.requires_grad() && at::GradMode::is_enabled())
     bad(std::string(name) + ": this operator has no gradient; call it under torch.no_grad()");
 }
+// Pages are read, and by most calls written: neither with a gradient.
+void no_gradient(const Tensor& k, const Tensor& v) {
+  no_gradient(k, "k_pages");
+  no_gradient(v, "v_pages");
+}
 void rows3(const Tensor& t, int64_t heads, int64_t dim, const char* name) {
   if (t.dim() != 3 || t.size(2) != dim || (heads >= 0 && t.size(1) != heads))
     bad(std::string(name) + ": [rows, heads, head_dim] that fits the pages");
@@ -119,6 +124,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
   need(k.dim() == 4, "k_pages, v_pages: two tensors [pages, kv_heads, page_size, head_dim] of one shape and type");
   const int64_t hd = k.size(3);
   dtype_of(k, "k_pages");
+  no_gradient(k, v);
   rows3(q, -1, hd, "q");
   need(q.scalar_type() == k.scalar_type(), "q: the type of the pages");
   const int64_t rows = q.size(0), heads = q.size(1);
@@ -126,6 +132,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
   on_device(out_in, dev);
   on_device(lse, dev);
   on_device(ws_in, dev);
+  if (lse) no_gradient(*lse, "lse");
   if (out_in) {
     rows3(*out_in, heads, hd, "out");
     need(out_in->size(0) == rows && out_in->scalar_type() == q.scalar_type(), "out: shape and type of q");
@@ -174,6 +181,8 @@ Tensor rope_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   need(k_pages.dim() == 4, "k_pages, v_pages: two tensors [pages, kv_heads, page_size, head_dim] of one shape and type");
   const int64_t hd = k_pages.size(3), nkv = k_pages.size(1);
   dtype_of(k_pages, "k_pages");
+  no_gradient(k_pages, v_pages);
+  no_gradient(inv_freq, "inv_freq");
   rows3(q, -1, hd, "q");
   rows3(k, nkv, hd, "k");
   rows3(v, nkv, hd, "v");
@@ -264,6 +273,7 @@ std::tuple<Tensor, Tensor> kv_fork(const Tensor& table, const Tensor& lens, cons
 
 Tensor kv_resize(const Tensor& table, const Tensor& lens, const Tensor& refs, const Tensor& k, const Tensor& v, int64_t delta,
               const OptTensor& new_lens, const OptTensor& ws_in) {
+  no_gradient(k, v);
   const c10::DeviceIndex dev = device_of(table, lens, refs, k, v);
   on_device(new_lens, dev);
   on_device(ws_in, dev);
@@ -280,6 +290,7 @@ Tensor kv_resize(const Tensor& table, const Tensor& lens, const Tensor& refs, co
 }
 
 Tensor kv_compact(const Tensor& table, const Tensor& lens, const Tensor& refs, const Tensor& k, const Tensor& v, const OptTensor& ws_in) {
+  no_gradient(k, v);
   const c10::DeviceIndex dev = device_of(table, lens, refs, k, v);
   on_device(ws_in, dev);
   const auto [pool, page] = pool_of(k, v);
@@ -293,6 +304,7 @@ Tensor kv_compact(const Tensor& table, const Tensor& lens, const Tensor& refs, c
 }
 
 void copy_pages(const Tensor& k, const Tensor& v, const Tensor& src, const Tensor& dst) {
+  no_gradient(k, v);
   const c10::DeviceIndex dev = device_of(k, v, src, dst);
   const auto [pool, page] = pool_of(k, v);
   need(src.dim() == 1, "src: a vector");
@@ -313,6 +325,7 @@ py::tuple beam_select(const Tensor& logits, const Tensor& scores, std::optional<
   need(scores.scalar_type() == at::kFloat && scores.dim() == 2 && scores.size(0) == b && scores.size(1) == n && scores.is_contiguous(),
        "scores: contiguous float32 [batch, beams]");
   no_gradient(logits, "logits");
+  no_gradient(scores, "scores");
   const c10::DeviceIndex dev = device_of(logits, scores);
   on_device(history, dev);
   on_device(hist_len, dev);

@@ -257,3 +257,35 @@ for hd in (64, 128, 256):
 @pytest.mark.parametrize("cap", [1e-40, -1e-40, -0.5, math.nan])
 def test_attention_refuses_caps_without_a_reciprocal(cap):
     assert attn(softcap=cap) == I
+
+
+def test_tensors_with_a_gradient_are_refused():
+    """The operators have no backward pass: a gradient would be lost."""
+    torch = pytest.importorskip("torch")
+    from rai_b200 import beams, paged
+    i32 = dict(dtype=torch.int32)
+    q = torch.zeros(2, 4, 64)
+    kx = torch.zeros(2, 2, 64)
+    k = torch.zeros(3, 2, 8, 64)
+    grad = torch.zeros(3, 2, 8, 64, requires_grad=True)
+    t, n, s, refs = torch.zeros(1, 2, **i32), torch.ones(1, **i32), torch.zeros(2, **i32), torch.zeros(3, **i32)
+    inv = torch.zeros(32)
+    calls = [lambda a, b: paged.attention(q, a, b, t, n, s, 2), lambda a, b: paged.rope_append(q, kx, kx, a, b, t, n, s, inv),
+             lambda a, b: paged.resize(t, n, refs, a, b, delta=1), lambda a, b: paged.compact(t, n, refs, a, b),
+             lambda a, b: paged.copy_pages(a, b, n, n)]
+    for call in calls:
+        for a, b in ((grad, k), (k, grad)):
+            with pytest.raises(ValueError, match="no gradient"):
+                call(a, b)
+            with torch.no_grad(), pytest.raises(ValueError, match="device"):
+                call(a, b)
+    for call in (lambda: paged.rope_append(q, kx, kx, k, k, t, n, s, inv.clone().requires_grad_()),
+                 lambda: paged.attention(q, k, k, t, n, s, 2, lse=torch.zeros(2, 4, requires_grad=True)),
+                 lambda: beams.select(torch.zeros(1, 2, 9), torch.zeros(1, 2, requires_grad=True)),
+                 lambda: beams.select(torch.zeros(1, 2, 9, requires_grad=True), torch.zeros(1, 2))):
+        with pytest.raises(ValueError, match="no gradient|device"):
+            call()
+    with pytest.raises(ValueError, match="scores: .*no gradient"):
+        beams.select(torch.zeros(1, 2, 9), torch.zeros(1, 2, requires_grad=True))
+    with pytest.raises(ValueError, match="inv_freq: .*no gradient"):
+        paged.rope_append(q, kx, kx, k, k, t, n, s, inv.clone().requires_grad_())
