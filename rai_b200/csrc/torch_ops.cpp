@@ -78,6 +78,12 @@ void no_gradient(const Tensor& t, const char* name) {
   if (t.requires_grad() && at::GradMode::is_enabled())
     bad(std::string(name) + ": this operator has no gradient; call it under torch.no_grad()");
 }
+// A call writes t in place: a graph that has saved it has to notice.
+// (Inference tensors count no versions.)
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // Pages are read, and by most calls written: neither with a gradient.
 void no_gradient(const Tensor& k, const Tensor& v) {
   no_gradient(k, "k_pages");
@@ -160,6 +166,8 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
   }
   if (ws.defined()) a.workspace = ws.data_ptr(), a.workspace_bytes = ws.nbytes();
   check(rai_gpu_paged_attention(&a, on.stream));
+  if (out_in) written(*out_in);
+  if (lse) written(*lse);
   return out;
 }
 
@@ -208,6 +216,8 @@ Tensor rope_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   a.n_heads = u32(heads, "heads"), a.rot_dim = u32(2 * inv_freq.size(0), "inv_freq");
   a.interleaved = interleaved, a.in_dtype = dtype_of(q, "q"), a.mscale = (float)mscale;
   check(rai_gpu_rope_append(&a, on.stream));
+  written(k_pages), written(v_pages);
+  if (out_in) written(*out_in);
   return out;
 }
 
@@ -268,6 +278,9 @@ std::tuple<Tensor, Tensor> kv_fork(const Tensor& table, const Tensor& lens, cons
   Tensor out_lens = lens_in ? *lens_in : at::empty({n}, lens.options());
   const rai_page_table a = table_of(table, lens, refs, page_size), b = table_of(out, out_lens, refs, page_size);
   check(rai_gpu_kv_fork(&a, &b, ints(parents, n, "parents"), on.stream));
+  written(refs);
+  if (table_in) written(*table_in);
+  if (lens_in) written(*lens_in);
   return {out, out_lens};
 }
 
@@ -286,6 +299,7 @@ Tensor kv_resize(const Tensor& table, const Tensor& lens, const Tensor& refs, co
   Tensor ws = ws_in ? *ws_in : bytes(rai_gpu_kv_resize_workspace_bytes(t.n_seqs), lens);
   check(rai_gpu_kv_resize(&t, &pool, new_lens ? ints(*new_lens, t.n_seqs, "new_lens") : nullptr, (int32_t)delta,
                           status.data_ptr<int32_t>(), ws.data_ptr(), ws.nbytes(), on.stream));
+  for (const Tensor* x : {&table, &lens, &refs, &k, &v}) written(*x);
   return status;
 }
 
@@ -300,6 +314,7 @@ Tensor kv_compact(const Tensor& table, const Tensor& lens, const Tensor& refs, c
   if (ws_in) need(ws_in->is_contiguous(), "workspace: contiguous");
   Tensor ws = ws_in ? *ws_in : bytes(rai_gpu_kv_compact_workspace_bytes(t.n_pages), refs);
   check(rai_gpu_kv_compact(&t, &pool, used.data_ptr<int32_t>(), ws.data_ptr(), ws.nbytes(), on.stream));
+  for (const Tensor* x : {&table, &refs, &k, &v}) written(*x);
   return used;
 }
 
@@ -310,6 +325,7 @@ void copy_pages(const Tensor& k, const Tensor& v, const Tensor& src, const Tenso
   need(src.dim() == 1, "src: a vector");
   On on(dev);
   check(rai_gpu_kv_copy_pages(&pool, ints(src, src.size(0), "src"), ints(dst, src.size(0), "dst"), (size_t)src.size(0), on.stream));
+  written(k), written(v);
 }
 
 py::tuple beam_select(const Tensor& logits, const Tensor& scores, std::optional<int64_t> keep_in, int64_t eos, const OptTensor& history,

@@ -399,3 +399,35 @@ def test_fork_into_given_outputs(children):
     assert got[0].data_ptr() == out.data_ptr() and got[1].data_ptr() == n.data_ptr()
     check_pages(want, out, n, c.refs)
     assert (wide[:, width:] == 77).all()
+
+
+def test_a_graph_notices_pages_that_were_written():
+    """Pages saved for a backward pass and written since: an error, as for any
+    operation in place; inference tensors stay allowed."""
+    from rai_b200 import paged
+    dev = torch.device("cuda", 0)
+    c = ref.Cache([20, 9], 1, 64, 16, torch.float32, dev, junk=0.0)
+    inv = torch.from_numpy(paged.rope_frequencies(64)[0]).to(dev)
+    q, k = torch.randn((2, 2, 64), device=dev), torch.randn((2, 1, 64), device=dev)
+    starts = ref.starts_of([1, 1], dev)
+    one = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = torch.zeros_like(q)
+    calls = [(lambda: paged.rope_append(q, k, k, c.k, c.v, c.table, c.kv_len, starts, inv), (c.k, c.v)),
+             (lambda: paged.rope_append(q, k, k, c.k, c.v, c.table, c.kv_len, starts, inv, q_out=out), (out, c.k)),
+             (lambda: paged.attention(q, c.k, c.v, c.table, c.kv_len, starts, 1, out=out), (out,)),
+             (lambda: paged.copy_pages(c.k, c.v, one, one + 1), (c.k, c.v)),
+             (lambda: paged.resize(c.table, c.kv_len, c.refs, c.k, c.v, delta=0), (c.k, c.v, c.table, c.kv_len, c.refs)),
+             (lambda: paged.compact(c.table, c.kv_len, c.refs, c.k, c.v), (c.k, c.v, c.table, c.refs))]
+    for call, tensors in calls:
+        before = [t._version for t in tensors]
+        call()
+        assert all(t._version > b for t, b in zip(tensors, before))
+    w = torch.ones(64, device=dev, requires_grad=True)
+    loss = (w * c.k).sum()
+    paged.copy_pages(c.k, c.v, one, one + 1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        ks, vs = c.k.clone(), c.v.clone()
+    paged.copy_pages(ks, vs, one, one + 1)
+    assert torch.equal(ks[1], ks[0])
