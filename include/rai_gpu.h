@@ -349,8 +349,10 @@ RAI_API int rai_gpu_step_kernel_count(const rai_dec* dec, size_t* kernels);
  * keep nothing between calls; call them with the stream's device current.
  * (The first call on a device looks up the status word: make one before
  * capturing a stream.) Workspaces need no initialisation; calls that may
- * overlap on the GPU need one each. Addresses and strides: the innermost dimension is contiguous,
- * every row of a tensor starts on a 16-byte boundary. */
+ * overlap on the GPU need one each. Addresses and strides: the innermost
+ * dimension is contiguous, every row of a tensor starts on a 16-byte
+ * boundary, rows that are written lie apart (rows that are only read may
+ * share memory, a stride of 0 included). */
 enum { RAI_F32 = 0, RAI_F16 = 1, RAI_BF16 = 2 };
 
 /* One layer's pages and a ragged chunk of new rows. Sequence s has the rows
@@ -377,7 +379,8 @@ typedef struct {
  * of a sequence sees the tokens up to its own position, with window > 0 only
  * the last `window` of them. scores = scale * q.k, with softcap > 0
  * softcap * tanh(scale * q.k / softcap). q and out [rows][n_heads][head_dim]
- * in the pages' dtype; lse (f32 [rows][n_heads], may be NULL) the natural
+ * in the pages' dtype, out another memory than the inputs or q itself (same
+ * strides); lse (f32 [rows][n_heads], may be NULL) the natural
  * logarithm of the row's sum of exponentials. A row at a negative position
  * (kv_len below the row count) sees nothing: its output is 0, its lse
  * -infinity. What a row may not see does not reach its output, whatever it

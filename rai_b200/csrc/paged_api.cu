@@ -2,6 +2,7 @@
 // launches of kernels_paged_*.cu and kernels_beam.cu.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -77,6 +78,21 @@ bool overlap(const void* a, size_t na, const void* b, size_t nb) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
   return x < y + nb && y < x + na;
 }
+// Whether the rows of `inner` elements of a tensor that is written lie apart:
+// each stride, from the smallest, passes what lies below it.
+struct Dim {
+  int64_t stride, count;
+};
+template <int N>
+bool apart(int64_t inner, Dim (&&dims)[N]) {
+  std::sort(dims, dims + N, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+  for (const Dim& d : dims) {
+    if (d.count <= 1) continue;
+    if (d.stride < inner) return false;
+    inner += (d.count - 1) * d.stride;
+  }
+  return true;
+}
 size_t table_bytes(const rai_page_table& t) { return ((size_t)(t.n_seqs - 1) * t.table_stride + t.max_pages) * 4; }
 
 int attention_args(const rai_paged_attention* a, rai::AttnArgs* out) {
@@ -88,6 +104,7 @@ int attention_args(const rai_paged_attention* a, rai::AttnArgs* out) {
   if (!vec_stride(a->q_row, elt) || !vec_stride(a->q_head, elt) || !vec_stride(a->out_row, elt) ||
       !vec_stride(a->out_head, elt) || !aligned(a->q, 16) || !aligned(a->out, 16))
     return bad("q, out: every vector has to start on a 16-byte boundary");
+  if (!apart(a->chunk.head_dim, {{a->out_row, a->chunk.rows}, {a->out_head, a->n_heads}})) return bad("out: rows share memory");
   if ((uint64_t)a->chunk.n_seqs * (((uint64_t)a->chunk.max_rows * (a->n_heads / a->chunk.n_kv_heads) + 15) / 16) > (1u << 30))
     return bad("n_seqs * max_rows is out of range");
   if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return bad("scale has to be positive");
@@ -184,6 +201,11 @@ int rai_gpu_rope_append(const rai_rope_append* a, void* stream) {
     o.v_row = a->v_row, o.v_head = a->v_head, o.o_row = a->out_row, o.o_head = a->out_head;
     if (a->q_out == a->q && (ei != eo || a->q_row != a->out_row || a->q_head != a->out_head || a->in_dtype != a->chunk.dtype))
       return bad("q_out is q with other strides or another type");
+    const rai_paged_chunk& c = a->chunk;
+    if (!apart(c.head_dim, {{a->out_row, c.rows}, {a->out_head, a->n_heads}})) return bad("q_out: rows share memory");
+    if (!apart(c.head_dim, {{c.k_page, c.n_pages}, {c.k_head, c.n_kv_heads}, {c.k_slot, c.page_size}}) ||
+        !apart(c.head_dim, {{c.v_page, c.n_pages}, {c.v_head, c.n_kv_heads}, {c.v_slot, c.page_size}}) || c.k == c.v)
+      return bad("pages: vectors share memory");
     o.heads = (int)a->n_heads, o.rot = (int)a->rot_dim, o.interleaved = a->interleaved != 0;
     o.in_dtype = (int)a->in_dtype, o.cache_dtype = (int)a->chunk.dtype, o.mscale = a->mscale;
     if (int rc = rai::kernel_status_word(&o.c.err)) return rc;
@@ -238,6 +260,9 @@ int rai_gpu_kv_fork(const rai_page_table* in, const rai_page_table* out, const i
     if (overlap(in->table, table_bytes(*in), out->table, table_bytes(*out)) ||
         overlap(in->lens, in->n_seqs * 4ull, out->lens, out->n_seqs * 4ull))
       return bad("fork: the new table and lengths need their own memory");
+    if (overlap(parents, out->n_seqs * 4ull, out->table, table_bytes(*out)) ||
+        overlap(parents, out->n_seqs * 4ull, out->lens, out->n_seqs * 4ull))
+      return bad("fork: the new table and lengths need their own memory");
     if (int rc = rai::kernel_status_word(&a.err)) return rc;
     b.err = a.err;
     return done(rai::kv_fork(a, b, parents, static_cast<cudaStream_t>(stream)));
@@ -258,6 +283,8 @@ int rai_gpu_kv_resize(const rai_page_table* table, const rai_page_pool* pool, co
     if (!status) return bad("null argument");
     if (t.n_seqs > rai::kMaxTableSeqs) return unsupported("resize: at most 4096 sequences");
     if (!ws || !aligned(ws, 4) || ws_bytes < rai::kv_resize_workspace(t.n_seqs)) return bad("workspace is too small");
+    if (new_lens && new_lens != t.lens && overlap(new_lens, t.n_seqs * 4ull, t.lens, t.n_seqs * 4ull))
+      return bad("resize: the new lengths overlap the old ones");
     if (int rc = rai::kernel_status_word(&t.err)) return rc;
     return done(rai::kv_resize(t, p, new_lens, delta, status, ws, static_cast<cudaStream_t>(stream)));
   });

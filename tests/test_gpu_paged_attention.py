@@ -419,3 +419,39 @@ def test_infinite_keys_and_values_that_rows_see(dtype, hd, rows):
     got, lse = run(c, q, [rows])
     agree(Without(c, 37), q, [rows], got, lse)
     assert (got[:, :, 3] == math.inf).all() and (got[:, :2, 5] == -math.inf).all() and torch.isnan(got[:, 2:, 7]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("hd,rows,lens", [(64, [1, 5, 1], [3000, 900, 40]), (128, [2, 300, 1], [9000, 700, 64]), (128, [1, 9, 4], [9000, 9000, 700])])
+def test_output_in_place_of_the_queries(dtype, hd, rows, lens):
+    from rai_b200 import paged
+    dev = torch.device("cuda", 0)
+    c = ref.Cache(lens, 2, hd, 16, dtype, dev, seed=hd, wide=3000)
+    big = make_q(sum(rows), 12, hd, dtype, dev)
+    q = big[:, 2:10]
+    want = paged.attention(q, c.k, c.v, c.table, c.kv_len, ref.starts_of(rows, dev), max(rows))
+    rest = big[:, 10:].clone()
+    got = paged.attention(q, c.k, c.v, c.table, c.kv_len, ref.starts_of(rows, dev), max(rows), out=q)
+    paged.status()
+    assert got.data_ptr() == q.data_ptr() and torch.equal(got, want) and torch.equal(big[:, 10:], rest)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("hd,rows", [(64, [1, 5]), (128, [2, 200])])
+def test_pages_that_heads_share(dtype, hd, rows):
+    """One KV head's pages expanded to four (a stride of 0) are read as if
+    copied; the same as an output is refused."""
+    import rai_b200
+    from rai_b200 import paged
+    dev = torch.device("cuda", 0)
+    c = ref.Cache([700, 300], 1, hd, 16, dtype, dev, seed=hd)
+    q = make_q(sum(rows), 8, hd, dtype, dev)
+    starts = ref.starts_of(rows, dev)
+    k, v = (t.expand(-1, 4, -1, -1) for t in (c.k, c.v))
+    got = paged.attention(q, k, v, c.table, c.kv_len, starts, max(rows))
+    full = ref.Cache([700, 300], 4, hd, 16, dtype, dev)
+    full.k, full.v, full.rows = k, v, c.rows
+    want, bound, _ = ref.attention(q, full, rows, hd ** -0.5)
+    assert ((got.double() - want).abs() <= bound).all()
+    with pytest.raises(rai_b200.RaiError):
+        paged.attention(q, k, v, c.table, c.kv_len, starts, max(rows), out=torch.zeros_like(q[:, :1]).expand(-1, 8, -1))

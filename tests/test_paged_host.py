@@ -289,3 +289,23 @@ def test_tensors_with_a_gradient_are_refused():
         beams.select(torch.zeros(1, 2, 9), torch.zeros(1, 2, requires_grad=True))
     with pytest.raises(ValueError, match="inv_freq: .*no gradient"):
         paged.rope_append(q, kx, kx, k, k, t, n, s, inv.clone().requires_grad_())
+
+
+def test_written_rows_that_share_memory_are_refused():
+    """Strides of 0 (expanded tensors) or below a row, where a call writes;
+    reading such pages is fine."""
+    assert attn(out_row=0) == I and "share" in native.last_error()
+    assert attn(out_head=0) == I and "share" in native.last_error()
+    assert attn(out_head=32, out_row=256) == I and "share" in native.last_error()
+    assert attn(out_row=192) == I and "share" in native.last_error()
+    assert rope(dict(v=2 * P), out_row=0) == I and "share" in native.last_error()
+    for kw in (dict(k_head=0), dict(v_slot=0), dict(k_page=0), dict(v_page=512)):
+        assert rope(dict(v=2 * P, **kw)) == I and "share" in native.last_error(), kw
+    assert rope() == I and "share" in native.last_error()  # k and v pages in one memory
+    L = native.lib()
+    far = dict(table=P + 4096, lens=P + 8192)
+    for parents in (P + 4096, P + 4100, P + 8192, P + 8200):
+        assert L.rai_gpu_kv_fork(C.byref(table()), C.byref(table(**far)), parents, None) == I
+    ws = L.rai_gpu_kv_resize_workspace_bytes(3)
+    assert L.rai_gpu_kv_resize(C.byref(table()), C.byref(pool()), P + 4, 0, P, P, ws, None) == I
+    assert "overlap" in native.last_error()
