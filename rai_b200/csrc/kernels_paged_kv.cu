@@ -268,7 +268,7 @@ __device__ __forceinline__ bool good_page(const TableArgs& t, int page) {
 
 // CTA i: child i's table row, and parent i's change of references (its
 // children less one for each page). Integer sums: the order does not matter.
-__global__ void __launch_bounds__(256) kv_fork_kernel(TableArgs in, TableArgs out, const int* __restrict__ parents) {
+__global__ void __launch_bounds__(256) kv_fork_kernel(TableArgs in, TableArgs out, const int* parents) {
   pdl_wait_prior();
   pdl_launch_dependents();
   const int i = blockIdx.x;
@@ -383,7 +383,7 @@ __device__ __forceinline__ int warp_scan(int v, int* sh, int* total) {
 // that is partly filled (all holders but the last copy it), then new pages.
 // Copies are listed as (src, dst) for kv_copy_kernel: ws = [count, src[n],
 // dst[n]].
-__global__ void __launch_bounds__(kMetaThreads) kv_resize_kernel(TableArgs t, const int* __restrict__ new_lens,
+__global__ void __launch_bounds__(kMetaThreads) kv_resize_kernel(TableArgs t, const int* new_lens,
                                                                  int delta, int* status, int* ws) {
   __shared__ int tail[kMaxTableSeqs];   // page to copy on write, or -1
   __shared__ int place[kMaxTableSeqs];  // exclusive sum of the pages that sequences take
@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(kMetaThreads) kv_compact_kernel(TableArgs t, i
   pdl_launch_dependents();
 }
 
-__global__ void __launch_bounds__(256) kv_rename_kernel(TableArgs t, const int* __restrict__ moved) {
+__global__ void __launch_bounds__(256) kv_rename_kernel(TableArgs t, const int* moved) {
   pdl_wait_prior();
   pdl_launch_dependents();
   for (int s = blockIdx.x; s < t.n_seqs; s += gridDim.x) {
@@ -565,9 +565,9 @@ __global__ void __launch_bounds__(256) kv_rename_kernel(TableArgs t, const int* 
 constexpr int kCopyThreads = 256;
 constexpr int kCopyVecs = 8;
 constexpr long long kPiece = kCopyThreads * kCopyVecs * 16ll;
-__global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(PagePool pool, const int* __restrict__ src,
-                                                               const int* __restrict__ dst,
-                                                               const int* __restrict__ n_dev, int n, uint32_t* err) {
+__global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(PagePool pool, const int* src,
+                                                               const int* dst,
+                                                               const int* n_dev, int n, uint32_t* err) {
   pdl_wait_prior();
   pdl_launch_dependents();
   const int pairs = n_dev ? min(max(*n_dev, 0), n) : n;

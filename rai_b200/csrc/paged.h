@@ -13,6 +13,10 @@
 
 #include "common.cuh"
 
+// Kernels here are launched while their predecessors still run, so what these
+// write (tables, lists of copies) is read by plain loads behind the wait, not by
+// __ldg or through __restrict__: read-only loads want memory that does not
+// change while the kernel runs, and may be moved ahead of the wait.
 namespace rai {
 
 enum : int { kF32 = 0, kF16 = 1, kBF16 = 2 };  // RAI_F32, RAI_F16, RAI_BF16

@@ -169,7 +169,7 @@ struct TilePages {
     for (int i = 0; i < NT / 32; ++i) {
       const int t = t0 + lane + 32 * i;
       page[i] = -1;
-      if (t >= it.lo && t < it.hi) page[i] = __ldg(c.table + (long long)it.seq * c.table_stride + c.page.quot(t));
+      if (t >= it.lo && t < it.hi) page[i] = c.table[(long long)it.seq * c.table_stride + c.page.quot(t)];
     }
   }
   __device__ __forceinline__ void check(const PagedChunk& c, const Item& it, int t0, int lane) {
@@ -313,7 +313,7 @@ struct TilePieces {
     page = -1;
     if (!mine(box, lane, &block, &piece)) return;
     const int t = t0 + piece * box;
-    if (t < it.hi && t + box > it.lo) page = __ldg(c.table + (long long)it.seq * c.table_stride + c.page.quot(t));
+    if (t < it.hi && t + box > it.lo) page = c.table[(long long)it.seq * c.table_stride + c.page.quot(t)];
   }
   // One tile of K or V into dst, completing on bar (one arrival). Pieces that
   // no row sees are left out: their slots hold what they held. A page outside
