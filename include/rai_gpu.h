@@ -342,8 +342,8 @@ RAI_API int rai_gpu_step_kernel_count(const rai_dec* dec, size_t* kernels);
  * device, so a step needs no host round trip and can be captured in a CUDA
  * graph; sizes here are upper bounds (max_pages columns of the table,
  * max_rows rows of a sequence). A value on the device that passes those
- * bounds is cut to them (a page number outside the pool reads as masked and
- * is not written) and reported by rai_gpu_kernel_status.
+ * bounds is cut to them (a page number outside the pool reads as keys and
+ * values of zeros and is not written) and reported by rai_gpu_kernel_status.
  *
  * All calls return as soon as their kernels are queued, allocate nothing and
  * keep nothing between calls; call them with the stream's device current.

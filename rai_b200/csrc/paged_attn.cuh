@@ -331,13 +331,16 @@ struct TilePieces {
     const bool want = any && t < it.hi && t + box > it.lo;
     const bool good = want && (unsigned)page < (unsigned)c.n_pages;
     const uint32_t at = block * (NT * 128) + piece * box * 128;
-    if (want && !good) {
-      atomicOr(c.err, kErrBadInput);
-      for (int i = 0; i < box * 8; ++i) {
-        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(dst + at + i * 16), "r"(0) : "memory");
-        if (map2) asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(dst2 + at + i * 16), "r"(0) : "memory");
+    if (__any_sync(~0u, want && !good)) {
+      if (want && !good) {
+        atomicOr(c.err, kErrBadInput);
+        for (int i = 0; i < box * 8; ++i) {
+          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(dst + at + i * 16), "r"(0) : "memory");
+          if (map2) asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(dst2 + at + i * 16), "r"(0) : "memory");
+        }
       }
       fence_async();
+      __syncwarp();  // lane 0's arrival below stands for every lane's zeros
     }
     const uint32_t n = __popc(__ballot_sync(~0u, good));
     if (lane == 0) mbar_arrive_expect_tx(bar, (map2 ? 2 : 1) * n * box * 128);

@@ -455,3 +455,30 @@ def test_pages_that_heads_share(dtype, hd, rows):
     assert ((got.double() - want).abs() <= bound).all()
     with pytest.raises(rai_b200.RaiError):
         paged.attention(q, k, v, c.table, c.kv_len, starts, max(rows), out=torch.zeros_like(q[:, :1]).expand(-1, 8, -1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("page", [8, 16, 24, 128])
+@pytest.mark.parametrize("hd,rows", [(64, [1, 2]), (128, [1, 2]), (128, [80, 2])])
+def test_pages_outside_the_pool_read_as_zeros(dtype, page, hd, rows):
+    """Also after calls whose tiles left NaN behind them in shared memory."""
+    import rai_b200
+    from rai_b200 import paged
+    dev = torch.device("cuda", 0)
+    c = ref.Cache([400, 300], 2, hd, page, dtype, dev, seed=hd, wide=40000 // page)
+    q = make_q(sum(rows), 8, hd, dtype, dev)
+    starts = ref.starts_of(rows, dev)
+    table, k, v = c.table.clone(), c.k.clone(), c.v.clone()
+    for s, cell in ((0, 1), (0, 2), (1, 0)):
+        k[c.rows[s][cell]] = 0
+        v[c.rows[s][cell]] = 0
+        table[s, cell] = -1 if cell else c.n_pages
+    want = paged.attention(q, k, v, c.table, c.kv_len, starts, max(rows))
+    paged.status()
+    junk = [torch.full_like(t, math.nan) for t in (c.k, c.v)]
+    for _ in range(4):
+        paged.attention(q, *junk, c.table, c.kv_len, starts, max(rows))
+        got = paged.attention(q, c.k, c.v, table, c.kv_len, starts, max(rows))
+        with pytest.raises(rai_b200.RaiError):
+            paged.status()
+        assert torch.equal(got, want)
