@@ -71,12 +71,15 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torc
 
 
 def rope_frequencies(rot_dim: int, theta: float = 10000.0, kind: str = "plain", *, factor: float = 1.0, low: float = 1.0,
-                     high: float = 4.0, original: float = 8192.0) -> Tuple[np.ndarray, float]:
+                     high: Optional[float] = None, original: float = 8192.0) -> Tuple[np.ndarray, float]:
     """(inv_freq, mscale) for `rope_append` (rai_rope_frequencies): kind plain,
     linear, ntk, llama3 (rai-infer/src/layers.rs:760-808) or yarn, for
-    contexts `factor` times the `original` positions."""
+    contexts `factor` times the `original` positions. `high` is 4 by default,
+    for yarn 32 (the pairs that turn more often in `original` are kept)."""
     if kind not in ROPE_KINDS:
         raise ValueError(f"kind: one of {', '.join(ROPE_KINDS)}")
+    if high is None:
+        high = 32.0 if kind == "yarn" else 4.0
     out = np.zeros(max(rot_dim, 0) // 2, np.float32)
     m = C.c_float()
     check(native.lib().rai_rope_frequencies(ROPE_KINDS[kind], rot_dim, theta, factor, low, high, original, out.ctypes.data,

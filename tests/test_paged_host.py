@@ -309,3 +309,13 @@ def test_written_rows_that_share_memory_are_refused():
     ws = L.rai_gpu_kv_resize_workspace_bytes(3)
     assert L.rai_gpu_kv_resize(C.byref(table()), C.byref(pool()), P + 4, 0, P, P, ws, None) == I
     assert "overlap" in native.last_error()
+
+
+def test_rope_frequencies_by_default():
+    """YaRN's ramp ends at 32 turns, Llama 3's at 4."""
+    from rai_b200 import paged
+    args = dict(factor=8.0, original=4096.0)
+    for kind, high in (("yarn", 32.0), ("llama3", 4.0)):
+        f, m = paged.rope_frequencies(128, 10000.0, kind, **args)
+        g, n = paged.rope_frequencies(128, 10000.0, kind, low=1.0, high=high, **args)
+        assert np.array_equal(f, g) and m == n
