@@ -112,19 +112,31 @@ def build(force: bool = False, verbose: bool = False) -> str:
 TORCH_OPS = os.path.join(HERE, "_torch_ops.so")
 
 
+def python_headers() -> str:
+    return sysconfig.get_paths()["include"]
+
+
 def build_torch_ops(force: bool = False, verbose: bool = False) -> str | None:
     """The extension behind rai_b200.paged and rai_b200.beams (csrc/
-    torch_ops.cpp), against the installed torch; None without torch."""
+    torch_ops.cpp), against the installed torch; None without torch or without
+    Python's headers, which the rest of the package does not need."""
     try:
         import torch
         from torch.utils import cpp_extension
     except ImportError:
         return None
+    if not os.path.exists(os.path.join(python_headers(), "Python.h")):
+        # Only rai_b200.paged and rai_b200.beams need it (they say so when
+        # imported); one of an earlier build may not fit this library.
+        if os.path.exists(TORCH_OPS):
+            os.remove(TORCH_OPS)
+        print("rai_b200: no Python headers, built without rai_b200.paged and rai_b200.beams", file=sys.stderr)
+        return None
     src = os.path.join(CSRC, "torch_ops.cpp")
     lib_dir = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(f"-I{p}" for p in cpp_extension.include_paths("cuda")), "-I" + sysconfig.get_paths()["include"], src,
+           *(f"-I{p}" for p in cpp_extension.include_paths("cuda")), "-I" + python_headers(), src,
            "-L" + HERE, "-l:librai_gpu.so", "-Wl,-rpath,$ORIGIN", "-L" + lib_dir, "-Wl,-rpath," + lib_dir,
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-ltorch"]
     h = hashlib.sha256((torch.__version__ + " ".join(cmd)).encode())

@@ -319,3 +319,15 @@ def test_rope_frequencies_by_default():
         f, m = paged.rope_frequencies(128, 10000.0, kind, **args)
         g, n = paged.rope_frequencies(128, 10000.0, kind, low=1.0, high=high, **args)
         assert np.array_equal(f, g) and m == n
+
+
+def test_build_without_python_headers(tmp_path, monkeypatch, capsys):
+    """The library is built; the extension is left out, an older one with it."""
+    pytest.importorskip("torch")
+    from rai_b200 import build
+    old = tmp_path / "_torch_ops.so"
+    old.write_bytes(b"of another build")
+    monkeypatch.setattr(build, "TORCH_OPS", str(old))
+    monkeypatch.setattr(build, "python_headers", lambda: str(tmp_path / "none"))
+    assert build.build_torch_ops() is None
+    assert not old.exists() and "Python headers" in capsys.readouterr().err
