@@ -334,7 +334,7 @@ py::tuple beam_select(const Tensor& logits, const Tensor& scores, std::optional<
   need(logits.dim() == 3, "logits: [batch, beams, vocab]");
   const int64_t b = logits.size(0), n = logits.size(1), v = logits.size(2), keep = keep_in ? *keep_in : 2 * n;
   need(b > 0 && n > 0 && v > 0, "logits: a size is zero");
-  need(keep > 0, "keep");
+  need(keep >= n && keep <= 64, "keep: from beams to 64");  // before outputs of that size are made
   need(v == 1 || logits.stride(2) == 1, "logits: vocab has to be contiguous");
   const int64_t row = n > 1 ? logits.stride(1) : b > 1 ? logits.stride(0) : v;
   need(n == 1 || b == 1 || logits.stride(0) == n * row, "logits: rows have to be evenly spaced");

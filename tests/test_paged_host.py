@@ -331,3 +331,11 @@ def test_build_without_python_headers(tmp_path, monkeypatch, capsys):
     monkeypatch.setattr(build, "python_headers", lambda: str(tmp_path / "none"))
     assert build.build_torch_ops() is None
     assert not old.exists() and "Python headers" in capsys.readouterr().err
+
+
+@pytest.mark.parametrize("keep", [0, 2, 65, 1 << 40])
+def test_beams_refuse_keep_before_they_allocate(keep):
+    torch = pytest.importorskip("torch")
+    from rai_b200 import beams
+    with pytest.raises(ValueError, match="keep"):
+        beams.select(torch.zeros(1, 3, 9), torch.zeros(1, 3), keep=keep)
