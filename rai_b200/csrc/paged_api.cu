@@ -107,7 +107,8 @@ int attention_args(const rai_paged_attention* a, rai::AttnArgs* out) {
   if (!apart(a->chunk.head_dim, {{a->out_row, a->chunk.rows}, {a->out_head, a->n_heads}})) return bad("out: rows share memory");
   if ((uint64_t)a->chunk.n_seqs * (((uint64_t)a->chunk.max_rows * (a->n_heads / a->chunk.n_kv_heads) + 15) / 16) > (1u << 30))
     return bad("n_seqs * max_rows is out of range");
-  if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return bad("scale has to be positive");
+  // (The kernels use scale * log2(e).)
+  if (!(a->scale > 0.f) || !std::isfinite(a->scale * 1.4426950408889634f)) return bad("scale has to be positive, up to 2.3e38");
   if (!(a->softcap == 0.f || std::isnormal(a->softcap)) || a->softcap < 0.f) return bad("softcap: 0, or a positive normal number");
   if (a->window > (1u << 30)) return bad("window");
   o.q = a->q, o.out = a->out, o.lse = a->lse;

@@ -339,3 +339,8 @@ def test_beams_refuse_keep_before_they_allocate(keep):
     from rai_b200 import beams
     with pytest.raises(ValueError, match="keep"):
         beams.select(torch.zeros(1, 3, 9), torch.zeros(1, 3), keep=keep)
+
+
+def test_attention_refuses_scales_whose_product_overflows():
+    for scale in (2.4e38, 3.4e38):
+        assert attn(scale=scale) == I and "scale" in native.last_error()
