@@ -465,8 +465,11 @@ __global__ void __launch_bounds__(kThreads)
       for (int x = 0; x < NTW / 8; ++x) top = fmaxf(top, fmaxf(s[x][2 * h], s[x][2 * h + 1]));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-      const float mc = top == -INFINITY ? 0.f : top * p.c;
-      const float fix = exp2_fast(m[h] * p.c - mc);  // m = -inf: 0
+      // Both products rounded before their difference: fused, a maximum that
+      // stays would rescale by its own rounding at every tile (at 20,000 tokens
+      // f32 outputs were off by 1.8e-5 so).
+      const float mc = top == -INFINITY ? 0.f : __fmul_rn(top, p.c);
+      const float fix = exp2_fast(__fmul_rn(m[h], p.c) - mc);  // m = -inf: 0
       m[h] = top;
       float sum = 0.f;
 #pragma unroll
@@ -550,11 +553,11 @@ __global__ void __launch_bounds__(kThreads)
             w[x] = *reinterpret_cast<const float2*>(ml + ((wm + x * C::WM) * 16 + g + 8 * h) * 2);
             top = fmaxf(top, w[x].x);
           }
-          const float mc = top == -INFINITY ? 0.f : top * p.c;
+          const float mc = top == -INFINITY ? 0.f : __fmul_rn(top, p.c);
           float sum = 0.f;
 #pragma unroll
-          for (int x = 0; x < WN; ++x) sum += w[x].y * exp2_fast(w[x].x * p.c - mc);
-          const float fix = exp2_fast(m[h] * p.c - mc);
+          for (int x = 0; x < WN; ++x) sum += w[x].y * exp2_fast(__fmul_rn(w[x].x, p.c) - mc);
+          const float fix = exp2_fast(__fmul_rn(m[h], p.c) - mc);
           m[h] = top;
           l[h] = sum;
 #pragma unroll

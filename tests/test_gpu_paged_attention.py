@@ -482,3 +482,35 @@ def test_pages_outside_the_pool_read_as_zeros(dtype, page, hd, rows):
         with pytest.raises(rai_b200.RaiError):
             paged.status()
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.float32, 64), (torch.float32, 128), (torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float16, 64)], ids=str)
+def test_weights_do_not_drift_along_a_context(dtype, hd):
+    """Equal scores of several hundred: each token's weight is the same however
+    many tiles lie behind it. Values of 1 in the first half and -1 in the second
+    cancel."""
+    from rai_b200 import paged
+    dev = torch.device("cuda", 0)
+    n, seqs, page, H = 100_000, 150, 100 if hd == 64 else 128, 4
+    n = n // (2 * page) * 2 * page
+    pages = n // page
+    k = torch.full((pages, 1, page, hd), 2.0 ** -4, dtype=dtype, device=dev)
+    v = torch.ones((pages, 1, page, hd), dtype=dtype, device=dev)
+    v[pages // 2:, :, :, ::2] = -1
+    q = torch.empty((seqs, H, hd), dtype=dtype, device=dev)
+    for h in range(H):
+        q[:, h] = 180.0 + 7 * h  # (exact in every type)
+    table = torch.arange(pages, dtype=torch.int32, device=dev).expand(seqs, pages).contiguous()
+    lens = torch.full((seqs,), n, dtype=torch.int32, device=dev)
+    lse = torch.zeros((seqs, H), device=dev)
+    scale = 0.7137
+    got = paged.attention(q, k, v, table, lens, torch.arange(seqs + 1, dtype=torch.int32, device=dev), 1, scale=scale, lse=lse)
+    paged.status()
+    score = scale * hd * q[0, :, 0].double() * 2.0 ** -4  # 514 to 574
+    # Sums of n / 3 equal terms in f32, by threads that add some hundred tiles
+    # of up to 32 terms: 2^-24 of the sum for each addition, 2^13 of them. The
+    # score is rounded twice, times log2(e) once more.
+    tol = 2.0 ** -11
+    assert ((lse.double() - (score + math.log(n))).abs() <= tol + score * 2.0 ** -21).all()
+    assert (got[:, :, ::2].double().abs() <= tol).all()
+    assert ((got[:, :, 1::2].double() - 1).abs() <= tol + ref.EPS[dtype]).all()
