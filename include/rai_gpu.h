@@ -256,7 +256,10 @@ RAI_API int rai_gpu_w4a8_matmul(float* out, const void* packed, const float* inp
  * gave up since the last query (that call's output is incomplete),
  * RAI_ERR_INVALID if a paged-cache or beam call met a value on the device
  * (a page number, length, row range or parent) outside its tensors, else
- * RAI_OK. The status word is per device and cleared by the query. */
+ * RAI_OK. The status word is per device, shared by every thread and stream and
+ * by all kernel-level calls, and cleared by the query: a report says that some
+ * call did, not which. Hosts with several callers on a device query in one
+ * place, behind the calls they ask about. */
 RAI_API int rai_gpu_kernel_status(void* stream);
 
 /* The same linear on the tcgen05 tensor cores (w4a8_matmul,

@@ -15,10 +15,16 @@
 // odd tiles of an item, and A joins the two at the item's end.
 //
 // Per tile of 256 rows and head size 128 that is 2,048 cycles of tensor core
-// and, at 16 exponentials a cycle, 2,048 cycles of the special function units,
-// so both bound it. With few rows HBM bounds it: a tile's K and V are 64 KB,
+// and, at 16 exponentials a cycle, 2,048 cycles of the special function units
+// (1.1 us); a tile takes 2.1 to 2.4 us, the rest being the way S -> registers
+// -> P that the halves do not wholly hide from each other. With few rows HBM bounds it: a tile's K and V are 64 KB,
 // 1.45 us of an SM's share of the bandwidth, against 0.55 us of tensor core;
 // warps whose rows do not exist skip the softmax.
+//
+// (Two row halves in turn, P in place of S and a maximum that seldom moves are
+// a published arrangement of attention for these tensor cores; the line of
+// tiles, the paged loads, the form for few rows and the handling of masked V
+// are this file's own.)
 //
 // The running maximum is lazy: m only moves (and O is only rescaled, in TMEM)
 // when a row's maximum passes it by more than 2^8; until then probabilities
@@ -72,9 +78,13 @@ struct Tc {
 constexpr float kLazy = 8.f;  // log2 units
 // Few rows and heads wider than 64: from how many tokens a sequence, and a
 // call's sequences and KV heads together, can have this kernel is the faster
-// one. (8 KV heads of 128: 256 x 1,000 tokens 305 us here and 404 us on
-// mma.sync, 16 x 2,000 73 / 83, 1 x 16,000 56 / 61; 64 x 1,000 134 / 136,
-// 256 x 300 167 / 162, 1 x 1,500 52 / 42. Heads of 64, 64 x 8,000: 233 / 120.)
+// one. (Device time, calls in a captured graph, one row a sequence, tables as
+// wide as the sequences; 8 KV heads of 128: 256 x 1,000 tokens 302 us here and
+// 430 us on mma.sync, 64 x 2,000 151 / 213, 64 x 1,000 104 / 115, 16 x 2,000
+// 50 / 61; 16 x 1,000 36 / 35, 1 x 16,000 39 / 38, 64 x 700 89 / 85, 1 x 4,000
+// 34 / 20; 256 x 300 143 / 156 goes the slower way. Heads of 64, 64 x 2,000:
+// 67 / 32.) The host knows the table's width, not the lengths: short sequences
+// in a wide table come here too.
 constexpr long long kTcFewRowsTokens = 768, kTcFewRowsTotal = 131072;
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -812,13 +822,14 @@ cudaError_t launch(const AttnArgs& a, const KvMaps& maps, int box, cudaStream_t 
   p.grid = device_sm_count();
   p.whole = p.direct = false;
   p.min_tiles = 10;
-  // An item costs about 5 us beside its tiles of 1.8 us: three prompts of
-  // 3,000 tokens take 325 / 324 / 329 / 342 us at 2 / 3 / 4 / 6.
+  // An item costs about 7 us beside its tiles of 2.1 us (capped ones take 4.9
+  // us): three prompts of 3,000 tokens take 280 / 278 / 280 / 290 us at 2 / 3 /
+  // 4 / 6, the capped chunks 162 / 163 / 162 / 165.
   p.item_cost = 3;
   p.c = a.softcap > 0.f ? kLog2e : a.scale * kLog2e;
   p.inv_cap = a.softcap > 0.f ? 1.f / a.softcap : 0.f;
   // Not launched ahead of its predecessor's end: a batch of prompts took 344
-  // us so and 357 us with it (long verification: 165 either way).
+  // us so and 357 us with it when that was tried, long verification the same.
   paged_attn_tc_kernel<C, CAP, TMA><<<p.grid, kTcThreads, C::kSmem, s>>>(p, maps, box, q_map, q_tma);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;

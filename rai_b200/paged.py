@@ -125,7 +125,9 @@ def copy_pages(k: torch.Tensor, v: torch.Tensor, src: torch.Tensor, dst: torch.T
 def status(device=None) -> None:
     """Wait for the current stream and raise RaiError if a kernel-level call
     since the last query met a value on the device outside its tensors, or a
-    device wait that gave up (rai_gpu_kernel_status)."""
+    device wait that gave up (rai_gpu_kernel_status). One word per device, that
+    all threads and streams share: a report may be about another caller's call,
+    and is not given twice."""
     with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
         check(native.lib().rai_gpu_kernel_status(torch.cuda.current_stream().cuda_stream))
 
