@@ -17,9 +17,10 @@
 // Per tile of 256 rows and head size 128 that is 2,048 cycles of tensor core
 // and, at 16 exponentials a cycle, 2,048 cycles of the special function units
 // (1.1 us); a tile takes 2.1 to 2.4 us, the rest being the way S -> registers
-// -> P that the halves do not wholly hide from each other. With few rows HBM bounds it: a tile's K and V are 64 KB,
-// 1.45 us of an SM's share of the bandwidth, against 0.55 us of tensor core;
-// warps whose rows do not exist skip the softmax.
+// -> P that the halves do not wholly hide from each other. With few rows HBM
+// bounds it: a tile's K and V are 64 KB, 1.45 us of an SM's share of the
+// bandwidth, against 0.55 us of tensor core; warps whose rows do not exist
+// skip the softmax.
 //
 // (Two row halves in turn, P in place of S and a maximum that seldom moves are
 // a published arrangement of attention for these tensor cores; the line of
